@@ -42,7 +42,7 @@ extern "C" {
 #define TGAF_ERR_NCCL 4
 #define TGAF_ERR_UNSUPPORTED 5
 #define TGAF_ERR_TIMEOUT 6
-#define TGAF_ERR_DEVICE_FLAG 7 /* a kernel's bounded wait ran out and set its error word */
+#define TGAF_ERR_DEVICE_FLAG 7 /* a kernel set its error word: a bounded wait ran out, or (tgaf_kv_*, tgaf_attention*) a bad block table */
 
 /* scales dtype tags: core/src/compute/cuda/gaffine_u4_matvec.zig:13-14 */
 #define TGAF_SCALES_F16 0u
@@ -265,6 +265,81 @@ int32_t tgaf_dequant_f32_host(tgaf_ctx *ctx, const tgaf_weight *w, float *h_out)
  * is enqueued: an id >= N is TGAF_ERR_INVALID_ARGUMENT (the reference's error.InvalidTokenId). */
 int32_t tgaf_embedding_lookup_f32(tgaf_ctx *ctx, const tgaf_weight *w, const uint32_t *token_ids,
                                   uint32_t count, float multiplier, float *d_out);
+
+/* ---- the quantised KV cache and its attention --------------------------------
+ * What a decoder runs between its qkv linear and its o linear.  Replaces the KV store and decode attention kernels of
+ * the reference's CUDA backend (talu_kv_write_f16, core/src/compute/cuda/kernels/ops/norm_rope_ops.cu:164;
+ * talu_attn_scores_heads_f16_kv / talu_softmax_rows_f32 / talu_attn_weighted_sum_heads_f16_kv /
+ * talu_attn_fused_heads_f16_kv, kernels/ops/attention_ops.cu:20-215), whose cache is dense f16 and holds one sequence.
+ * Here the cache is paged and its rows are grouped-affine codes like the weights': for every cached token, K or V and
+ * head, head_dim codes of 4 or 8 bits and per group one bf16 scale and one bf16 bias.
+ *
+ *   packed  u32 [pages][2][kv_heads][page_tokens][head_dim*bits/32]   index 0 of the second axis: K, 1: V
+ *   scales  u16 [pages][2][kv_heads][page_tokens][head_dim/group]     bf16
+ *   biases  u16 [pages][2][kv_heads][page_tokens][head_dim/group]     bf16
+ *   value = f32(code) * f32(scale) + f32(bias)                        one rounding (fused multiply-add)
+ *
+ * The quantiser of a group of values x: bias = bf16(min x), scale = bf16((max x - min x) / (2^bits - 1)), 0 where that is
+ * below the smallest normal number, code = clamp(rint((x - bias) / scale), 0, 2^bits - 1), all in f32 with ties to even;
+ * the codes are taken against the stored (rounded) scale and bias, so a value is off by half a step at most wherever the
+ * rounded scale reaches it.  A group that holds an infinity or a NaN reads back as NaN.
+ * bits in {4, 8}; group in {32, 64, 128}; head_dim a multiple of group, at most 256; page_tokens in {16, 32, 64, 128, 256};
+ * pages * 2 * kv_heads * page_tokens < 2^31.  The three buffers are the caller's device memory (16-byte aligned), are not
+ * copied and must outlive the cache; the kernels read nothing of rows that no sequence reaches. */
+typedef struct tgaf_kv_cache tgaf_kv_cache;
+int32_t tgaf_kv_cache_wrap_device(tgaf_ctx *ctx, void *d_packed, void *d_scales, void *d_biases, uint64_t pages,
+                                  uint32_t kv_heads, uint32_t page_tokens, uint32_t head_dim, uint32_t group_size,
+                                  uint32_t bits, tgaf_kv_cache **out_cache);
+int32_t tgaf_kv_cache_free(tgaf_ctx *ctx, tgaf_kv_cache *cache);
+
+/* The sequences of a call; all arrays on the device, so that a captured call follows them from replay to replay.
+ *   d_table  i32 [batch][table_width], rows table_stride elements apart: page of the sequence's tokens
+ *            [i*page_tokens, (i+1)*page_tokens); entries behind a sequence's last page are not read
+ *   d_lens   i32 [batch]      cached tokens of each sequence, the call's own included
+ *   d_cu     i32 [batch + 1]  the call's own tokens of sequence b are rows [d_cu[b], d_cu[b+1]) of its packed tensors and the
+ *            LAST ones of the sequence; non-decreasing, d_cu[0] = 0.  NULL: total / batch tokens of each sequence.
+ *   total    rows of the packed tensors; rows from d_cu[batch] on are left as they were
+ * A row whose position would be negative (more own tokens than d_lens has) is not stored, not read back and sees no key.
+ * A table entry outside the cache, or a length beyond the table's width: the tokens in question are skipped (not stored, read
+ * back or seen) and the next tgaf_synchronize returns TGAF_ERR_DEVICE_FLAG. */
+typedef struct tgaf_kv_seqs {
+    const int32_t *d_table;
+    uint64_t table_stride;
+    uint32_t table_width;
+    uint32_t batch;
+    const int32_t *d_lens;
+    const int32_t *d_cu;
+    uint32_t total;
+} tgaf_kv_seqs;
+
+/* Quantises the call's own rows k, v [total, kv_heads, head_dim] (device, f32 or bf16: TGAF_DTYPE_*; strides in elements,
+ * head_dim contiguous, so that slices of a fused qkv output need no copy) into the sequences' pages.  A page must not be
+ * written for two sequences by one call (which row is kept there is not defined). */
+int32_t tgaf_kv_append(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *seqs, uint32_t dtype, const void *k,
+                       uint64_t k_token_stride, uint64_t k_head_stride, const void *v, uint64_t v_token_stride,
+                       uint64_t v_head_stride);
+/* The inverse: the same rows read back, f32 or rounded once to bf16. */
+int32_t tgaf_kv_read(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *seqs, uint32_t dtype, void *k,
+                     uint64_t k_token_stride, uint64_t k_head_stride, void *v, uint64_t v_token_stride,
+                     uint64_t v_head_stride);
+
+/* out[t, h] = sum_j softmax_j(scale * q[t, h] . K[j, h / (q_heads / kv_heads)]) V[j, ...] over the cached tokens j of t's
+ * sequence up to t itself (causal; the sequence's tokens are appended first).  q, out: f32 or bf16
+ * [total, q_heads, head_dim], strides in elements, head_dim contiguous; out must not overlap q.  f32 statistics and sums.
+ * max_new: an upper bound of the own tokens of any sequence (the launch is sized by it; a sequence with more sets the
+ * error word and its rows from max_new on are left as they were).  A row that sees no key gives 0.
+ * The partial results of long sequences lie in a workspace of the context, made with its first cache: calls captured into
+ * graphs must not be replayed at the same time as other attention calls of the same context (one context per stream). */
+int32_t tgaf_attention(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *seqs, uint32_t dtype, const void *q,
+                       uint64_t q_token_stride, uint64_t q_head_stride, uint32_t q_heads, uint32_t max_new, float scale,
+                       void *out, uint64_t out_token_stride, uint64_t out_head_stride);
+/* The same where every sequence continues one shared prefix of prefix_len tokens, in the pages d_prefix_table
+ * i32 [ceil(prefix_len / page_tokens)]: every row sees the whole prefix, then its own sequence's tokens as above (d_lens and
+ * d_table do not count the prefix).  The prefix is read once for all rows of the batch instead of once per sequence. */
+int32_t tgaf_attention_shared_prefix(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const int32_t *d_prefix_table,
+                                     uint32_t prefix_len, const tgaf_kv_seqs *seqs, uint32_t dtype, const void *q,
+                                     uint64_t q_token_stride, uint64_t q_head_stride, uint32_t q_heads, uint32_t max_new,
+                                     float scale, void *out, uint64_t out_token_stride, uint64_t out_head_stride);
 
 /* ---- the SwiGLU FFN as one operator ---------------------------------------
  * y[m, d_model] = down( silu(gate(x)) * up(x) ), the body of SwiGLU.forward

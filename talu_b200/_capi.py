@@ -43,6 +43,12 @@ SIGNATURES = {
     "tgaf_dequant_f32": (_i32, [_vp, _vp, _vp]),
     "tgaf_dequant_f32_host": (_i32, [_vp, _vp, _vp]),
     "tgaf_embedding_lookup_f32": (_i32, [_vp, _vp, _vp, _u32, C.c_float, _vp]),
+    "tgaf_kv_cache_wrap_device": (_i32, [_vp, _vp, _vp, _vp, _u64, _u32, _u32, _u32, _u32, _u32, _pp]),
+    "tgaf_kv_cache_free": (_i32, [_vp, _vp]),
+    "tgaf_kv_append": (_i32, [_vp, _vp, _vp, _u32, _vp, _u64, _u64, _vp, _u64, _u64]),
+    "tgaf_kv_read": (_i32, [_vp, _vp, _vp, _u32, _vp, _u64, _u64, _vp, _u64, _u64]),
+    "tgaf_attention": (_i32, [_vp, _vp, _vp, _u32, _vp, _u64, _u64, _u32, _u32, C.c_float, _vp, _u64, _u64]),
+    "tgaf_attention_shared_prefix": (_i32, [_vp, _vp, _vp, _u32, _vp, _u32, _vp, _u64, _u64, _u32, _u32, C.c_float, _vp, _u64, _u64]),
     "tgaf_comm_make_id": (_i32, [_vp]),
     "tgaf_comm_init": (_i32, [_vp, _vp, _u32, _u32]),
     "tgaf_comm_destroy": (_i32, [_vp]),
@@ -60,6 +66,14 @@ SIGNATURES = {
     "tgaf_batch_uses_one_launch": (_i32, [_vp]),
     "tgaf_batch_destroy": (_i32, [_vp, _vp]),
 }
+
+
+
+class KvSeqs(C.Structure):
+    """tgaf_kv_seqs: the sequences of a call on the quantised KV cache"""
+    _fields_ = [("d_table", C.c_void_p), ("table_stride", C.c_uint64), ("table_width", C.c_uint32), ("batch", C.c_uint32),
+                ("d_lens", C.c_void_p), ("d_cu", C.c_void_p), ("total", C.c_uint32)]
+
 
 # tgaf_watch_fns: the three hooks of tgaf_watchdog_wait
 WORK_DONE_FN = C.CFUNCTYPE(C.c_int32, C.c_void_p)

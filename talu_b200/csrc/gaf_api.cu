@@ -157,6 +157,10 @@ struct tgaf_host_batch {
     uint8_t *d_x = nullptr, *d_y = nullptr;
 };
 
+struct tgaf_kv_cache {
+    KvView v;
+};
+
 struct tgaf_weight {
     WeightView v;
     bool owns = false;
@@ -367,6 +371,54 @@ int32_t raw_matvec(tgaf_ctx *ctx, uint32_t bits, const float *input, const uint3
     const int slot = ctx->raw_cache_used < tgaf_ctx::kRawCache ? ctx->raw_cache_used++ : (ctx->raw_cache_next++ % tgaf_ctx::kRawCache);
     ctx->raw_cache[slot] = v;
     return linear_device(ctx, ctx->raw_cache[slot], input, batch_rows, out, true);
+}
+
+// Checks shared by the cache's entry points, and the sequences as the kernels take them.
+int32_t kv_seqs(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *in, uint32_t dtype, const void *a, const void *b,
+                KvSeqs *out) {
+    if (!ctx) return TGAF_ERR_INVALID_ARGUMENT;
+    if (!cache || !in) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "null cache or sequences");
+    if (dtype != TGAF_DTYPE_F32 && dtype != TGAF_DTYPE_BF16) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "bad dtype %u", dtype);
+    *out = {in->d_table, in->table_stride, in->table_width, in->batch, in->d_lens, in->d_cu, in->total, 1u};
+    if (in->total == 0) return TGAF_OK;
+    if (in->batch == 0) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "rows without a sequence");
+    if (!in->d_table || !in->d_lens || !a || !b) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "null device pointer");
+    if (in->table_width == 0 || in->table_stride < in->table_width) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "bad table width %u", in->table_width);
+    if (in->batch > 0x7FFFFFFEu || static_cast<uint64_t>(in->total) * cache->v.kv_heads * cache->v.head_dim / 4 / 256 >= 0x7FFFFFFFull)
+        return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "too many rows: %u", in->total);
+    if (!in->d_cu) {
+        if (in->total % in->batch != 0) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "%u rows are no equal share of %u sequences", in->total, in->batch);
+        out->per = in->total / in->batch;
+    }
+    return TGAF_OK;
+}
+
+int32_t attend(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const int32_t *prefix_table, uint32_t prefix_len,
+               const tgaf_kv_seqs *seqs, uint32_t dtype, const void *q, KvStrides qs, uint32_t q_heads, uint32_t max_new,
+               float scale, void *out, KvStrides os) {
+    AttnArgs a;
+    const int32_t st = kv_seqs(ctx, cache, seqs, dtype, q, out, &a.seqs);
+    if (st != TGAF_OK) return st;
+    a.kv = cache->v;
+    if (q_heads == 0 || q_heads % a.kv.kv_heads != 0)
+        return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "%u query heads are no multiple of %u cached heads", q_heads, a.kv.kv_heads);
+    if (!(scale - scale == 0.0f)) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "scale must be finite");
+    if (a.seqs.total == 0) return TGAF_OK;
+    if (max_new == 0 || (!a.seqs.cu && a.seqs.per > max_new)) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "max_new %u is below the rows of a sequence", max_new);
+    if (static_cast<uint64_t>(a.seqs.total) * q_heads > 0x7FFFFFFFull) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "too many query rows");
+    a.prefix_table = prefix_table;
+    a.prefix_len = prefix_len;
+    a.q = q;
+    a.out = out;
+    a.qs = qs;
+    a.os = os;
+    a.q_heads = q_heads;
+    a.max_new = max_new < a.seqs.total ? max_new : a.seqs.total;
+    a.scale = scale;
+    a.error_word = ctx->d_error_word;
+    TGAF_CUDA(ctx, cudaSetDevice(ctx->device));
+    const cudaError_t e = attention_generic(a, dtype == TGAF_DTYPE_F32, ctx->stream);
+    return e == cudaSuccess ? TGAF_OK : cuda_fail(ctx, e, "attention launch");
 }
 
 }  // namespace
@@ -682,6 +734,8 @@ int32_t tgaf_synchronize(tgaf_ctx *ctx) {
             if (b->list) gemv_list_reset(b->list);
             if (b->tagged) cudaMemset(b->tagged, 0, b->tagged_bytes);
         }
+        if (flag & kKvBadTable) return fail(ctx, TGAF_ERR_DEVICE_FLAG, "a block table named a page outside the cache, or a length was beyond its table");
+        if (flag & kKvBadCount) return fail(ctx, TGAF_ERR_DEVICE_FLAG, "a sequence had more new tokens than max_new");
         return fail(ctx, TGAF_ERR_DEVICE_FLAG, "a kernel gave up a bounded wait (code 0x%x)", flag);
     }
     return TGAF_OK;
@@ -1531,6 +1585,94 @@ int32_t tgaf_linear_bf16_allreduce(tgaf_ctx *ctx, const tgaf_weight *w, const vo
     if (!ctx->comm) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "no communicator: call tgaf_comm_init first");
     cudaSetDevice(ctx->device);
     return linear_device(ctx, w->v, x_bf16, m, y_bf16, false, true);
+}
+
+// ---- quantised KV cache ----
+
+int32_t tgaf_kv_cache_wrap_device(tgaf_ctx *ctx, void *d_packed, void *d_scales, void *d_biases, uint64_t pages,
+                                  uint32_t kv_heads, uint32_t page_tokens, uint32_t head_dim, uint32_t group_size,
+                                  uint32_t bits, tgaf_kv_cache **out_cache) {
+    if (!out_cache) return TGAF_ERR_INVALID_ARGUMENT;
+    *out_cache = nullptr;
+    if (!ctx) return TGAF_ERR_INVALID_ARGUMENT;
+    if (!d_packed || !d_scales || !d_biases) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "null cache pointer");
+    if (bits != 4 && bits != 8) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "bits must be 4 or 8");
+    if (group_size != 32 && group_size != 64 && group_size != 128) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "group must be 32, 64 or 128");
+    if (head_dim == 0 || head_dim % group_size != 0 || head_dim > 256) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "head_dim must be a multiple of the group, at most 256");
+    if (page_tokens < 16 || page_tokens > 256 || (page_tokens & (page_tokens - 1)) != 0)
+        return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "page_tokens must be 16, 32, 64, 128 or 256");
+    if (pages == 0 || kv_heads == 0 || kv_heads > 65535 || pages > 0x7FFFFFFFull || pages * 2 * kv_heads > 0x7FFFFFFFull / page_tokens)
+        return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "bad cache size: pages=%llu kv_heads=%u page_tokens=%u", (unsigned long long)pages, kv_heads, page_tokens);
+    if ((reinterpret_cast<uintptr_t>(d_packed) | reinterpret_cast<uintptr_t>(d_scales) | reinterpret_cast<uintptr_t>(d_biases)) % 16 != 0)
+        return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "cache buffers must be 16-byte aligned");
+    tgaf_kv_cache *c = new (std::nothrow) tgaf_kv_cache();
+    if (!c) return fail(ctx, TGAF_ERR_OUT_OF_MEMORY, "host allocation failed");
+    KvView &v = c->v;
+    v.packed = static_cast<uint8_t *>(d_packed);
+    v.scales = static_cast<uint16_t *>(d_scales);
+    v.biases = static_cast<uint16_t *>(d_biases);
+    v.pages = static_cast<uint32_t>(pages);
+    v.kv_heads = kv_heads;
+    v.page_tokens = page_tokens;
+    v.page_shift = 0;
+    while ((1u << v.page_shift) < page_tokens) ++v.page_shift;
+    v.head_dim = head_dim;
+    v.group = group_size;
+    v.group_shift = group_size == 32 ? 5 : group_size == 64 ? 6 : 7;
+    v.groups = head_dim / group_size;
+    v.bits = bits;
+    v.row_bytes = head_dim * bits / 8;
+    *out_cache = c;
+    return TGAF_OK;
+}
+
+int32_t tgaf_kv_cache_free(tgaf_ctx *ctx, tgaf_kv_cache *cache) {
+    if (!cache) return TGAF_OK;
+    if (!ctx) return TGAF_ERR_INVALID_ARGUMENT;
+    delete cache;   // nothing on the device belongs to it; launches in flight hold copies of what they need
+    return TGAF_OK;
+}
+
+int32_t tgaf_kv_append(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *seqs, uint32_t dtype, const void *k,
+                       uint64_t k_token_stride, uint64_t k_head_stride, const void *v, uint64_t v_token_stride,
+                       uint64_t v_head_stride) {
+    KvSeqs s;
+    const int32_t st = kv_seqs(ctx, cache, seqs, dtype, k, v, &s);
+    if (st != TGAF_OK || s.total == 0) return st;
+    TGAF_CUDA(ctx, cudaSetDevice(ctx->device));
+    const cudaError_t e = kv_append(cache->v, s, dtype == TGAF_DTYPE_F32, k, {k_token_stride, k_head_stride}, v,
+                                    {v_token_stride, v_head_stride}, ctx->d_error_word, ctx->stream);
+    return e == cudaSuccess ? TGAF_OK : cuda_fail(ctx, e, "kv_append launch");
+}
+
+int32_t tgaf_kv_read(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *seqs, uint32_t dtype, void *k,
+                     uint64_t k_token_stride, uint64_t k_head_stride, void *v, uint64_t v_token_stride,
+                     uint64_t v_head_stride) {
+    KvSeqs s;
+    const int32_t st = kv_seqs(ctx, cache, seqs, dtype, k, v, &s);
+    if (st != TGAF_OK || s.total == 0) return st;
+    TGAF_CUDA(ctx, cudaSetDevice(ctx->device));
+    const cudaError_t e = kv_read(cache->v, s, dtype == TGAF_DTYPE_F32, k, {k_token_stride, k_head_stride}, v,
+                                  {v_token_stride, v_head_stride}, ctx->d_error_word, ctx->stream);
+    return e == cudaSuccess ? TGAF_OK : cuda_fail(ctx, e, "kv_read launch");
+}
+
+int32_t tgaf_attention(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *seqs, uint32_t dtype, const void *q,
+                       uint64_t q_token_stride, uint64_t q_head_stride, uint32_t q_heads, uint32_t max_new, float scale,
+                       void *out, uint64_t out_token_stride, uint64_t out_head_stride) {
+    return attend(ctx, cache, nullptr, 0, seqs, dtype, q, {q_token_stride, q_head_stride}, q_heads, max_new, scale, out,
+                  {out_token_stride, out_head_stride});
+}
+
+int32_t tgaf_attention_shared_prefix(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const int32_t *d_prefix_table,
+                                     uint32_t prefix_len, const tgaf_kv_seqs *seqs, uint32_t dtype, const void *q,
+                                     uint64_t q_token_stride, uint64_t q_head_stride, uint32_t q_heads, uint32_t max_new,
+                                     float scale, void *out, uint64_t out_token_stride, uint64_t out_head_stride) {
+    if (!ctx) return TGAF_ERR_INVALID_ARGUMENT;
+    if (prefix_len != 0 && !d_prefix_table) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "null prefix table");
+    if (prefix_len > 0x7FFFFFFFu) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "prefix_len %u too large", prefix_len);
+    return attend(ctx, cache, prefix_len ? d_prefix_table : nullptr, prefix_len, seqs, dtype, q, {q_token_stride, q_head_stride},
+                  q_heads, max_new, scale, out, {out_token_stride, out_head_stride});
 }
 
 }  // extern "C"

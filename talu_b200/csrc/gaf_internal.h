@@ -130,6 +130,46 @@ bool gemm_tc_eligible(const WeightView &w, uint32_t M, uint32_t min_m = 17u);
 size_t gemm_tc_workspace_bytes(int sm_count);
 size_t gemm_tc_flag_count(int sm_count);
 
+// ---- quantised KV cache and its attention (gaf_kv.cu) ----
+// The pages as the kernels see them; rows are numbered ((page * 2 + which) * kv_heads + head) * page_tokens + token.
+struct KvView {
+    uint8_t *packed;    // [rows][row_bytes]
+    uint16_t *scales;   // [rows][groups] bf16
+    uint16_t *biases;
+    uint32_t pages, kv_heads, page_tokens, page_shift;   // page_tokens = 1 << page_shift
+    uint32_t head_dim, group, group_shift, groups, bits, row_bytes;
+};
+struct KvSeqs {
+    const int32_t *table;
+    uint64_t table_stride;
+    uint32_t width, batch;
+    const int32_t *lens, *cu;   // cu == null: `per` own tokens of each sequence
+    uint32_t total, per;
+};
+struct KvStrides {
+    uint64_t token, head;   // elements
+};
+struct AttnArgs {
+    KvView kv;
+    KvSeqs seqs;
+    const int32_t *prefix_table;   // null: no shared prefix
+    uint32_t prefix_len;
+    const void *q;
+    void *out;
+    KvStrides qs, os;
+    uint32_t q_heads, max_new;
+    float scale;
+    unsigned int *error_word;
+};
+// bits of the error word
+constexpr unsigned int kKvBadTable = 0x40000000u;   // a table entry outside the cache, or a length beyond the table
+constexpr unsigned int kKvBadCount = 0x20000000u;   // a sequence with more own tokens than max_new
+cudaError_t kv_append(const KvView &kv, const KvSeqs &seqs, bool f32, const void *k, KvStrides ks, const void *v, KvStrides vs,
+                      unsigned int *error_word, cudaStream_t stream);
+cudaError_t kv_read(const KvView &kv, const KvSeqs &seqs, bool f32, void *k, KvStrides ks, void *v, KvStrides vs,
+                    unsigned int *error_word, cudaStream_t stream);
+cudaError_t attention_generic(const AttnArgs &a, bool f32, cudaStream_t stream);
+
 // ---- all-reduce over NVLink peer memory (gaf_peer.cu) ----
 constexpr int kPeerMaxRanks = 8;                      // ranks of one node
 constexpr int kPeerCtas = 16;                         // CTAs of the all-reduce kernel (always all launched)

@@ -1,0 +1,353 @@
+// The quantised KV cache: rows written (quantised) into their pages and read back, and the attention over it for head
+// sizes that the tensor-core kernel does not take.
+//
+// A group of G values x along head_dim is stored as codes q, a bf16 scale s and a bf16 bias b:
+//   b = bf16(min x),  s = bf16((max x - min x) / maxq),  q = clamp(rint((x - b) / s), 0, maxq),  value = q s + b
+// b is exact for bf16 inputs (the minimum is one of them).  s and b are rounded to nearest once, because 16 bits each is
+// what the format stores; the codes are taken against the rounded pair, which makes the rounding of s part of the grid and
+// not an error of every value: only the top value can be off by more than half a step, (max x - min x) 2^-9 + s / 2.
+// Differences are formed of halves (0.5 x - 0.5 b), which is exact scaling, so that no finite input overflows.
+#include "gaf_internal.h"
+
+#include <cuda_bf16.h>
+
+#include <cfloat>
+
+namespace tgaf {
+namespace {
+
+constexpr int kThreadsKv = 256;
+
+__device__ __forceinline__ float bf16_f32(uint32_t raw) { return __uint_as_float(raw << 16); }
+__device__ __forceinline__ uint32_t f32_bf16(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Sequence of packed row t, or -1 for a row behind the last sequence.
+__device__ __forceinline__ int seq_of(const KvSeqs &s, uint32_t t) {
+    if (!s.cu) return static_cast<int>(t / s.per);
+    uint32_t lo = 0, hi = s.batch + 1u;   // cu[lo - 1] <= t < cu[hi], with cu[-1] = -inf
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (s.cu[mid] <= static_cast<int64_t>(t)) lo = mid + 1u;
+        else hi = mid;
+    }
+    return lo >= 1u && lo <= s.batch ? static_cast<int>(lo) - 1 : -1;
+}
+// Row of the cache that holds packed row t (head 0, K), or -1 where there is none.
+__device__ __forceinline__ int64_t row_of(const KvView &kv, const KvSeqs &s, uint32_t t, unsigned int *error_word) {
+    const int b = seq_of(s, t);
+    if (b < 0) return -1;
+    const int64_t end = s.cu ? static_cast<int64_t>(s.cu[b + 1]) : static_cast<int64_t>(b + 1) * s.per;
+    const int64_t pos = static_cast<int64_t>(s.lens[b]) - (end - static_cast<int64_t>(t));
+    if (pos < 0) return -1;
+    const int64_t pi = pos >> kv.page_shift;
+    const int32_t page = pi < s.width ? s.table[static_cast<uint64_t>(b) * s.table_stride + static_cast<uint64_t>(pi)] : -1;
+    if (page < 0 || static_cast<uint32_t>(page) >= kv.pages) {
+        atomicOr(error_word, kKvBadTable);
+        return -1;
+    }
+    return ((static_cast<int64_t>(page) * 2 * kv.kv_heads) << kv.page_shift) + (pos & (kv.page_tokens - 1));
+}
+
+template <bool F32, bool VEC>
+__device__ __forceinline__ void load8(const void *p, uint64_t at, float (&x)[8]) {
+    if (F32) {
+        const float *f = static_cast<const float *>(p) + at;
+        if (VEC) {
+            const float4 a = *reinterpret_cast<const float4 *>(f), b = *reinterpret_cast<const float4 *>(f + 4);
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = f[i];
+        }
+    } else {
+        const uint16_t *f = static_cast<const uint16_t *>(p) + at;
+        if (VEC) {
+            const uint4 a = *reinterpret_cast<const uint4 *>(f);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = bf16_f32(f[i]);
+        }
+    }
+}
+template <bool F32, bool VEC>
+__device__ __forceinline__ void store8(void *p, uint64_t at, const float (&x)[8]) {
+    if (F32) {
+        float *f = static_cast<float *>(p) + at;
+        if (VEC) {
+            *reinterpret_cast<float4 *>(f) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4 *>(f + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = x[i];
+        }
+    } else {
+        uint16_t *f = static_cast<uint16_t *>(p) + at;
+        if (VEC) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = f32_bf16(x[2 * i]) | (f32_bf16(x[2 * i + 1]) << 16);
+            *reinterpret_cast<uint4 *>(f) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = static_cast<uint16_t>(f32_bf16(x[i]));
+        }
+    }
+}
+
+struct KvRows {
+    const void *x[2];    // K, V
+    KvStrides st[2];
+};
+
+// Thread = 8 values of one (token, K or V, head); the group's lanes (G / 8 neighbours) share minimum and maximum.
+template <bool F32, bool VEC>
+__global__ void __launch_bounds__(kThreadsKv) gaf_kv_append_kernel(const KvView kv, const KvSeqs seqs, const KvRows in,
+                                                                   unsigned int *error_word) {
+    const uint32_t per_row = kv.head_dim >> 3;
+    const uint64_t total = static_cast<uint64_t>(seqs.total) * 2u * kv.kv_heads * per_row;
+    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kThreadsKv + threadIdx.x;
+    const bool live = at < total;
+    const uint64_t row_id = (live ? at : total - 1) / per_row;
+    const uint32_t vec = static_cast<uint32_t>((live ? at : total - 1) % per_row);
+    const uint32_t head = static_cast<uint32_t>(row_id % kv.kv_heads);
+    const uint32_t which = static_cast<uint32_t>(row_id / kv.kv_heads) & 1u;
+    const uint32_t t = static_cast<uint32_t>(row_id / (2u * kv.kv_heads));
+    const int64_t row0 = row_of(kv, seqs, t, error_word);
+    float x[8];
+    load8<F32, VEC>(in.x[which], t * in.st[which].token + head * in.st[which].head + vec * 8u, x);
+    float lo = x[0], hi = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        lo = -max_nan(-lo, -x[i]);
+        hi = max_nan(hi, x[i]);
+    }
+    for (uint32_t o = kv.group >> 4; o >= 1u; o >>= 1) {
+        lo = -max_nan(-lo, -__shfl_xor_sync(0xFFFFFFFFu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
+    }
+    const float maxq = kv.bits == 4u ? 15.0f : 255.0f;
+    const float range = 0.5f * hi - 0.5f * lo;             // of halves: finite for finite values
+    uint32_t sraw = f32_bf16(__fdiv_rn(range, 0.5f * maxq)), braw = f32_bf16(lo);
+    if ((braw & 0x7FFFu) == 0x7F80u) braw -= 1u;           // f32 values beyond the largest bf16
+    float s = bf16_f32(sraw);
+    if (s < FLT_MIN) s = 0.0f, sraw = 0u;
+    const bool finite = range <= FLT_MAX;
+    if (!finite) sraw = braw = 0x7FC0u, s = 0.0f;          // an infinity or a NaN in the group
+    const float half_b = 0.5f * bf16_f32(braw), half_s = 0.5f * s;
+    const float r = s > 0.0f ? __frcp_rn(half_s) : 0.0f;
+    uint32_t q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float u = __fsub_rn(0.5f * x[i], half_b);
+        float c = u * r;
+        // the product is within 2^-15 of the quotient: only next to a tie does the division decide the code
+        if (s > 0.0f && fabsf(c - rintf(c)) > 0.4995f) c = __fdiv_rn(u, half_s);
+        q[i] = finite ? static_cast<uint32_t>(fminf(fmaxf(rintf(c), 0.0f), maxq)) : 0u;
+    }
+    if (!live || row0 < 0) return;
+    const int64_t row = row0 + ((static_cast<int64_t>(which) * kv.kv_heads + head) << kv.page_shift);
+    uint8_t *dst = kv.packed + row * kv.row_bytes + vec * kv.bits;   // 8 codes are `bits` bytes
+    if (kv.bits == 8u) {
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
+    } else {
+        uint32_t w = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w |= q[i] << (4 * i);
+        *reinterpret_cast<uint32_t *>(dst) = w;
+    }
+    if ((vec & ((kv.group >> 3) - 1u)) == 0u) {
+        const int64_t g = row * kv.groups + (vec * 8u >> kv.group_shift);
+        kv.scales[g] = static_cast<uint16_t>(sraw);
+        kv.biases[g] = static_cast<uint16_t>(braw);
+    }
+}
+
+// Thread = 8 values of one (token, K or V, head).
+template <bool F32, bool VEC>
+__global__ void __launch_bounds__(kThreadsKv) gaf_kv_read_kernel(const KvView kv, const KvSeqs seqs, const KvRows out,
+                                                                 unsigned int *error_word) {
+    const uint32_t per_row = kv.head_dim >> 3;
+    const uint64_t total = static_cast<uint64_t>(seqs.total) * 2u * kv.kv_heads * per_row;
+    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kThreadsKv + threadIdx.x;
+    if (at >= total) return;
+    const uint64_t row_id = at / per_row;
+    const uint32_t vec = static_cast<uint32_t>(at % per_row);
+    const uint32_t head = static_cast<uint32_t>(row_id % kv.kv_heads);
+    const uint32_t which = static_cast<uint32_t>(row_id / kv.kv_heads) & 1u;
+    const uint32_t t = static_cast<uint32_t>(row_id / (2u * kv.kv_heads));
+    const int64_t row0 = row_of(kv, seqs, t, error_word);
+    if (row0 < 0) return;
+    const int64_t row = row0 + ((static_cast<int64_t>(which) * kv.kv_heads + head) << kv.page_shift);
+    const uint8_t *src = kv.packed + row * kv.row_bytes + vec * kv.bits;
+    const int64_t g = row * kv.groups + (vec * 8u >> kv.group_shift);
+    const float s = bf16_f32(kv.scales[g]), b = bf16_f32(kv.biases[g]);
+    float x[8];
+    if (kv.bits == 8u) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(src);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = fmaf(static_cast<float>(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xFFu), s, b);
+    } else {
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(src);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = fmaf(static_cast<float>((w >> (4 * i)) & 15u), s, b);
+    }
+    store8<F32, VEC>(const_cast<void *>(out.x[which]), t * out.st[which].token + head * out.st[which].head + vec * 8u, x);
+}
+
+bool vec_ok(const void *p, KvStrides st, bool f32) {
+    const uint64_t n = f32 ? 4u : 8u;   // elements of 16 bytes
+    return reinterpret_cast<uintptr_t>(p) % 16u == 0u && st.token % n == 0u && st.head % n == 0u;
+}
+
+// ---- attention for any head size ------------------------------------------------------------------------------------
+// CTA = one query row (token, head); its warps take every fourth run of 32 keys.  In a run a lane owns a key for the scores
+// and 1 / 32 of the head for the weighted sum; one running maximum and sum per warp, joined at the end.
+constexpr int kWarpsGen = 4;
+constexpr int kMaxDim = 256;
+
+__device__ __forceinline__ uint32_t code_at(const KvView &kv, const uint8_t *row, uint32_t d) {
+    return kv.bits == 8u ? row[d] : (row[d >> 1] >> (4u * (d & 1u))) & 15u;
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(kWarpsGen * 32) gaf_attention_generic_kernel(const AttnArgs a) {
+    __shared__ float s_q[kMaxDim];
+    __shared__ float s_o[kWarpsGen][kMaxDim];
+    __shared__ float s_m[kWarpsGen], s_l[kWarpsGen];
+    const KvView &kv = a.kv;
+    const uint32_t t = blockIdx.x / a.q_heads, hq = blockIdx.x % a.q_heads, head = hq / (a.q_heads / kv.kv_heads);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t D = kv.head_dim;
+    const int b = seq_of(a.seqs, t);
+    if (b < 0) return;
+    const int64_t begin = a.seqs.cu ? static_cast<int64_t>(a.seqs.cu[b]) : static_cast<int64_t>(b) * a.seqs.per;
+    const int64_t end = a.seqs.cu ? static_cast<int64_t>(a.seqs.cu[b + 1]) : begin + a.seqs.per;
+    if (static_cast<int64_t>(t) - begin >= static_cast<int64_t>(a.max_new)) {
+        if (threadIdx.x == 0) atomicOr(a.error_word, kKvBadCount);
+        return;
+    }
+    for (uint32_t d = threadIdx.x; d < D; d += kWarpsGen * 32) {
+        const uint64_t at = t * a.qs.token + hq * a.qs.head + d;
+        s_q[d] = F32 ? static_cast<const float *>(a.q)[at] : bf16_f32(static_cast<const uint16_t *>(a.q)[at]);
+    }
+    __syncthreads();
+    const int64_t limit = static_cast<int64_t>(a.seqs.lens[b]) - (end - 1 - static_cast<int64_t>(t));   // keys seen
+    float m = -INFINITY, l = 0.0f, o[kMaxDim / 32];
+#pragma unroll
+    for (int i = 0; i < kMaxDim / 32; ++i) o[i] = 0.0f;
+    for (int part = a.prefix_table ? 0 : 1; part < 2; ++part) {
+        const int64_t keys = part == 0 ? static_cast<int64_t>(a.prefix_len) : limit;
+        const int32_t *table = part == 0 ? a.prefix_table : a.seqs.table + static_cast<uint64_t>(b) * a.seqs.table_stride;
+        for (int64_t j0 = warp * 32; j0 < keys; j0 += kWarpsGen * 32) {
+            const int64_t j = j0 + lane, pi = j >> kv.page_shift;
+            int64_t krow = -1;
+            if (j < keys) {
+                const int32_t page = part == 0 || pi < a.seqs.width ? table[pi] : -1;
+                if (page < 0 || static_cast<uint32_t>(page) >= kv.pages) atomicOr(a.error_word, kKvBadTable);
+                else krow = ((static_cast<int64_t>(page) * 2 * kv.kv_heads + head) << kv.page_shift) + (j & (kv.page_tokens - 1));
+            }
+            float score = -INFINITY;
+            if (krow >= 0) {
+                score = 0.0f;
+                const uint8_t *row = kv.packed + krow * kv.row_bytes;
+                for (uint32_t g = 0; g < kv.groups; ++g) {
+                    const float s = bf16_f32(kv.scales[krow * kv.groups + g]), bias = bf16_f32(kv.biases[krow * kv.groups + g]);
+                    for (uint32_t d = g * kv.group; d < (g + 1u) * kv.group; ++d)
+                        score = fmaf(s_q[d], fmaf(static_cast<float>(code_at(kv, row, d)), s, bias), score);
+                }
+                score *= a.scale;
+            }
+            float top = score;
+            for (int x = 16; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+            const float m1 = fmaxf(m, top);
+            if (m1 == -INFINITY && !__any_sync(0xFFFFFFFFu, score != score)) continue;   // no key of the run can be seen
+            const float keep = m == m1 ? 1.0f : expf(m - m1);
+            const float p = krow >= 0 ? expf(score - m1) : 0.0f;
+            m = m1;
+            l *= keep;
+            float sum = p;
+            for (int x = 16; x >= 1; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+            l += sum;
+#pragma unroll
+            for (int i = 0; i < kMaxDim / 32; ++i) o[i] *= keep;
+            for (int k = 0; k < 32; ++k) {
+                const int64_t kr = __shfl_sync(0xFFFFFFFFu, krow, k);
+                const float pk = __shfl_sync(0xFFFFFFFFu, p, k);
+                if (kr < 0) continue;
+                const int64_t vrow = kr + (static_cast<int64_t>(kv.kv_heads) << kv.page_shift);
+                const uint8_t *row = kv.packed + vrow * kv.row_bytes;
+#pragma unroll
+                for (int i = 0; i < kMaxDim / 32; ++i) {
+                    const uint32_t d = i * 32u + lane;
+                    if (d >= D) continue;
+                    const int64_t g = vrow * kv.groups + (d >> kv.group_shift);
+                    o[i] = fmaf(pk, fmaf(static_cast<float>(code_at(kv, row, d)), bf16_f32(kv.scales[g]), bf16_f32(kv.biases[g])), o[i]);
+                }
+            }
+        }
+    }
+    if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+#pragma unroll
+    for (int i = 0; i < kMaxDim / 32; ++i)
+        if (i * 32u + lane < D) s_o[warp][i * 32 + lane] = o[i];
+    __syncthreads();
+    float top = -INFINITY, total = 0.0f;
+    for (int w = 0; w < kWarpsGen; ++w) top = fmaxf(top, s_m[w]);
+    for (int w = 0; w < kWarpsGen; ++w) total += s_m[w] == -INFINITY ? s_l[w] : s_l[w] * expf(s_m[w] - top);
+    for (uint32_t d = threadIdx.x; d < D; d += kWarpsGen * 32) {
+        float v = 0.0f;
+        for (int w = 0; w < kWarpsGen; ++w) v += s_m[w] == -INFINITY ? s_o[w][d] : s_o[w][d] * expf(s_m[w] - top);
+        v = total == 0.0f ? 0.0f : v / total;
+        const uint64_t at = t * a.os.token + hq * a.os.head + d;
+        if (F32) static_cast<float *>(a.out)[at] = v;
+        else static_cast<uint16_t *>(a.out)[at] = static_cast<uint16_t>(f32_bf16(v));
+    }
+}
+
+}  // namespace
+
+cudaError_t kv_append(const KvView &kv, const KvSeqs &seqs, bool f32, const void *k, KvStrides ks, const void *v, KvStrides vs,
+                      unsigned int *error_word, cudaStream_t stream) {
+    const uint64_t n = static_cast<uint64_t>(seqs.total) * 2u * kv.kv_heads * (kv.head_dim / 8u);
+    if (n == 0) return cudaSuccess;
+    const KvRows in = {{k, v}, {ks, vs}};
+    const bool vec = vec_ok(k, ks, f32) && vec_ok(v, vs, f32);
+    const unsigned int grid = static_cast<unsigned int>((n + kThreadsKv - 1) / kThreadsKv);
+    if (f32 && vec) gaf_kv_append_kernel<true, true><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, error_word);
+    else if (f32) gaf_kv_append_kernel<true, false><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, error_word);
+    else if (vec) gaf_kv_append_kernel<false, true><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, error_word);
+    else gaf_kv_append_kernel<false, false><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, error_word);
+    return cudaGetLastError();
+}
+
+cudaError_t kv_read(const KvView &kv, const KvSeqs &seqs, bool f32, void *k, KvStrides ks, void *v, KvStrides vs,
+                    unsigned int *error_word, cudaStream_t stream) {
+    const uint64_t n = static_cast<uint64_t>(seqs.total) * 2u * kv.kv_heads * (kv.head_dim / 8u);
+    if (n == 0) return cudaSuccess;
+    const KvRows out = {{k, v}, {ks, vs}};
+    const bool vec = vec_ok(k, ks, f32) && vec_ok(v, vs, f32);
+    const unsigned int grid = static_cast<unsigned int>((n + kThreadsKv - 1) / kThreadsKv);
+    if (f32 && vec) gaf_kv_read_kernel<true, true><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, error_word);
+    else if (f32) gaf_kv_read_kernel<true, false><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, error_word);
+    else if (vec) gaf_kv_read_kernel<false, true><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, error_word);
+    else gaf_kv_read_kernel<false, false><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, error_word);
+    return cudaGetLastError();
+}
+
+cudaError_t attention_generic(const AttnArgs &a, bool f32, cudaStream_t stream) {
+    if (a.seqs.total == 0) return cudaSuccess;
+    const unsigned int grid = a.seqs.total * a.q_heads;
+    if (f32) gaf_attention_generic_kernel<true><<<grid, kWarpsGen * 32, 0, stream>>>(a);
+    else gaf_attention_generic_kernel<false><<<grid, kWarpsGen * 32, 0, stream>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace tgaf
