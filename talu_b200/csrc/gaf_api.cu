@@ -112,6 +112,12 @@ struct tgaf_ctx {
     size_t gemm_ws_bytes = 0;
     unsigned int *gemm_flags = nullptr;
     size_t gemm_flag_count = 0;
+    // attention over the quantised KV cache: partial results of sequences cut across CTAs, and the rows' results against a
+    // shared prefix.  The latter grows; what it has outgrown is kept until the context ends, since a captured graph may hold it
+    float *attn_partials = nullptr;
+    unsigned int *attn_tickets = nullptr;
+    std::vector<float *> attn_prefix;
+    size_t attn_prefix_bytes = 0;
     std::vector<tgaf_batch *> batches;   // live launch lists (their counters are reset after an abandoned launch)
     NcclComm comm = nullptr;
     uint32_t comm_rank = 0, comm_size = 1;
@@ -159,6 +165,8 @@ struct tgaf_host_batch {
 
 struct tgaf_kv_cache {
     KvView v;
+    CUtensorMap tmap;   // the codes' rows
+    bool fast = false;  // the tensor-core attention kernels take this head size
 };
 
 struct tgaf_weight {
@@ -417,7 +425,28 @@ int32_t attend(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const int32_t *prefix_
     a.scale = scale;
     a.error_word = ctx->d_error_word;
     TGAF_CUDA(ctx, cudaSetDevice(ctx->device));
-    const cudaError_t e = attention_generic(a, dtype == TGAF_DTYPE_F32, ctx->stream);
+    cudaError_t e;
+    if (cache->fast) {
+        const uint64_t rows = static_cast<uint64_t>(a.seqs.total) * q_heads;
+        if (prefix_table) {
+            const size_t need = rows * (a.kv.head_dim + 1u) * sizeof(float);
+            if (need > ctx->attn_prefix_bytes) {
+                cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+                TGAF_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &cap));
+                if (cap != cudaStreamCaptureStatusNone)
+                    return fail(ctx, TGAF_ERR_UNSUPPORTED, "the workspace must grow to %zu bytes: make a call of this size before the capture", need);
+                float *b = nullptr;
+                const size_t want = need < (size_t(8) << 20) ? size_t(8) << 20 : need;
+                TGAF_CUDA(ctx, cudaMalloc(reinterpret_cast<void **>(&b), want));
+                ctx->attn_prefix.push_back(b);
+                ctx->attn_prefix_bytes = want;
+            }
+        }
+        const AttnWorkspace ws = {ctx->attn_partials, ctx->attn_tickets, prefix_table ? ctx->attn_prefix.back() : nullptr};
+        e = attention(a, cache->tmap, ws, dtype == TGAF_DTYPE_F32, ctx->sm_count, ctx->stream);
+    } else {
+        e = attention_generic(a, dtype == TGAF_DTYPE_F32, ctx->stream);
+    }
     return e == cudaSuccess ? TGAF_OK : cuda_fail(ctx, e, "attention launch");
 }
 
@@ -619,6 +648,9 @@ int32_t tgaf_ctx_destroy(tgaf_ctx *ctx) {
     if (ctx->d_grid_bar) cudaFree(ctx->d_grid_bar);
     if (ctx->gemm_ws) cudaFree(ctx->gemm_ws);
     if (ctx->gemm_flags) cudaFree(ctx->gemm_flags);
+    if (ctx->attn_partials) cudaFree(ctx->attn_partials);
+    if (ctx->attn_tickets) cudaFree(ctx->attn_tickets);
+    for (float *b : ctx->attn_prefix) cudaFree(b);
     if (ctx->owns_stream && ctx->stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
     return TGAF_OK;
@@ -730,6 +762,7 @@ int32_t tgaf_synchronize(tgaf_ctx *ctx) {
         if (ctx->scratch.tagged) cudaMemset(ctx->scratch.tagged, 0, ctx->scratch.tagged_bytes);  // ... or tags set
         if (ctx->d_grid_bar) cudaMemset(ctx->d_grid_bar, 0, 4 * sizeof(unsigned int));
         if (ctx->gemm_flags) cudaMemset(ctx->gemm_flags, 0, ctx->gemm_flag_count * sizeof(unsigned int));
+        if (ctx->attn_tickets) cudaMemset(ctx->attn_tickets, 0, attention_ticket_count(ctx->sm_count) * sizeof(unsigned int));
         for (tgaf_batch *b : ctx->batches) {
             if (b->list) gemv_list_reset(b->list);
             if (b->tagged) cudaMemset(b->tagged, 0, b->tagged_bytes);
@@ -1622,6 +1655,22 @@ int32_t tgaf_kv_cache_wrap_device(tgaf_ctx *ctx, void *d_packed, void *d_scales,
     v.groups = head_dim / group_size;
     v.bits = bits;
     v.row_bytes = head_dim * bits / 8;
+    cudaError_t e = cudaSetDevice(ctx->device);
+    if (e == cudaSuccess && attention_fast(v)) {
+        // the workspace has one size for all calls: captured calls may go on using it
+        if (!ctx->attn_partials) e = cudaMalloc(reinterpret_cast<void **>(&ctx->attn_partials), attention_partial_bytes(ctx->sm_count));
+        if (e == cudaSuccess && !ctx->attn_tickets) {
+            const size_t bytes = attention_ticket_count(ctx->sm_count) * sizeof(unsigned int);
+            e = cudaMalloc(reinterpret_cast<void **>(&ctx->attn_tickets), bytes);
+            if (e == cudaSuccess) e = cudaMemsetAsync(ctx->attn_tickets, 0, bytes, ctx->stream);
+        }
+        if (e == cudaSuccess) e = make_kv_tmap(v, &c->tmap);
+        c->fast = e == cudaSuccess;
+    }
+    if (e != cudaSuccess) {
+        delete c;
+        return cuda_fail(ctx, e, "kv cache set-up");
+    }
     *out_cache = c;
     return TGAF_OK;
 }

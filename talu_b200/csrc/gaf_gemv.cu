@@ -2472,6 +2472,19 @@ cudaError_t make_packed_tmap(const WeightView &w, CUtensorMap *out) {
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t make_row_tmap(const void *base, uint64_t rows, uint32_t row_bytes, uint32_t box_rows, CUtensorMap *out) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {row_bytes, rows};
+    const cuuint64_t strides[1] = {row_bytes};
+    const cuuint32_t box[2] = {row_bytes, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUtensorMapSwizzle swizzle = row_bytes == 128u ? CU_TENSOR_MAP_SWIZZLE_128B : row_bytes == 64u ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+    const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 // Tensor map of a scale / bias array as bytes [N][groups * 2], tile 128 rows x max(16, groups-per-unit * 2) bytes.
 static cudaError_t make_sb_tmap(const WeightView &w, const uint16_t *base, CUtensorMap *out) {
     EncodeTiledFn enc = encode_tiled_fn();

@@ -63,6 +63,8 @@ bool gemv_mma_eligible(const WeightView &w, const void *x, const void *y, bool x
 // fills w.tmap / w.has_tmap from the other fields
 void attach_packed_tmap(WeightView &w);
 cudaError_t make_packed_tmap(const WeightView &w, CUtensorMap *out);
+// `rows` rows of 32, 64 or 128 bytes, tile box_rows x a row, with the swizzle of the row's width
+cudaError_t make_row_tmap(const void *base, uint64_t rows, uint32_t row_bytes, uint32_t box_rows, CUtensorMap *out);
 // scratch the fast path needs for this problem
 // SwiGLU FFN (stacked gate|up weight, then down) for M = 1 in one launch; `mid` is fp32 [M][2 d_ff] scratch and
 // `grid_bar` two zeroed counters.  cudaErrorNotSupported when the pair is not eligible.
@@ -168,7 +170,19 @@ cudaError_t kv_append(const KvView &kv, const KvSeqs &seqs, bool f32, const void
                       unsigned int *error_word, cudaStream_t stream);
 cudaError_t kv_read(const KvView &kv, const KvSeqs &seqs, bool f32, void *k, KvStrides ks, void *v, KvStrides vs,
                     unsigned int *error_word, cudaStream_t stream);
+// Any head size the cache takes.
 cudaError_t attention_generic(const AttnArgs &a, bool f32, cudaStream_t stream);
+// Heads of 64 or 128 values.  The map covers all rows of the codes: a box of min(64, page_tokens) rows.
+struct AttnWorkspace {
+    float *partials;          // attention_partial_bytes(sm_count)
+    unsigned int *tickets;    // attention_ticket_count(sm_count), zero between launches
+    float *prefix;            // [total * q_heads][head_dim + 1], with a shared prefix only
+};
+bool attention_fast(const KvView &kv);
+cudaError_t make_kv_tmap(const KvView &kv, CUtensorMap *out);
+size_t attention_partial_bytes(int sm_count);
+size_t attention_ticket_count(int sm_count);
+cudaError_t attention(const AttnArgs &a, const CUtensorMap &tmap, const AttnWorkspace &ws, bool f32, int sm_count, cudaStream_t stream);
 
 // ---- all-reduce over NVLink peer memory (gaf_peer.cu) ----
 constexpr int kPeerMaxRanks = 8;                      // ranks of one node

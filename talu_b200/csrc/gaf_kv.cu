@@ -7,6 +7,7 @@
 // what the format stores; the codes are taken against the rounded pair, which makes the rounding of s part of the grid and
 // not an error of every value: only the top value can be off by more than half a step, (max x - min x) 2^-9 + s / 2.
 // Differences are formed of halves (0.5 x - 0.5 b), which is exact scaling, so that no finite input overflows.
+#include "gaf_attend.cuh"
 #include "gaf_internal.h"
 
 #include <cuda_bf16.h>
@@ -348,6 +349,50 @@ cudaError_t attention_generic(const AttnArgs &a, bool f32, cudaStream_t stream) 
     if (f32) gaf_attention_generic_kernel<true><<<grid, kWarpsGen * 32, 0, stream>>>(a);
     else gaf_attention_generic_kernel<false><<<grid, kWarpsGen * 32, 0, stream>>>(a);
     return cudaGetLastError();
+}
+
+bool attention_fast(const KvView &kv) { return kv.head_dim == 64u || kv.head_dim == 128u; }
+size_t attention_ticket_count(int sm_count) { return static_cast<size_t>(sm_count) * attend::kMaxCtas; }
+size_t attention_partial_bytes(int sm_count) {
+    return attention_ticket_count(sm_count) * 2u * attend::kMaxRows * (attend::kMaxDim + 2) * sizeof(float);
+}
+
+cudaError_t make_kv_tmap(const KvView &kv, CUtensorMap *out) {
+    const uint64_t rows = static_cast<uint64_t>(kv.pages) * 2u * kv.kv_heads * kv.page_tokens;
+    const uint32_t box = kv.page_tokens < static_cast<uint32_t>(attend::kKeys) ? kv.page_tokens : attend::kKeys;
+    return make_row_tmap(kv.packed, rows, kv.row_bytes, box, out);
+}
+
+cudaError_t attention(const AttnArgs &a, const CUtensorMap &tmap, const AttnWorkspace &ws, bool f32, int sm_count, cudaStream_t stream) {
+    attend::Params p;
+    p.a = a;
+    p.per_kv = a.q_heads / a.kv.kv_heads;
+    p.partials = ws.partials;
+    p.tickets = ws.tickets;
+    p.prefix_o = ws.prefix;
+    p.prefix_lse = ws.prefix ? ws.prefix + static_cast<uint64_t>(a.seqs.total) * a.q_heads * a.kv.head_dim : nullptr;
+    const uint64_t align = f32 ? 4u : 4u;
+    p.o_vec = reinterpret_cast<uintptr_t>(a.out) % (f32 ? 16u : 8u) == 0u && a.os.token % align == 0u && a.os.head % align == 0u;
+    p.q_vec = 0u;
+    auto run = [&](uint64_t rows) {
+        // 8 rows a tile cost least where they suffice; more rows read the cache less often
+        const int nt = rows <= 8u ? 1 : rows <= 16u || f32 ? 2 : 4;
+        p.row_tiles = static_cast<uint32_t>((rows + 8u * nt - 1u) / (8u * nt));
+        p.elements = p.prefix_pass ? p.row_tiles : p.row_tiles * a.seqs.batch;
+        const int limbs = f32 ? 2 : 1;
+        if (a.kv.head_dim == 64u)
+            return a.kv.bits == 4u ? attend::launch_d64_b4(p, tmap, nt, limbs, sm_count, stream) : attend::launch_d64_b8(p, tmap, nt, limbs, sm_count, stream);
+        return a.kv.bits == 4u ? attend::launch_d128_b4(p, tmap, nt, limbs, sm_count, stream) : attend::launch_d128_b8(p, tmap, nt, limbs, sm_count, stream);
+    };
+    p.merge_prefix = 0u;
+    if (a.prefix_table) {
+        p.prefix_pass = 1u;
+        const cudaError_t e = run(static_cast<uint64_t>(a.seqs.total) * p.per_kv);
+        if (e != cudaSuccess) return e;
+        p.merge_prefix = 1u;
+    }
+    p.prefix_pass = 0u;
+    return run(static_cast<uint64_t>(a.max_new) * p.per_kv);
 }
 
 }  // namespace tgaf
