@@ -153,7 +153,7 @@ struct Params {
     float *prefix_lse;      // [rows], base 2
     float *partials;        // [2 * gridDim.x][R * (D + 2)]
     unsigned int *tickets;  // [gridDim.x], zero between launches
-    uint32_t q_vec, o_vec;  // rows of q / out can be read / written 4 values at a time
+    uint32_t q_vec, o_vec;  // rows of q / out can be read / written by vectors
 };
 
 // An item is one (cached head, element); an element one row tile of one sequence.
@@ -168,7 +168,7 @@ struct Item {
     int32_t seq;
 };
 
-template <int R>
+template <int R, int KEYS>
 __device__ __forceinline__ Item item_at(const Params &p, uint32_t n) {
     Item it;
     const KvSeqs &s = p.a.seqs;
@@ -179,7 +179,7 @@ __device__ __forceinline__ Item item_at(const Params &p, uint32_t n) {
         it.rows = s.total * p.per_kv;
         it.token0 = 0;
         it.keys = it.first_seen = it.seen0 = static_cast<int32_t>(p.a.prefix_len);
-        it.tiles = (p.a.prefix_len + kKeys - 1) / kKeys;
+        it.tiles = (p.a.prefix_len + KEYS - 1) / KEYS;
         return it;
     }
     int64_t begin, count;
@@ -212,8 +212,106 @@ __device__ __forceinline__ Item item_at(const Params &p, uint32_t n) {
     it.keys = static_cast<int32_t>(keys < 0 ? 0 : keys);
     it.first_seen = static_cast<int32_t>(first < 0 ? 0 : first > keys ? keys : first);
     it.seen0 = static_cast<int32_t>(seen0 < -0x40000000ll ? -0x40000000ll : seen0);
-    it.tiles = it.keys > 0 ? (static_cast<uint32_t>(it.keys) + kKeys - 1u) / kKeys : 1u;   // an item without keys is one empty unit
+    it.tiles = it.keys > 0 ? (static_cast<uint32_t>(it.keys) + KEYS - 1u) / KEYS : 1u;   // an item without keys is one empty unit
     return it;
+}
+
+// The item at (head, elem), or the next one that has units; there is one.
+template <int R, int KEYS>
+__device__ __forceinline__ Item next_item(const Params &p, uint32_t &head, uint32_t &elem) {
+    Item item = item_at<R, KEYS>(p, elem);
+    while (item.tiles == 0u) {
+        if (++elem == p.elements) elem = 0u, ++head;
+        item = item_at<R, KEYS>(p, elem);
+    }
+    return item;
+}
+
+// The CTA's share of all units: equal contiguous ranges, in the order cached head, element, unit.  A sum over the elements
+// that every CTA forms alike; false: nothing to do.
+struct Range {
+    uint64_t u0, u1, units, ctas;
+};
+template <int R, int KEYS, int THREADS>
+__device__ __forceinline__ bool cta_range(const Params &p, uint32_t *s_scan, uint32_t *s_begin, Range &out) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t per_thread = (p.elements + THREADS - 1u) / THREADS;
+    const uint32_t n_lo = threadIdx.x * per_thread, n_hi = n_lo + per_thread < p.elements ? n_lo + per_thread : p.elements;
+    uint32_t mine = 0;
+    for (uint32_t n = n_lo; n < n_hi; ++n) mine += item_at<R, KEYS>(p, n).tiles;
+    uint32_t pre = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, pre, o);
+        if (lane >= o) pre += v;
+    }
+    if (lane == 31) s_scan[warp] = pre;
+    __syncthreads();
+    uint32_t per_head = 0;
+    pre -= mine;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) pre += s_scan[w];
+        per_head += s_scan[w];
+    }
+    out.units = static_cast<uint64_t>(per_head) * p.a.kv.kv_heads;
+    if (out.units == 0) return false;
+    out.ctas = out.units < gridDim.x ? out.units : gridDim.x;
+    if (blockIdx.x >= out.ctas) return false;
+    out.u0 = out.units * blockIdx.x / out.ctas;
+    out.u1 = out.units * (blockIdx.x + 1u) / out.ctas;
+    const uint32_t start = static_cast<uint32_t>(out.u0 % per_head);
+    if (start >= pre && start < pre + mine) {
+        uint32_t n = n_lo, at = pre;
+        for (;; ++n) {
+            const uint32_t t = item_at<R, KEYS>(p, n).tiles;
+            if (start < at + t) break;
+            at += t;
+        }
+        s_begin[0] = static_cast<uint32_t>(out.u0 / per_head);
+        s_begin[1] = n;
+        s_begin[2] = start - at;
+    }
+    __syncthreads();
+    return true;
+}
+
+// Four values of a finished row: the prefix's part added, divided by the sum, rounded once.  top: base 2.
+template <int D, bool F32>
+__device__ __forceinline__ void finish_row(const Params &p, const Item &item, uint32_t head, uint32_t r, uint32_t d, float top, float sum, float4 v) {
+    const uint32_t row = item.row0 + r;
+    const uint64_t token = static_cast<uint64_t>(item.token0 + row / p.per_kv);
+    const uint32_t hq = head * p.per_kv + row % p.per_kv;
+    const uint64_t prow = token * p.a.q_heads + hq;
+    if (p.prefix_pass) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        *reinterpret_cast<float4 *>(p.prefix_o + prow * D + d) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        if (d == 0) p.prefix_lse[prow] = sum == 0.0f ? -INFINITY : top + log2f(sum);
+        return;
+    }
+    if (p.merge_prefix) {
+        const float lse = p.prefix_lse[prow];
+        const float both = fmaxf(top, lse);
+        const float wa = top == both ? 1.0f : exp2_approx(top - both), wb = lse == both ? 1.0f : exp2_approx(lse - both);
+        if (lse != -INFINITY) {
+            const float4 x = *reinterpret_cast<const float4 *>(p.prefix_o + prow * D + d);
+            v = make_float4(fmaf(x.x, wb, v.x * wa), fmaf(x.y, wb, v.y * wa), fmaf(x.z, wb, v.z * wa), fmaf(x.w, wb, v.w * wa));
+            sum = fmaf(sum, wa, wb);
+        }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+    const uint64_t at = token * p.a.os.token + hq * p.a.os.head + d;
+    if (F32) {
+        float *dst = static_cast<float *>(p.a.out) + at;
+        if (p.o_vec) *reinterpret_cast<float4 *>(dst) = make_float4(y[0], y[1], y[2], y[3]);
+        else dst[0] = y[0], dst[1] = y[1], dst[2] = y[2], dst[3] = y[3];
+    } else {
+        uint16_t *dst = static_cast<uint16_t *>(p.a.out) + at;
+        const uint32_t lo = pack_bf16x2(y[0], y[1]), hi = pack_bf16x2(y[2], y[3]);
+        if (p.o_vec) *reinterpret_cast<uint2 *>(dst) = make_uint2(lo, hi);
+        else dst[0] = static_cast<uint16_t>(lo), dst[1] = static_cast<uint16_t>(lo >> 16), dst[2] = static_cast<uint16_t>(hi), dst[3] = static_cast<uint16_t>(hi >> 16);
+    }
 }
 
 template <int D, int BITS, int GROUP, int NT, int LIMBS>
@@ -338,44 +436,9 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // ---- this CTA's range of units: a sum over the elements, the same in every CTA ----
-    const uint32_t per_thread = (p.elements + kThreads - 1u) / kThreads;
-    const uint32_t n_lo = threadIdx.x * per_thread, n_hi = n_lo + per_thread < p.elements ? n_lo + per_thread : p.elements;
-    uint32_t mine = 0;
-    for (uint32_t n = n_lo; n < n_hi; ++n) mine += item_at<R>(p, n).tiles;
-    uint32_t pre = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, pre, o);
-        if (lane >= o) pre += v;
-    }
-    if (lane == 31) s_scan[warp] = pre;
-    __syncthreads();
-    uint32_t per_head = 0;
-    pre -= mine;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < warp) pre += s_scan[w];
-        per_head += s_scan[w];
-    }
-    const uint64_t units = static_cast<uint64_t>(per_head) * kv.kv_heads;
-    if (units == 0) return;
-    const uint64_t ctas = units < gridDim.x ? units : gridDim.x;
-    if (blockIdx.x >= ctas) return;
-    const uint64_t u0 = units * blockIdx.x / ctas, u1 = units * (blockIdx.x + 1u) / ctas;
-    const uint32_t start_in_head = static_cast<uint32_t>(u0 % per_head);
-    if (start_in_head >= pre && start_in_head < pre + mine) {
-        uint32_t n = n_lo, at = pre;
-        for (;; ++n) {
-            const uint32_t t = item_at<R>(p, n).tiles;
-            if (start_in_head < at + t) break;
-            at += t;
-        }
-        s_begin[0] = static_cast<uint32_t>(u0 / per_head);
-        s_begin[1] = n;
-        s_begin[2] = start_in_head - at;
-    }
-    __syncthreads();
+    Range range;
+    if (!cta_range<R, kKeys, kThreads>(p, s_scan, s_begin, range)) return;
+    const uint64_t u0 = range.u0, u1 = range.u1, units = range.units, ctas = range.ctas;
     uint32_t head = s_begin[0], elem = s_begin[1], tile0 = s_begin[2];
 
     if (warp == kConsumers) {
@@ -386,8 +449,7 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
         bool ok = true;
         if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap)) : "memory");
         for (uint64_t u = u0; u < u1 && ok;) {
-            Item item = item_at<R>(p, elem);
-            while (item.tiles == 0u) item = item_at<R>(p, ++elem);
+            const Item item = next_item<R, kKeys>(p, head, elem);
             const uint32_t left = item.tiles - tile0;
             const uint32_t count = u1 - u < left ? static_cast<uint32_t>(u1 - u) : left;
             const int32_t *table = p.prefix_pass ? p.a.prefix_table : p.a.seqs.table + static_cast<uint64_t>(item.seq) * p.a.seqs.table_stride;
@@ -459,8 +521,7 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
     uint32_t it = 0;
     bool failed = false;
     for (uint64_t u = u0; u < u1;) {
-        Item item = item_at<R>(p, elem);
-        while (item.tiles == 0u) item = item_at<R>(p, ++elem);
+        const Item item = next_item<R, kKeys>(p, head, elem);
         const uint32_t left = item.tiles - tile0;
         const uint32_t count = u1 - u < left ? static_cast<uint32_t>(u1 - u) : left;
 
@@ -773,42 +834,6 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
 #pragma unroll
             for (int w = 0; w < kConsumers; ++w) sum += s_ml[w][r][1] * (s_ml[w][r][0] == top ? 1.0f : exp2_approx(s_ml[w][r][0] - top));
         };
-        // four values of a finished row: the prefix's part added, divided, rounded once
-        auto finish = [&](int r, uint32_t d, float top, float sum, float4 v) {
-            const uint32_t row = item.row0 + r;
-            const uint64_t token = static_cast<uint64_t>(item.token0 + row / p.per_kv);
-            const uint32_t hq = head * p.per_kv + row % p.per_kv;
-            const uint64_t prow = token * p.a.q_heads + hq;
-            if (p.prefix_pass) {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                *reinterpret_cast<float4 *>(p.prefix_o + prow * D + d) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-                if (d == 0) p.prefix_lse[prow] = sum == 0.0f ? -INFINITY : top + log2f(sum);
-                return;
-            }
-            if (p.merge_prefix) {
-                const float lse = p.prefix_lse[prow];
-                const float both = fmaxf(top, lse);
-                const float wa = top == both ? 1.0f : exp2_approx(top - both), wb = lse == both ? 1.0f : exp2_approx(lse - both);
-                if (lse != -INFINITY) {
-                    const float4 x = *reinterpret_cast<const float4 *>(p.prefix_o + prow * D + d);
-                    v = make_float4(fmaf(x.x, wb, v.x * wa), fmaf(x.y, wb, v.y * wa), fmaf(x.z, wb, v.z * wa), fmaf(x.w, wb, v.w * wa));
-                    sum = fmaf(sum, wa, wb);
-                }
-            }
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
-            const uint64_t at = token * p.a.os.token + hq * p.a.os.head + d;
-            if (LIMBS == 2) {
-                float *dst = static_cast<float *>(p.a.out) + at;
-                if (p.o_vec) *reinterpret_cast<float4 *>(dst) = make_float4(y[0], y[1], y[2], y[3]);
-                else dst[0] = y[0], dst[1] = y[1], dst[2] = y[2], dst[3] = y[3];
-            } else {
-                uint16_t *dst = static_cast<uint16_t *>(p.a.out) + at;
-                const uint32_t lo = pack_bf16x2(y[0], y[1]), hi = pack_bf16x2(y[2], y[3]);
-                if (p.o_vec) *reinterpret_cast<uint2 *>(dst) = make_uint2(lo, hi);
-                else dst[0] = static_cast<uint16_t>(lo), dst[1] = static_cast<uint16_t>(lo >> 16), dst[2] = static_cast<uint16_t>(hi), dst[3] = static_cast<uint16_t>(hi >> 16);
-            }
-        };
         constexpr int kWide = D / S::HALVES;
 #pragma unroll
         for (int half = 0; half < S::HALVES; ++half) {
@@ -836,7 +861,7 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                 float top, sum;
                 row_sum(r, top, sum);
                 if (whole) {
-                    finish(r, half * kWide + d, top, sum, v);
+                    finish_row<D, LIMBS == 2>(p, item, head, r, half * kWide + d, top, sum, v);
                 } else {
                     __stcg(reinterpret_cast<float4 *>(part + r * D + half * kWide + d), v);
                     if (half == 0 && d == 0) {
@@ -877,7 +902,7 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                         sum = fmaf(sum, wa, lc * wb);
                         v = make_float4(fmaf(v.x, wa, y.x * wb), fmaf(v.y, wa, y.y * wb), fmaf(v.z, wa, y.z * wb), fmaf(v.w, wa, y.w * wb));
                     }
-                    finish(r, d, top, sum, v);
+                    finish_row<D, LIMBS == 2>(p, item, head, r, d, top, sum, v);
                 }
             }
         }
@@ -912,8 +937,11 @@ cudaError_t launch_rows(const Params &p, const CUtensorMap &tmap, int nt, int li
     return launch<D, BITS, GROUP, 4, 1>(p, tmap, sm_count, stream);
 }
 
-constexpr int kMaxCtas = 3;      // per SM, of any instance
-constexpr int kMaxRows = 32;
+// tcgen05, bf16 rows (gaf_attend_wide.cuh): 256 rows a tile
+cudaError_t launch_wide(const Params &p, const CUtensorMap &tmap, int sm_count, cudaStream_t stream);
+
+constexpr int kMaxCtas = 3;             // per SM, of any instance
+constexpr int kMaxPartRows = 256 * 2;   // rows of the partial results of an SM's CTAs (3 CTAs x 2 slots x 32 rows; 1 x 2 x 256)
 constexpr int kMaxDim = 128;
 
 }  // namespace attend

@@ -351,10 +351,13 @@ cudaError_t attention_generic(const AttnArgs &a, bool f32, cudaStream_t stream) 
     return cudaGetLastError();
 }
 
+// Up to so many rows of a cached head and sequence the register-path kernel takes bf16 calls.
+constexpr uint64_t kNarrowRows = 32;
+
 bool attention_fast(const KvView &kv) { return kv.head_dim == 64u || kv.head_dim == 128u; }
 size_t attention_ticket_count(int sm_count) { return static_cast<size_t>(sm_count) * attend::kMaxCtas; }
 size_t attention_partial_bytes(int sm_count) {
-    return attention_ticket_count(sm_count) * 2u * attend::kMaxRows * (attend::kMaxDim + 2) * sizeof(float);
+    return static_cast<size_t>(sm_count) * attend::kMaxPartRows * (attend::kMaxDim + 2) * sizeof(float);
 }
 
 cudaError_t make_kv_tmap(const KvView &kv, CUtensorMap *out) {
@@ -371,10 +374,14 @@ cudaError_t attention(const AttnArgs &a, const CUtensorMap &tmap, const AttnWork
     p.tickets = ws.tickets;
     p.prefix_o = ws.prefix;
     p.prefix_lse = ws.prefix ? ws.prefix + static_cast<uint64_t>(a.seqs.total) * a.q_heads * a.kv.head_dim : nullptr;
-    const uint64_t align = f32 ? 4u : 4u;
-    p.o_vec = reinterpret_cast<uintptr_t>(a.out) % (f32 ? 16u : 8u) == 0u && a.os.token % align == 0u && a.os.head % align == 0u;
-    p.q_vec = 0u;
+    p.o_vec = reinterpret_cast<uintptr_t>(a.out) % (f32 ? 16u : 8u) == 0u && a.os.token % 4u == 0u && a.os.head % 4u == 0u;
+    p.q_vec = vec_ok(a.q, a.qs, f32);
     auto run = [&](uint64_t rows) {
+        if (!f32 && rows > kNarrowRows) {
+            p.row_tiles = static_cast<uint32_t>((rows + 255u) / 256u);
+            p.elements = p.prefix_pass ? p.row_tiles : p.row_tiles * a.seqs.batch;
+            return attend::launch_wide(p, tmap, sm_count, stream);
+        }
         // 8 rows a tile cost least where they suffice; more rows read the cache less often
         const int nt = rows <= 8u ? 1 : rows <= 16u || f32 ? 2 : 4;
         p.row_tiles = static_cast<uint32_t>((rows + 8u * nt - 1u) / (8u * nt));
