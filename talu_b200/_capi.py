@@ -9,9 +9,16 @@ LIB_PATH = Path(__file__).resolve().parent / "libtalu_gaf.so"
 
 COMM_ID_BYTES = 128
 
+class KvSeqs(C.Structure):
+    """tgaf_kv_seqs: the sequences of a call on the quantised KV cache"""
+    _fields_ = [("d_table", C.c_void_p), ("table_stride", C.c_uint64), ("table_width", C.c_uint32), ("batch", C.c_uint32),
+                ("d_lens", C.c_void_p), ("d_cu", C.c_void_p), ("total", C.c_uint32)]
+
+
 # name -> (restype, argtypes); every symbol include/talu_gaf.h declares
 _vp, _i32, _u32, _u64, _i64, _cp = C.c_void_p, C.c_int32, C.c_uint32, C.c_uint64, C.c_int64, C.c_char_p
 _pp = C.POINTER(C.c_void_p)
+_sq = C.POINTER(KvSeqs)
 SIGNATURES = {
     "tgaf_abi_version": (_i32, []),
     "tgaf_status_string": (_cp, [_i32]),
@@ -45,10 +52,10 @@ SIGNATURES = {
     "tgaf_embedding_lookup_f32": (_i32, [_vp, _vp, _vp, _u32, C.c_float, _vp]),
     "tgaf_kv_cache_wrap_device": (_i32, [_vp, _vp, _vp, _vp, _u64, _u32, _u32, _u32, _u32, _u32, _pp]),
     "tgaf_kv_cache_free": (_i32, [_vp, _vp]),
-    "tgaf_kv_append": (_i32, [_vp, _vp, _vp, _u32, _vp, _u64, _u64, _vp, _u64, _u64]),
-    "tgaf_kv_read": (_i32, [_vp, _vp, _vp, _u32, _vp, _u64, _u64, _vp, _u64, _u64]),
-    "tgaf_attention": (_i32, [_vp, _vp, _vp, _u32, _vp, _u64, _u64, _u32, _u32, C.c_float, _vp, _u64, _u64]),
-    "tgaf_attention_shared_prefix": (_i32, [_vp, _vp, _vp, _u32, _vp, _u32, _vp, _u64, _u64, _u32, _u32, C.c_float, _vp, _u64, _u64]),
+    "tgaf_kv_append": (_i32, [_vp, _vp, _sq, _u32, _vp, _u64, _u64, _vp, _u64, _u64]),
+    "tgaf_kv_read": (_i32, [_vp, _vp, _sq, _u32, _vp, _u64, _u64, _vp, _u64, _u64]),
+    "tgaf_attention": (_i32, [_vp, _vp, _sq, _u32, _vp, _u64, _u64, _u32, _u32, C.c_float, _vp, _u64, _u64]),
+    "tgaf_attention_shared_prefix": (_i32, [_vp, _vp, _vp, _u32, _sq, _u32, _vp, _u64, _u64, _u32, _u32, C.c_float, _vp, _u64, _u64]),
     "tgaf_comm_make_id": (_i32, [_vp]),
     "tgaf_comm_init": (_i32, [_vp, _vp, _u32, _u32]),
     "tgaf_comm_destroy": (_i32, [_vp]),
@@ -67,12 +74,6 @@ SIGNATURES = {
     "tgaf_batch_destroy": (_i32, [_vp, _vp]),
 }
 
-
-
-class KvSeqs(C.Structure):
-    """tgaf_kv_seqs: the sequences of a call on the quantised KV cache"""
-    _fields_ = [("d_table", C.c_void_p), ("table_stride", C.c_uint64), ("table_width", C.c_uint32), ("batch", C.c_uint32),
-                ("d_lens", C.c_void_p), ("d_cu", C.c_void_p), ("total", C.c_uint32)]
 
 
 # tgaf_watch_fns: the three hooks of tgaf_watchdog_wait

@@ -28,6 +28,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 namespace tgaf {
 namespace attend {
 
@@ -913,11 +915,28 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
     }
 }
 
+// Something that is done once for each device (a kernel's shared-memory opt-in), from any host thread.
+struct DeviceOnce {
+    std::atomic<uint64_t> done{0};
+    template <class F>
+    cudaError_t run(F &&f) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0u;
+        if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+        e = f();
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+        return e;
+    }
+};
+
 template <int D, int BITS, int GROUP, int NT, int LIMBS>
 cudaError_t launch(const Params &p, const CUtensorMap &tmap, int sm_count, cudaStream_t stream) {
     using S = Shape<D, BITS, GROUP, NT, LIMBS>;
     auto kernel = gaf_attend_kernel<D, BITS, GROUP, NT, LIMBS>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    static DeviceOnce once;    // of this instance
+    const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
     if (e != cudaSuccess) return e;
     kernel<<<sm_count * S::CTAS, kThreads, S::SMEM, stream>>>(p, tmap);
     return cudaGetLastError();

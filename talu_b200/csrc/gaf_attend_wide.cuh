@@ -664,7 +664,8 @@ template <int D, int BITS, int GROUP>
 cudaError_t launch_wide(const Params &p, const CUtensorMap &tmap, int sm_count, cudaStream_t stream) {
     using W = Wide<D, BITS, GROUP>;
     auto kernel = gaf_attend_wide_kernel<D, BITS, GROUP>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W::SMEM);
+    static DeviceOnce once;    // of this instance
+    const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W::SMEM); });
     if (e != cudaSuccess) return e;
     kernel<<<sm_count, kWideThreads, W::SMEM, stream>>>(p, tmap);
     return cudaGetLastError();

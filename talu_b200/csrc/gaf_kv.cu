@@ -108,99 +108,177 @@ struct KvRows {
     KvStrides st[2];
 };
 
-// Thread = 8 values of one (token, K or V, head); the group's lanes (G / 8 neighbours) share minimum and maximum.
+// Both kernels: a CTA takes `tokens` packed rows; it looks up where they lie once, and its threads then walk the rows'
+// vectors of 8 values (K heads, then V heads).  What bounds them: HBM, with enough rows; the index arithmetic has to stay
+// small beside 8 values' work, so it is carried from step to step and each thread has kUnroll loads in flight.
+constexpr int kMaxTokens = 32;    // of a CTA
+constexpr int kUnroll = 4;
+
+struct Walk {                     // position of a thread in the vectors of the CTA's rows
+    uint32_t token, v;
+    uint32_t step_token, step_v, per_token, per_row_inv;   // the last: 2^32 over the vectors of a row, rounded up
+    __device__ __forceinline__ void next() {
+        v += step_v;
+        token += step_token;
+        if (v >= per_token) v -= per_token, ++token;
+    }
+};
+__device__ __forceinline__ Walk walk_rows(const KvView &kv, const KvSeqs &seqs, uint32_t tokens, int64_t *s_row, unsigned int *error_word) {
+    for (uint32_t x = threadIdx.x; x < tokens; x += kThreadsKv) {
+        const uint64_t t = static_cast<uint64_t>(blockIdx.x) * tokens + x;
+        s_row[x] = t < seqs.total ? row_of(kv, seqs, static_cast<uint32_t>(t), error_word) : -1;
+    }
+    __syncthreads();
+    Walk w;
+    w.per_token = 2u * kv.kv_heads * (kv.head_dim >> 3);
+    w.token = threadIdx.x / w.per_token;
+    w.v = threadIdx.x - w.token * w.per_token;
+    w.step_token = kThreadsKv / w.per_token;
+    w.step_v = kThreadsKv - w.step_token * w.per_token;
+    w.per_row_inv = 0xFFFFFFFFu / (kv.head_dim >> 3) + 1u;
+    return w;
+}
+struct Place {
+    uint32_t which, head, vec;
+    uint64_t token;
+    int64_t row;     // of the cache; -1: none
+};
+__device__ __forceinline__ Place place_of(const KvView &kv, const Walk &w, uint32_t tokens, const int64_t *s_row) {
+    const uint32_t per_row = kv.head_dim >> 3;       // at most 32, so that the product is exact for v below 2^27
+    const uint32_t h = __umulhi(w.v, w.per_row_inv);
+    Place p;
+    p.vec = w.v - h * per_row;
+    p.which = h >= kv.kv_heads ? 1u : 0u;
+    p.head = h - p.which * kv.kv_heads;
+    p.token = static_cast<uint64_t>(blockIdx.x) * tokens + w.token;
+    const int64_t row0 = w.token < tokens ? s_row[w.token] : -1;
+    p.row = row0 < 0 ? -1 : row0 + (static_cast<int64_t>(h) << kv.page_shift);
+    return p;
+}
+
+// The group's lanes (G / 8 neighbours) share minimum and maximum.
 template <bool F32, bool VEC>
-__global__ void __launch_bounds__(kThreadsKv) gaf_kv_append_kernel(const KvView kv, const KvSeqs seqs, const KvRows in,
+__global__ void __launch_bounds__(kThreadsKv) gaf_kv_append_kernel(const KvView kv, const KvSeqs seqs, const KvRows in, uint32_t tokens,
                                                                    unsigned int *error_word) {
-    const uint32_t per_row = kv.head_dim >> 3;
-    const uint64_t total = static_cast<uint64_t>(seqs.total) * 2u * kv.kv_heads * per_row;
-    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kThreadsKv + threadIdx.x;
-    const bool live = at < total;
-    const uint64_t row_id = (live ? at : total - 1) / per_row;
-    const uint32_t vec = static_cast<uint32_t>((live ? at : total - 1) % per_row);
-    const uint32_t head = static_cast<uint32_t>(row_id % kv.kv_heads);
-    const uint32_t which = static_cast<uint32_t>(row_id / kv.kv_heads) & 1u;
-    const uint32_t t = static_cast<uint32_t>(row_id / (2u * kv.kv_heads));
-    const int64_t row0 = row_of(kv, seqs, t, error_word);
-    float x[8];
-    load8<F32, VEC>(in.x[which], t * in.st[which].token + head * in.st[which].head + vec * 8u, x);
-    float lo = x[0], hi = x[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        lo = -max_nan(-lo, -x[i]);
-        hi = max_nan(hi, x[i]);
-    }
-    for (uint32_t o = kv.group >> 4; o >= 1u; o >>= 1) {
-        lo = -max_nan(-lo, -__shfl_xor_sync(0xFFFFFFFFu, lo, o));
-        hi = max_nan(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
-    }
+    __shared__ int64_t s_row[kMaxTokens];
+    Walk walk = walk_rows(kv, seqs, tokens, s_row, error_word);
+    const uint32_t steps = (tokens * walk.per_token + kThreadsKv - 1u) / kThreadsKv;
     const float maxq = kv.bits == 4u ? 15.0f : 255.0f;
-    const float range = 0.5f * hi - 0.5f * lo;             // of halves: finite for finite values
-    uint32_t sraw = f32_bf16(__fdiv_rn(range, 0.5f * maxq)), braw = f32_bf16(lo);
-    if ((braw & 0x7FFFu) == 0x7F80u) braw -= 1u;           // f32 values beyond the largest bf16
-    float s = bf16_f32(sraw);
-    if (s < FLT_MIN) s = 0.0f, sraw = 0u;
-    const bool finite = range <= FLT_MAX;
-    if (!finite) sraw = braw = 0x7FC0u, s = 0.0f;          // an infinity or a NaN in the group
-    const float half_b = 0.5f * bf16_f32(braw), half_s = 0.5f * s;
-    const float r = s > 0.0f ? __frcp_rn(half_s) : 0.0f;
-    uint32_t q[8];
+    for (uint32_t step = 0; step < steps; step += kUnroll) {
+        Place pl[kUnroll];
+        float x[kUnroll][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float u = __fsub_rn(0.5f * x[i], half_b);
-        float c = u * r;
-        // the product is within 2^-15 of the quotient: only next to a tie does the division decide the code
-        if (s > 0.0f && fabsf(c - rintf(c)) > 0.4995f) c = __fdiv_rn(u, half_s);
-        q[i] = finite ? static_cast<uint32_t>(fminf(fmaxf(rintf(c), 0.0f), maxq)) : 0u;
-    }
-    if (!live || row0 < 0) return;
-    const int64_t row = row0 + ((static_cast<int64_t>(which) * kv.kv_heads + head) << kv.page_shift);
-    uint8_t *dst = kv.packed + row * kv.row_bytes + vec * kv.bits;   // 8 codes are `bits` bytes
-    if (kv.bits == 8u) {
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
-    } else {
-        uint32_t w = 0u;
+        for (int k = 0; k < kUnroll; ++k, walk.next()) {
+            pl[k] = place_of(kv, walk, tokens, s_row);
+            if (pl[k].row >= 0) {
+                load8<F32, VEC>(in.x[pl[k].which], pl[k].token * in.st[pl[k].which].token + pl[k].head * in.st[pl[k].which].head + pl[k].vec * 8u, x[k]);
+            } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w |= q[i] << (4 * i);
-        *reinterpret_cast<uint32_t *>(dst) = w;
-    }
-    if ((vec & ((kv.group >> 3) - 1u)) == 0u) {
-        const int64_t g = row * kv.groups + (vec * 8u >> kv.group_shift);
-        kv.scales[g] = static_cast<uint16_t>(sraw);
-        kv.biases[g] = static_cast<uint16_t>(braw);
+                for (int i = 0; i < 8; ++i) x[k][i] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            if (step + k >= steps) break;
+            float lo = x[k][0], hi = x[k][0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) {
+                lo = -max_nan(-lo, -x[k][i]);
+                hi = max_nan(hi, x[k][i]);
+            }
+            for (uint32_t o = kv.group >> 4; o >= 1u; o >>= 1) {
+                lo = -max_nan(-lo, -__shfl_xor_sync(0xFFFFFFFFu, lo, o));
+                hi = max_nan(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
+            }
+            const float range = 0.5f * hi - 0.5f * lo;             // of halves: finite for finite values
+            uint32_t sraw = f32_bf16(__fdiv_rn(range, 0.5f * maxq)), braw = f32_bf16(lo);
+            if ((braw & 0x7FFFu) == 0x7F80u) braw -= 1u;           // f32 values beyond the largest bf16
+            float s = bf16_f32(sraw);
+            if (s < FLT_MIN) s = 0.0f, sraw = 0u;
+            const bool finite = range <= FLT_MAX;
+            if (!finite) sraw = braw = 0x7FC0u, s = 0.0f;          // an infinity or a NaN in the group
+            const float half_b = 0.5f * bf16_f32(braw), half_s = 0.5f * s;
+            const float r = s > 0.0f ? __frcp_rn(half_s) : 0.0f;
+            // adding 1.5 * 2^23 rounds to an integer (ties to even) and leaves it in the low bits
+            constexpr float kMagic = 12582912.0f;
+            uint32_t q[8];
+            float off = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float c = fminf(fmaxf(fmaf(0.5f, x[k][i], -half_b) * r, 0.0f), maxq);
+                const float y = c + kMagic;
+                off = fmaxf(off, fabsf(c - (y - kMagic)));
+                q[i] = __float_as_uint(y) & 0xFFu;
+            }
+            if (off > 0.4995f) {
+                // the product is within 2^-15 of the quotient: only next to a tie does the division decide the code
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    q[i] = __float_as_uint(fminf(fmaxf(__fdiv_rn(fmaf(0.5f, x[k][i], -half_b), half_s), 0.0f), maxq) + kMagic) & 0xFFu;
+            }
+            if (!finite) q[0] = q[1] = q[2] = q[3] = q[4] = q[5] = q[6] = q[7] = 0u;
+            if (pl[k].row < 0) continue;
+            uint8_t *dst = kv.packed + pl[k].row * kv.row_bytes + pl[k].vec * kv.bits;   // 8 codes are `bits` bytes
+            if (kv.bits == 8u) {
+                *reinterpret_cast<uint2 *>(dst) = make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
+            } else {
+                uint32_t w = 0u;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w |= q[i] << (4 * i);
+                *reinterpret_cast<uint32_t *>(dst) = w;
+            }
+            if ((pl[k].vec & ((kv.group >> 3) - 1u)) == 0u) {
+                const int64_t g = pl[k].row * kv.groups + (pl[k].vec * 8u >> kv.group_shift);
+                kv.scales[g] = static_cast<uint16_t>(sraw);
+                kv.biases[g] = static_cast<uint16_t>(braw);
+            }
+        }
     }
 }
 
-// Thread = 8 values of one (token, K or V, head).
 template <bool F32, bool VEC>
-__global__ void __launch_bounds__(kThreadsKv) gaf_kv_read_kernel(const KvView kv, const KvSeqs seqs, const KvRows out,
+__global__ void __launch_bounds__(kThreadsKv) gaf_kv_read_kernel(const KvView kv, const KvSeqs seqs, const KvRows out, uint32_t tokens,
                                                                  unsigned int *error_word) {
-    const uint32_t per_row = kv.head_dim >> 3;
-    const uint64_t total = static_cast<uint64_t>(seqs.total) * 2u * kv.kv_heads * per_row;
-    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kThreadsKv + threadIdx.x;
-    if (at >= total) return;
-    const uint64_t row_id = at / per_row;
-    const uint32_t vec = static_cast<uint32_t>(at % per_row);
-    const uint32_t head = static_cast<uint32_t>(row_id % kv.kv_heads);
-    const uint32_t which = static_cast<uint32_t>(row_id / kv.kv_heads) & 1u;
-    const uint32_t t = static_cast<uint32_t>(row_id / (2u * kv.kv_heads));
-    const int64_t row0 = row_of(kv, seqs, t, error_word);
-    if (row0 < 0) return;
-    const int64_t row = row0 + ((static_cast<int64_t>(which) * kv.kv_heads + head) << kv.page_shift);
-    const uint8_t *src = kv.packed + row * kv.row_bytes + vec * kv.bits;
-    const int64_t g = row * kv.groups + (vec * 8u >> kv.group_shift);
-    const float s = bf16_f32(kv.scales[g]), b = bf16_f32(kv.biases[g]);
-    float x[8];
-    if (kv.bits == 8u) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(src);
+    __shared__ int64_t s_row[kMaxTokens];
+    Walk walk = walk_rows(kv, seqs, tokens, s_row, error_word);
+    const uint32_t steps = (tokens * walk.per_token + kThreadsKv - 1u) / kThreadsKv;
+    for (uint32_t step = 0; step < steps; step += kUnroll) {
+        Place pl[kUnroll];
+        uint2 code[kUnroll];
+        float s[kUnroll], b[kUnroll];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fmaf(static_cast<float>(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xFFu), s, b);
-    } else {
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(src);
+        for (int k = 0; k < kUnroll; ++k, walk.next()) {
+            pl[k] = place_of(kv, walk, tokens, s_row);
+            if (pl[k].row < 0) continue;
+            const uint8_t *src = kv.packed + pl[k].row * kv.row_bytes + pl[k].vec * kv.bits;
+            if (kv.bits == 8u) code[k] = *reinterpret_cast<const uint2 *>(src);
+            else code[k].x = *reinterpret_cast<const uint32_t *>(src);
+            const int64_t g = pl[k].row * kv.groups + (pl[k].vec * 8u >> kv.group_shift);
+            s[k] = bf16_f32(kv.scales[g]);
+            b[k] = bf16_f32(kv.biases[g]);
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fmaf(static_cast<float>((w >> (4 * i)) & 15u), s, b);
+        for (int k = 0; k < kUnroll; ++k) {
+            if (pl[k].row < 0) continue;
+            float x[8];
+            if (kv.bits == 8u) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)      // 2^23 + code, less 2^23
+                    x[i] = fmaf(__uint_as_float(attend::prmt(i < 4 ? code[k].x : code[k].y, 0x4B000000u, 0x7650u | (i & 3))) - 8388608.0f, s[k], b[k]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = fmaf(static_cast<float>((code[k].x >> (4 * i)) & 15u), s[k], b[k]);
+            }
+            store8<F32, VEC>(const_cast<void *>(out.x[pl[k].which]),
+                             pl[k].token * out.st[pl[k].which].token + pl[k].head * out.st[pl[k].which].head + pl[k].vec * 8u, x);
+        }
     }
-    store8<F32, VEC>(const_cast<void *>(out.x[which]), t * out.st[which].token + head * out.st[which].head + vec * 8u, x);
+}
+
+// Rows of a CTA: as many as leave eight CTAs for each SM, so that the look-up in front of them is paid seldom and hidden
+uint32_t rows_of_cta(const KvSeqs &seqs) {
+    const uint32_t n = seqs.total / (148u * 8u);
+    return n < 1u ? 1u : n < static_cast<uint32_t>(kMaxTokens) ? n : kMaxTokens;
 }
 
 bool vec_ok(const void *p, KvStrides st, bool f32) {
@@ -317,29 +395,27 @@ __global__ void __launch_bounds__(kWarpsGen * 32) gaf_attention_generic_kernel(c
 
 cudaError_t kv_append(const KvView &kv, const KvSeqs &seqs, bool f32, const void *k, KvStrides ks, const void *v, KvStrides vs,
                       unsigned int *error_word, cudaStream_t stream) {
-    const uint64_t n = static_cast<uint64_t>(seqs.total) * 2u * kv.kv_heads * (kv.head_dim / 8u);
-    if (n == 0) return cudaSuccess;
+    if (seqs.total == 0) return cudaSuccess;
     const KvRows in = {{k, v}, {ks, vs}};
     const bool vec = vec_ok(k, ks, f32) && vec_ok(v, vs, f32);
-    const unsigned int grid = static_cast<unsigned int>((n + kThreadsKv - 1) / kThreadsKv);
-    if (f32 && vec) gaf_kv_append_kernel<true, true><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, error_word);
-    else if (f32) gaf_kv_append_kernel<true, false><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, error_word);
-    else if (vec) gaf_kv_append_kernel<false, true><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, error_word);
-    else gaf_kv_append_kernel<false, false><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, error_word);
+    const uint32_t n = rows_of_cta(seqs), grid = (seqs.total - 1u) / n + 1u;
+    if (f32 && vec) gaf_kv_append_kernel<true, true><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, n, error_word);
+    else if (f32) gaf_kv_append_kernel<true, false><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, n, error_word);
+    else if (vec) gaf_kv_append_kernel<false, true><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, n, error_word);
+    else gaf_kv_append_kernel<false, false><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, n, error_word);
     return cudaGetLastError();
 }
 
 cudaError_t kv_read(const KvView &kv, const KvSeqs &seqs, bool f32, void *k, KvStrides ks, void *v, KvStrides vs,
                     unsigned int *error_word, cudaStream_t stream) {
-    const uint64_t n = static_cast<uint64_t>(seqs.total) * 2u * kv.kv_heads * (kv.head_dim / 8u);
-    if (n == 0) return cudaSuccess;
+    if (seqs.total == 0) return cudaSuccess;
     const KvRows out = {{k, v}, {ks, vs}};
     const bool vec = vec_ok(k, ks, f32) && vec_ok(v, vs, f32);
-    const unsigned int grid = static_cast<unsigned int>((n + kThreadsKv - 1) / kThreadsKv);
-    if (f32 && vec) gaf_kv_read_kernel<true, true><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, error_word);
-    else if (f32) gaf_kv_read_kernel<true, false><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, error_word);
-    else if (vec) gaf_kv_read_kernel<false, true><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, error_word);
-    else gaf_kv_read_kernel<false, false><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, error_word);
+    const uint32_t n = rows_of_cta(seqs), grid = (seqs.total - 1u) / n + 1u;
+    if (f32 && vec) gaf_kv_read_kernel<true, true><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, n, error_word);
+    else if (f32) gaf_kv_read_kernel<true, false><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, n, error_word);
+    else if (vec) gaf_kv_read_kernel<false, true><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, n, error_word);
+    else gaf_kv_read_kernel<false, false><<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, n, error_word);
     return cudaGetLastError();
 }
 

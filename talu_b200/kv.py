@@ -12,45 +12,54 @@ follows them from replay to replay.  Calls only enqueue on the context's stream.
 from __future__ import annotations
 
 import ctypes as C
-import math
 
 from . import _capi
 from .gaf import DTYPE_BF16, DTYPE_F32, Context, GafError, _STATUS_INVALID_ARGUMENT
+
+
+_BF16 = _F32 = _I32 = None   # torch's dtypes, once torch is loaded
+
+
+def _torch():
+    global _BF16, _F32, _I32
+    import torch
+    _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 
 
 def _refuse(message: str):
     raise GafError(_STATUS_INVALID_ARGUMENT, message)
 
 
-def _check_device(ctx: Context, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and (t.device.type != "cuda" or t.device.index != ctx.device):
-            _refuse(f"{name} must be on cuda:{ctx.device}, got {t.device}")
+# The checks below run in front of every launch of a decoder step, so they ask each tensor once for what they need
+# (get_device() is the device's index, -1 on the CPU).
 
-
-def _dtype_tag(name: str, dtype) -> int:
-    import torch
-    tag = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}.get(dtype)
-    if tag is None:
+def _tag(name: str, dtype) -> int:
+    if _BF16 is None:
+        _torch()
+    if dtype is _BF16:
+        return DTYPE_BF16
+    if dtype is not _F32:
         _refuse(f"{name} must be bf16 or f32, got {dtype}")
-    return tag
+    return DTYPE_F32
 
 
-def _check_rows(name: str, t, heads: int, head_dim: int) -> None:
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
-        _refuse(f"{name} must be [tokens, {heads}, {head_dim}], got {tuple(t.shape)}")
-    if t.stride(2) != 1:
+def _rows(ctx: Context, name: str, t, heads: int, head_dim: int, written: bool = False):
+    """Rows of `t` and its pointer, token stride and head stride, if it is [rows, heads, head_dim] on the context's device."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
+        _refuse(f"{name} must be [tokens, {heads}, {head_dim}], got {tuple(shape)}")
+    if stride[2] != 1:
         _refuse(f"{name} must be contiguous along its last axis")
-
-
-def _check_written(name: str, t) -> None:
-    """A tensor that is written must not name one place twice."""
-    reach = 1
-    for stride, size in sorted(zip(t.stride(), t.shape)):
-        if size > 1:
-            if stride < reach:
-                _refuse(f"{name} must not overlap itself")
-            reach = stride * size
+    if t.get_device() != ctx.device:
+        _refuse(f"{name} must be on cuda:{ctx.device}, got {t.device}")
+    if written:        # a tensor that is written must not name one place twice
+        reach = 1
+        for step, size in sorted(zip(stride, shape)):
+            if size > 1:
+                if step < reach:
+                    _refuse(f"{name} must not overlap itself")
+                reach = step * size
+    return shape[0], (t.data_ptr(), stride[0], stride[1])
 
 
 class KvCache:
@@ -80,7 +89,9 @@ class KvCache:
                 _refuse(f"{name} must be bf16 (or int16 bit patterns) {want}, got {t.dtype} {tuple(t.shape)}")
         if not (packed.is_contiguous() and scales.is_contiguous() and biases.is_contiguous()):
             _refuse("cache buffers must be contiguous")
-        _check_device(ctx, packed=packed, scales=scales, biases=biases)
+        for name, t in (("packed", packed), ("scales", scales), ("biases", biases)):
+            if t.get_device() != ctx.device:
+                _refuse(f"{name} must be on cuda:{ctx.device}, got {t.device}")
         h = C.c_void_p()
         ctx._check(ctx._lib.tgaf_kv_cache_wrap_device(
             ctx._h, C.c_void_p(packed.data_ptr()), C.c_void_p(scales.data_ptr()), C.c_void_p(biases.data_ptr()), packed.shape[0],
@@ -112,93 +123,99 @@ class KvCache:
 
 
 def _seqs(ctx: Context, table, lens, cu, total: int) -> _capi.KvSeqs:
-    import torch
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        _refuse(f"table must be int32 [batch, pages] with contiguous rows, got {table.dtype} {tuple(table.shape)}")
-    batch = table.shape[0]
-    if lens.dtype != torch.int32 or tuple(lens.shape) != (batch,) or not lens.is_contiguous():
+    device = ctx.device
+    shape = table.shape
+    if table.dtype is not _I32 or len(shape) != 2:
+        _refuse(f"table must be int32 [batch, pages], got {table.dtype} {tuple(shape)}")
+    batch, width = shape
+    stride, inner = table.stride()
+    if (inner != 1 and width > 1) or (stride < width and batch > 1):
+        _refuse("table must have contiguous rows that do not overlap")
+    if lens.dtype is not _I32 or lens.shape != (batch,) or not lens.is_contiguous():
         _refuse(f"lens must be contiguous int32 [{batch}], got {lens.dtype} {tuple(lens.shape)}")
-    if cu is not None and (cu.dtype != torch.int32 or tuple(cu.shape) != (batch + 1,) or not cu.is_contiguous()):
-        _refuse(f"cu must be contiguous int32 [{batch + 1}], got {cu.dtype} {tuple(cu.shape)}")
-    if cu is None and (total % batch if batch else total):
+    if table.get_device() != device or lens.get_device() != device:
+        _refuse(f"table and lens must be on cuda:{device}, got {table.device} and {lens.device}")
+    at = None
+    if cu is not None:
+        if cu.dtype is not _I32 or cu.shape != (batch + 1,) or not cu.is_contiguous():
+            _refuse(f"cu must be contiguous int32 [{batch + 1}], got {cu.dtype} {tuple(cu.shape)}")
+        if cu.get_device() != device:
+            _refuse(f"cu must be on cuda:{device}, got {cu.device}")
+        at = cu.data_ptr()
+    elif total % batch if batch else total:
         _refuse(f"{total} rows are no equal share of {batch} sequences: give cu")
-    _check_device(ctx, table=table, lens=lens, cu=cu)
-    stride = table.stride(0) if batch > 1 else max(table.stride(0), table.shape[1])
-    if stride < table.shape[1]:
-        _refuse("table rows must not overlap")
-    return _capi.KvSeqs(table.data_ptr(), stride, table.shape[1], batch, lens.data_ptr(), cu.data_ptr() if cu is not None else None, total)
-
-
-def _row_args(t):
-    return C.c_void_p(t.data_ptr()), t.stride(0), t.stride(1)
+    return _capi.KvSeqs(table.data_ptr(), stride if batch > 1 else max(stride, width), width, batch, lens.data_ptr(), at, total)
 
 
 def kv_append(ctx: Context, cache: KvCache, k, v, table, lens, cu=None) -> None:
     """Quantises the call's own rows k, v [tokens, kv_heads, head_dim] (bf16 or f32, any token and head strides) into the
     sequences' pages (tgaf_kv_append).  lens counts them already; without cu every sequence has tokens / batch of them."""
-    tag = _dtype_tag("k", k.dtype)
-    for name, t in (("k", k), ("v", v)):
-        _check_rows(name, t, cache.kv_heads, cache.head_dim)
-    if v.dtype != k.dtype or v.shape[0] != k.shape[0]:
-        _refuse(f"k and v must have one dtype and length, got {k.dtype} {k.shape[0]} and {v.dtype} {v.shape[0]}")
-    _check_device(ctx, k=k, v=v)
-    s = _seqs(ctx, table, lens, cu, k.shape[0])
-    ctx._check(ctx._lib.tgaf_kv_append(ctx._h, cache._h, C.byref(s), tag, *_row_args(k), *_row_args(v)))
+    tag = _tag("k", k.dtype)
+    total, k_args = _rows(ctx, "k", k, cache.kv_heads, cache.head_dim)
+    v_rows, v_args = _rows(ctx, "v", v, cache.kv_heads, cache.head_dim)
+    if v.dtype is not k.dtype or v_rows != total:
+        _refuse(f"k and v must have one dtype and length, got {k.dtype} {total} and {v.dtype} {v_rows}")
+    seqs = _seqs(ctx, table, lens, cu, total)
+    st = ctx._lib.tgaf_kv_append(ctx._h, cache._h, seqs, tag, *k_args, *v_args)
+    if st:
+        ctx._check(st)
 
 
 def kv_read(ctx: Context, cache: KvCache, table, lens, cu=None, total: int | None = None, dtype=None, out=None):
     """The rows that kv_append with the same table, lens and cu wrote, read back: (k, v), each [total, kv_heads, head_dim],
     bf16 (default) or f32 (tgaf_kv_read).  total: rows of the call, needed unless `out` = (k, v) is given; whole sequences
     are cu = cumulated lens.  Rows that lie in no sequence are left as they were (undefined in new tensors)."""
-    import torch
+    if _BF16 is None:
+        _torch()
     if out is None:
         if total is None:
             _refuse("total (or out) is needed")
-        dtype = torch.bfloat16 if dtype is None else dtype
-        _dtype_tag("dtype", dtype)
-        shape, dev = (total, cache.kv_heads, cache.head_dim), f"cuda:{ctx.device}"
-        out = (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
-    k, v = out
-    tag = _dtype_tag("out", k.dtype)
-    for name, t in (("out k", k), ("out v", v)):
-        _check_rows(name, t, cache.kv_heads, cache.head_dim)
-        _check_written(name, t)
-    if v.dtype != k.dtype or v.shape[0] != k.shape[0] or (total is not None and total != k.shape[0]):
-        _refuse("out k and v must have one dtype and `total` rows")
-    _check_device(ctx, k=k, v=v)
-    s = _seqs(ctx, table, lens, cu, k.shape[0])
-    ctx._check(ctx._lib.tgaf_kv_read(ctx._h, cache._h, C.byref(s), tag, *_row_args(k), *_row_args(v)))
+        tag, rows = DTYPE_BF16 if dtype is None else _tag("dtype", dtype), total
+        seqs = _seqs(ctx, table, lens, cu, rows)
+        k, v = cache.scales.new_empty((2, total, cache.kv_heads, cache.head_dim), dtype=dtype or _BF16).unbind(0)
+        at, step = k.data_ptr(), cache.kv_heads * cache.head_dim
+        k_args, v_args = (at, step, cache.head_dim), (v.data_ptr(), step, cache.head_dim)
+    else:
+        k, v = out
+        tag = _tag("out", k.dtype)
+        rows, k_args = _rows(ctx, "out k", k, cache.kv_heads, cache.head_dim, True)
+        v_rows, v_args = _rows(ctx, "out v", v, cache.kv_heads, cache.head_dim, True)
+        if v.dtype is not k.dtype or v_rows != rows or (total is not None and total != rows):
+            _refuse("out k and v must have one dtype and `total` rows")
+        seqs = _seqs(ctx, table, lens, cu, rows)
+    st = ctx._lib.tgaf_kv_read(ctx._h, cache._h, seqs, tag, *k_args, *v_args)
+    if st:
+        ctx._check(st)
     return k, v
 
 
-def _attend(ctx: Context, cache: KvCache, q, prefix_table, prefix_len: int, table, lens, cu, max_new, scale, out):
-    import torch
-    tag = _dtype_tag("q", q.dtype)
-    if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % cache.kv_heads:
-        _refuse(f"q must be [tokens, heads, {cache.head_dim}] with heads a multiple of {cache.kv_heads}, got {tuple(q.shape)}")
-    _check_rows("q", q, q.shape[1], cache.head_dim)
-    _check_device(ctx, q=q)
-    s = _seqs(ctx, table, lens, cu, q.shape[0])
+def _attend(ctx: Context, cache: KvCache, q, prefix_at, prefix_len: int, table, lens, cu, max_new, scale, out):
+    tag = _tag("q", q.dtype)
+    heads, head_dim = q.shape[1] if q.dim() == 3 else 0, cache.head_dim
+    if heads == 0 or heads % cache.kv_heads:
+        _refuse(f"q must be [tokens, heads, {head_dim}] with heads a multiple of {cache.kv_heads}, got {tuple(q.shape)}")
+    total, q_args = _rows(ctx, "q", q, heads, head_dim)
+    seqs = _seqs(ctx, table, lens, cu, total)
     if max_new is None:
         if cu is not None:
             _refuse("max_new is needed with cu")
-        max_new = q.shape[0] // max(1, table.shape[0])
-    scale = 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale)
+        max_new = total // max(1, seqs.batch)
     if out is None:
-        out = torch.empty((q.shape[0], q.shape[1], cache.head_dim), dtype=q.dtype, device=q.device)
+        out = q.new_empty((total, heads, head_dim))
+        out_args = (out.data_ptr(), heads * head_dim, head_dim)
     else:
-        _check_rows("out", out, q.shape[1], cache.head_dim)
-        _check_written("out", out)
-        if out.dtype != q.dtype or out.shape[0] != q.shape[0]:
-            _refuse(f"out must be {q.dtype} with {q.shape[0]} rows")
-        _check_device(ctx, out=out)
-    if q.shape[0] == 0:
+        out_rows, out_args = _rows(ctx, "out", out, heads, head_dim, True)
+        if out.dtype is not q.dtype or out_rows != total:
+            _refuse(f"out must be {q.dtype} with {total} rows")
+    if total == 0:
         return out
-    tail = (tag, *_row_args(q), q.shape[1], int(max_new), scale, *_row_args(out))
-    if prefix_table is None:
-        ctx._check(ctx._lib.tgaf_attention(ctx._h, cache._h, C.byref(s), *tail))
+    scale = head_dim ** -0.5 if scale is None else scale
+    if prefix_at is None:
+        st = ctx._lib.tgaf_attention(ctx._h, cache._h, seqs, tag, *q_args, heads, max_new, scale, *out_args)
     else:
-        ctx._check(ctx._lib.tgaf_attention_shared_prefix(ctx._h, cache._h, C.c_void_p(prefix_table.data_ptr()), prefix_len, C.byref(s), *tail))
+        st = ctx._lib.tgaf_attention_shared_prefix(ctx._h, cache._h, prefix_at, prefix_len, seqs, tag, *q_args, heads, max_new, scale, *out_args)
+    if st:
+        ctx._check(st)
     return out
 
 
@@ -216,11 +233,11 @@ def attention_shared_prefix(ctx: Context, cache: KvCache, q, prefix_table, prefi
     """`attention` for sequences that all continue one shared prefix of `prefix_len` tokens in the pages `prefix_table`
     (int32 [pages], on the device); table and lens do not count the prefix.  Its pages are read once for the whole batch
     (tgaf_attention_shared_prefix)."""
-    import torch
-    prefix_len = int(prefix_len)
-    if prefix_table.dtype != torch.int32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous():
+    _tag("q", q.dtype)
+    if prefix_table.dtype is not _I32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous():
         _refuse(f"prefix_table must be contiguous int32 [pages], got {prefix_table.dtype} {tuple(prefix_table.shape)}")
     if prefix_len < 0 or prefix_len > prefix_table.shape[0] * cache.page_tokens:
         _refuse(f"prefix_len {prefix_len} does not fit {prefix_table.shape[0]} pages of {cache.page_tokens} tokens")
-    _check_device(ctx, prefix_table=prefix_table)
-    return _attend(ctx, cache, q, prefix_table, prefix_len, table, lens, cu, max_new, scale, out)
+    if prefix_table.get_device() != ctx.device:
+        _refuse(f"prefix_table must be on cuda:{ctx.device}, got {prefix_table.device}")
+    return _attend(ctx, cache, q, prefix_table.data_ptr(), int(prefix_len), table, lens, cu, max_new, scale, out)

@@ -20,13 +20,15 @@ class _FakeLib:
 
 class _FakeCtx:
     """Stands for a context whose device tensors are on the CPU: the checks run, no call may come through."""
-    device, _lib, _h = 0, _FakeLib(), 1
+    _lib, _h = _FakeLib(), 1
+
+    def __init__(self, device=-1):         # -1: what a tensor on the CPU gives as its device's index
+        self.device = device
 
 
 @pytest.fixture
-def fake(monkeypatch):
+def fake():
     from talu_b200 import kv
-    monkeypatch.setattr(kv, "_check_device", lambda ctx, **t: None)
     packed = torch.zeros(4, 2, 2, 16, 16, dtype=torch.int32)
     scales = torch.zeros(4, 2, 2, 16, 1, dtype=torch.bfloat16)
     return kv.KvCache(_FakeCtx(), None, packed, scales, scales, 64, 8)
@@ -107,11 +109,12 @@ def test_tensors_off_the_device_are_refused():
     packed = torch.zeros(4, 2, 2, 16, 16, dtype=torch.int32)
     scales = torch.zeros(4, 2, 2, 16, 1, dtype=torch.bfloat16)
     with pytest.raises(GafError):
-        KvCache.wrap_device(_FakeCtx(), packed, scales, scales, 64, 8)
-    cache = kv.KvCache(_FakeCtx(), None, packed, scales, scales, 64, 8)
+        KvCache.wrap_device(_FakeCtx(0), packed, scales, scales, 64, 8)
+    cache = kv.KvCache(_FakeCtx(0), None, packed, scales, scales, 64, 8)
     x, table, lens = _args()
-    with pytest.raises(GafError):
+    with pytest.raises(GafError) as e:
         kv.kv_append(cache.ctx, cache, x, x, table, lens)
+    assert "cuda:0" in e.value.message
 
 
 def test_null_arguments_at_the_c_entries():
