@@ -3,14 +3,17 @@
 //   out[r] = sum_j softmax_j(scale q_r . K_j) V_j,   K_jd = c_jd s_jg + b_jg (codes c, scale s and bias b of group g of d)
 //
 // Mathematics.  The affine map is taken out of the sums, so that the matrix products run on the codes as they are (exact in
-// f16 and bf16) and neither keys nor values are rounded:
+// f16) and neither keys nor values are rounded:
 //   q_r . K_j  = sum_g s_jg (sum_{d in g} q_rd c_jd) + b_jg (sum_{d in g} q_rd)
 //   out_rd     = sum_j (p_rj s_jg) (c_jd - h) + sum_j p_rj (b_jg + h s_jg),   h = 2^(bits - 1)
 // q is scaled by a power of two per row (so that it fits f16, which holds bf16's 8 bits and the codes) and the products
-// p s are rounded to bf16 once (2^-9 of each; bf16 for its range, since s is the caller's); everything else is f32.  The
-// values' codes are centred because that rounding is relative to p s |c - h|: with plain codes it is relative to the
-// distance from the group's minimum, some four times the value itself (measured: 4.5e-3 against 64 bits, 2.0e-3 centred).
-// LIMBS = 2 (f32 q): q is split into two f16 terms (22 bits) and p s into three bf16 terms (24 bits).
+// p s are rounded to f16 once (2^-12 of each); everything else is f32.  The values' codes are centred because that
+// rounding is relative to p s |c - h|: with plain codes it is relative to the distance from the group's minimum, some four
+// times the value itself.  f16 and not bf16 for the products, although s is the caller's and of any size: unpacking a
+// code to f16 takes two instructions a pair, to bf16 (8 bits of code in 8 bits of mantissa) four.  The range is kept
+// by the softmax's own freedom: weights are formed against a reference m that need not be the largest score, so m follows
+// the largest y_j + log2 s_j (y: scores in base 2), and p s stays within 2^-14 and 2^13 for every key that counts.
+// LIMBS = 2 (f32 q): q and p s are split into two f16 terms each (22 bits).
 //
 // Both products are formed transposed (keys as the 16 rows of the MMA's A operand, query rows as its 8 columns): with one
 // new token and 4 or 8 query heads per cached head, 8 columns are what there is, and an A operand of query rows would leave
@@ -18,8 +21,8 @@
 //
 // What bounds it: the cache is read once (HBM), and every code is unpacked once (2 to 3 instructions per pair).  A unit is 64
 // keys of one (head, sequence, row tile): codes by TMA (swizzled, so that the fragment reads below hit every bank once),
-// scales and biases by bulk copies into the same ring stage.  Each of the four consumer warps owns 16 keys of the unit for
-// both products, with its own running maximum and sum: no barrier between warps but at the end of a segment.  The units of
+// scales and biases by bulk copies into the same ring stage.  A consumer warp owns 16 keys of every unit, or (8 rows) 32 keys of
+// every other unit, for both products, with its own reference and sum: no barrier between warps but at the end of a segment.  The units of
 // all items are cut into equal contiguous ranges over a grid that fills the GPU once, whatever the lengths are; an item cut
 // across CTAs is joined by the last CTA to finish, in CTA order (the result does not depend on timing).
 #pragma once
@@ -29,14 +32,17 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <type_traits>
 
 namespace tgaf {
 namespace attend {
 
 constexpr int kKeys = 64;                      // keys of a unit
-constexpr int kConsumers = 4;                  // consumer warps, 16 keys each
+constexpr int kConsumers = 4;                  // consumer warps
 constexpr int kThreads = (kConsumers + 1) * 32;
-constexpr float kLazy = 8.0f;                  // the running maximum follows only when a score exceeds it by 2^8
+constexpr float kLazy = 8.0f;                  // the reference follows only when it is exceeded by 2^8
+constexpr float kTarget = 4.0f;                // largest p s of a row when its reference is set: 2^4 to 2^5
+constexpr float kNoMax = -3.0e38f;             // reference of a row that has seen no key: finite, so that -inf scores give 0
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ float bf16_f32(uint32_t raw) { return __uint_as_float(raw << 16); }
@@ -99,9 +105,14 @@ __device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
     asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-__device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t r;
-    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
@@ -121,11 +132,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -331,6 +337,8 @@ struct Shape {
     static constexpr int HALVES = NT >= 2 && NP >= 2 ? 2 : 1;   // the warps' sums are joined D / HALVES values at a time
     static constexpr int OW = D / HALVES + 4;              // pitch of a joined row (floats)
     static constexpr int JOIN = kConsumers * R * OW * 4;
+    static constexpr int H = NT == 1 && LIMBS == 1 ? 2 : 1;    // 16-key tiles of a warp in a unit
+    static constexpr int TURNS = H;                        // units among which the warps take turns
     static constexpr int CTAS = NT >= 2 ? 2 : 3;           // per SM
     static constexpr int FIXED = QF + JOIN + 1024;
     static constexpr int FIT = (226 * 1024 / CTAS - 2048 - FIXED) / STAGE;
@@ -360,6 +368,15 @@ __device__ __forceinline__ void lds(uint32_t addr, uint32_t *w) {
     else if (BYTES == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
     else asm volatile("{\n\t.reg .u16 h;\n\tld.shared.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(w[0]) : "r"(addr));
 }
+// Floor of log2 of a key's largest scale, kept where 2^-it times the weights stays finite; a scale that is not finite lends nothing.
+template <int GS>
+__device__ __forceinline__ float key_exponent(const float (&v)[GS]) {
+    float top = fabsf(v[0]);
+#pragma unroll
+    for (int i = 1; i < GS; ++i) top = fmaxf(top, fabsf(v[i]));
+    const float e = static_cast<float>(static_cast<int>(__float_as_uint(top) >> 23) - 127);
+    return top <= 3.4e38f ? fmaxf(e, -40.0f) : -40.0f;
+}
 // The GS bf16 values of a row of scales or biases.
 template <int GS>
 __device__ __forceinline__ void row_f32(uint32_t addr, float (&v)[GS]) {
@@ -368,17 +385,21 @@ __device__ __forceinline__ void row_f32(uint32_t addr, float (&v)[GS]) {
 #pragma unroll
     for (int i = 0; i < GS; ++i) v[i] = (i & 1) ? __uint_as_float(w[i >> 1] & 0xFFFF0000u) : bf16_f32(w[i >> 1]);
 }
-// K codes of one word as two A registers of one k step: f16, exact.
+// Codes as f16, exact.  A byte under 0x64 reads 1024 + code.  Of a word of 4-bit codes the lower nibbles of its bytes read
+// 1024 + code and the upper ones, left where they are, 1024 + 16 code; the multiply-add takes out both.
+constexpr uint32_t kF16One16th = 0x2C002C00u;
+__device__ __forceinline__ uint32_t f16_low(uint32_t x, uint32_t minus) { return add_f16x2((x & 0x000F000Fu) | 0x64006400u, minus); }
+__device__ __forceinline__ uint32_t f16_high(uint32_t x, uint32_t minus) { return fma_f16x2((x & 0x00F000F0u) | 0x64006400u, kF16One16th, minus); }
+// K codes of one k step as two A registers.
 template <int BITS>
 __device__ __forceinline__ void k_codes(const uint32_t *w, int step, uint32_t &lo, uint32_t &hi) {
-    constexpr uint32_t kMinus1024 = 0xE400E400u;
     if (BITS == 8) {
-        lo = add_f16x2(prmt(w[step], 0x64646464u, 0x4140u), kMinus1024);
-        hi = add_f16x2(prmt(w[step], 0x64646464u, 0x4342u), kMinus1024);
+        lo = add_f16x2(prmt(w[step], 0x64646464u, 0x4140u), 0xE400E400u);
+        hi = add_f16x2(prmt(w[step], 0x64646464u, 0x4342u), 0xE400E400u);
     } else {
-        const uint32_t x = w[step >> 1] >> (8 * (step & 1));
-        lo = add_f16x2((x & 0x000F000Fu) | 0x64006400u, kMinus1024);
-        hi = add_f16x2(((x >> 4) & 0x000F000Fu) | 0x64006400u, kMinus1024);
+        const uint32_t x = (step & 1) ? w[step >> 1] >> 8 : w[step >> 1];
+        lo = f16_low(x, 0xE400E400u);
+        hi = f16_high(x, 0xD400D400u);       // -64
     }
 }
 // Element of q in a k step of the score product: what k_codes pairs with it.
@@ -395,14 +416,16 @@ __device__ __forceinline__ void q_place(uint32_t d, uint32_t &step, uint32_t &t,
         slot = (c & 1u) * 2u + (c >> 2);
     }
 }
-// V codes c of two keys' words, less 2^(bits - 1), as one A register: bf16, exact.
-__device__ __forceinline__ uint32_t v_codes8(uint32_t w0, uint32_t w1, int c) {
-    // 128 + (code & 127), less 128 where bit 7 is set and less 256 where it is clear
-    const uint32_t u = prmt(w0, w1, static_cast<uint32_t>(c | (c << 4) | ((4 + c) << 8) | ((4 + c) << 12)));
-    return add_bf16x2((u & 0x007F007Fu) | 0x43004300u, (~u & 0x00800080u) | 0xC300C300u);
+// V codes c and c + 1 (less 2^(bits - 1)) of two keys' words as an A register each.
+__device__ __forceinline__ void v_codes8(uint32_t w0, uint32_t w1, int c, uint32_t &first, uint32_t &second) {
+    const uint32_t x = prmt(w0, w1, c == 0 ? 0x5140u : 0x7362u);
+    first = add_f16x2(prmt(x, 0x64646464u, 0x4140u), 0xE480E480u);
+    second = add_f16x2(prmt(x, 0x64646464u, 0x4342u), 0xE480E480u);
 }
+// x: half words of two keys, codes n = 0..3
 __device__ __forceinline__ uint32_t v_codes4(uint32_t x, int n) {
-    return add_bf16x2(((x >> (4 * n)) & 0x000F000Fu) | 0x43004300u, 0xC308C308u);
+    const uint32_t y = n >= 2 ? x >> 8 : x;
+    return (n & 1) ? f16_high(y, 0xD480D480u) : f16_low(y, 0xE408E408u);      // -(64 + 8), -(1024 + 8)
 }
 
 template <int D, int BITS, int GROUP, int NT, int LIMBS>
@@ -411,7 +434,6 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
     using S = Shape<D, BITS, GROUP, NT, LIMBS>;
     constexpr int R = S::R, RB = S::RB, GS = S::GS, PG = S::PG, NP = S::NP;
     constexpr bool kQReg = NT * LIMBS <= 2;
-    constexpr int kTerms = LIMBS == 2 ? 3 : 1;     // bf16 terms of p s
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t s_full[S::STAGES], s_empty[S::STAGES];
     __shared__ uint32_t s_bad[S::STAGES];          // bit w: keys 16w.. of the unit are in no page
@@ -517,9 +539,22 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
 
     // ---------------- consumers ----------------
     const uint32_t g = lane >> 2, t = lane & 3;
-    const uint32_t ra = warp * 16 + key_row<RB>(g);               // this lane's rows in the score product: ra, ra + 8
-    const uint32_t va = warp * 16 + key_row<RB>(2 * t), vb = warp * 16 + key_row<RB>(2 * t + 1);   // and the other's: va, vb, + 8
+    constexpr int H = S::H;
+    const uint32_t turn = S::TURNS == 1 ? 0u : static_cast<uint32_t>(warp) >> 1;         // units it % TURNS == turn are this warp's
+    const uint32_t wrow = (S::TURNS == 1 ? warp : (warp & 1)) * (16 * H);              // its first key of a unit
     constexpr int kPiece = PG / 4 * BITS / 8, vPiece = PG / 8 * BITS / 8;   // bytes of a row that a lane reads per step
+    const uint32_t ra = wrow + key_row<RB>(g);                    // this lane's rows in the score product: ra, ra + 8 (+ 16)
+    // offsets in a stage; rows 8 and 16 further on lie 8 and 16 row lengths further on under every swizzle
+    uint32_t k_off[NP], v_off[NP][2];
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        k_off[j] = code_offset<RB>(ra, j * (PG * BITS / 8) + t * kPiece);
+        v_off[j][0] = S::CODES + code_offset<RB>(wrow + key_row<RB>(2 * t), j * (PG * BITS / 8) + g * vPiece);
+        v_off[j][1] = S::CODES + code_offset<RB>(wrow + key_row<RB>(2 * t + 1), j * (PG * BITS / 8) + g * vPiece);
+    }
+    const uint32_t s_off = 2 * S::CODES + ra * GS * 2;
+    const uint32_t q_at = smem_u32(qf_ptr) + lane * 8;
+    const float s_hidden = __uint_as_float(0xFF800000u);      // score of a key that a row does not see
     uint32_t it = 0;
     bool failed = false;
     for (uint64_t u = u0; u < u1;) {
@@ -608,7 +643,7 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                m[nt][c] = -INFINITY;
+                m[nt][c] = kNoMax;
                 l[nt][c] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < GS; ++i) bsum[nt][c][i] = 0.0f;
@@ -620,139 +655,174 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[i][nt][c] = 0.0f;
 
-        for (uint32_t tile = tile0; tile < tile0 + count; ++tile, ++it) {
-            const uint32_t stage = it % S::STAGES;
-            if (!mbar_wait(smem_u32(&s_full[stage]), (it / S::STAGES) & 1u, &s_abort, p.a.error_word)) failed = true;
-            const uint32_t kc = base + stage * S::STAGE, vc = kc + S::CODES, sc = vc + S::CODES;
-            const int32_t key0 = static_cast<int32_t>(tile * kKeys);
-            const bool bad = (s_bad[stage] >> warp) & 1u;
-            const bool border = key0 + kKeys > item.first_seen || s_bad[stage] != 0u;
-            if (key0 + warp * 16 < item.keys && !bad) {
-                // ---- scores, transposed: [16 keys][8 NT rows] ----
-                float s[NT][4];
-                {
-                    float sa[GS], sb[GS], ba[GS], bb[GS];
-                    row_f32<GS>(sc + ra * GS * 2, sa);
-                    row_f32<GS>(sc + (ra + 8) * GS * 2, sb);
-                    row_f32<GS>(sc + S::SB + ra * GS * 2, ba);
-                    row_f32<GS>(sc + S::SB + (ra + 8) * GS * 2, bb);
+        // One unit.  kBorder: some row of the tile does not see all its keys, or some of its keys are in no page.
+        auto unit = [&](auto border_tag, uint32_t kc, int32_t key0, uint32_t bad) {
+            constexpr bool kBorder = decltype(border_tag)::value;
+            // ---- scores, transposed: [16 H keys][8 NT rows] ----
+            float s[H][NT][4];
 #pragma unroll
-                    for (int j = 0; j < NP; ++j) {
-                        constexpr int kWords = kPiece >= 4 ? kPiece / 4 : 1;
-                        uint32_t wa[kWords], wb[kWords];
-                        const uint32_t off = j * (PG * BITS / 8) + t * kPiece;
-                        lds<kPiece>(kc + code_offset<RB>(ra, off), wa);
-                        lds<kPiece>(kc + code_offset<RB>(ra + 8, off), wb);
-                        float acc[NT][4];
+            for (int h = 0; h < H; ++h) {
+                float sa[GS], sb[GS], ba[GS], bb[GS];
+                const uint32_t at = kc + s_off + h * (16 * GS * 2);
+                row_f32<GS>(at, sa);
+                row_f32<GS>(at + 8 * GS * 2, sb);
+                row_f32<GS>(at + S::SB, ba);
+                row_f32<GS>(at + S::SB + 8 * GS * 2, bb);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
+                for (int j = 0; j < NP; ++j) {
+                    constexpr int kWords = kPiece >= 4 ? kPiece / 4 : 1;
+                    uint32_t wa[kWords], wb[kWords];
+                    lds<kPiece>(kc + k_off[j] + h * (16 * RB), wa);
+                    lds<kPiece>(kc + k_off[j] + h * (16 * RB) + 8 * RB, wb);
+                    float acc[NT][4];
 #pragma unroll
-                        for (int k = 0; k < PG / 16; ++k) {
-                            uint32_t a[4];
-                            k_codes<BITS>(wa, k, a[0], a[2]);
-                            k_codes<BITS>(wb, k, a[1], a[3]);
+                    for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                for (int lb = 0; lb < LIMBS; ++lb) {
-                                    if (kQReg) {
-                                        const uint32_t *q = qreg[kQReg ? lb : 0][kQReg ? nt : 0][kQReg ? j * (PG / 16) + k : 0];
-                                        mma_f16(acc[nt], a, q[0], q[1]);
-                                    } else {
-                                        uint32_t q[2];
-                                        lds<8>(smem_u32(qf_ptr) + (((lb * NT + nt) * S::KS + j * (PG / 16) + k) * 32 + lane) * 8, q);
-                                        mma_f16(acc[nt], a, q[0], q[1]);
-                                    }
-                                }
-                        }
-                        constexpr int kPer = GROUP / PG;
+                    for (int k = 0; k < PG / 16; ++k) {
+                        uint32_t a[4];
+                        k_codes<BITS>(wa, k, a[0], a[2]);
+                        k_codes<BITS>(wb, k, a[1], a[3]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                const float ta = ba[j / kPer] * qsum[nt][c][j], tb = bb[j / kPer] * qsum[nt][c][j];
-                                s[nt][c] = fmaf(sa[j / kPer], acc[nt][c], j == 0 ? ta : s[nt][c] + ta);
-                                s[nt][2 + c] = fmaf(sb[j / kPer], acc[nt][2 + c], j == 0 ? tb : s[nt][2 + c] + tb);
+                            for (int lb = 0; lb < LIMBS; ++lb) {
+                                if (kQReg) {
+                                    const uint32_t *q = qreg[kQReg ? lb : 0][kQReg ? nt : 0][kQReg ? j * (PG / 16) + k : 0];
+                                    mma_f16(acc[nt], a, q[0], q[1]);
+                                } else {
+                                    uint32_t q[2];
+                                    lds<8>(q_at + ((lb * NT + nt) * S::KS + j * (PG / 16) + k) * 256, q);
+                                    mma_f16(acc[nt], a, q[0], q[1]);
+                                }
                             }
                     }
-                }
-                // ---- softmax: base 2, the maximum follows lazily ----
-                const int32_t pa = key0 + static_cast<int32_t>(ra), pb = pa + 8;
-                bool grow = false;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        s[nt][c] *= f[nt][c];
-                        s[nt][2 + c] *= f[nt][c];
-                        if (border) {
-                            const int32_t seen = s_seen[nt * 8 + 2 * t + c];
-                            if (pa >= seen) s[nt][c] = -INFINITY;
-                            if (pb >= seen) s[nt][2 + c] = -INFINITY;
-                        }
-                        grow |= fmaxf(s[nt][c], s[nt][2 + c]) > m[nt][c] + kLazy;
-                    }
-                if (__any_sync(0xFFFFFFFFu, grow)) {
+                    constexpr int kPer = GROUP / PG;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float top = fmaxf(s[nt][c], s[nt][2 + c]);
+                            s[h][nt][c] = j == 0 ? sa[0] * acc[nt][c] : fmaf(sa[j / kPer], acc[nt][c], s[h][nt][c]);
+                            s[h][nt][2 + c] = j == 0 ? sb[0] * acc[nt][2 + c] : fmaf(sb[j / kPer], acc[nt][2 + c], s[h][nt][2 + c]);
+                            s[h][nt][c] = fmaf(ba[j / kPer], qsum[nt][c][j], s[h][nt][c]);
+                            s[h][nt][2 + c] = fmaf(bb[j / kPer], qsum[nt][c][j], s[h][nt][2 + c]);
+                        }
+                }
+                if (kBorder) {
+                    const int32_t pa = key0 + static_cast<int32_t>(ra) + 16 * h, pb = pa + 8;
+                    const bool gone = (bad >> (wrow / 16 + h)) & 1u;
 #pragma unroll
-                            for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-                            top = fmaxf(top, m[nt][c]);
-                            const float keep = top == m[nt][c] ? 1.0f : exp2_approx(m[nt][c] - top);
-                            m[nt][c] = top;
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int32_t seen = gone ? 0 : s_seen[nt * 8 + 2 * t + c];
+                            if (pa >= seen) s[h][nt][c] = s_hidden;
+                            if (pb >= seen) s[h][nt][2 + c] = s_hidden;
+                        }
+                }
+            }
+            // ---- weights: against the row's reference; it follows lazily ----
+            float va[H][GS], vb[H][GS], ea[H], eb[H];     // scales of the values and the exponents that they lend the weights
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const uint32_t at = kc + s_off + 2 * S::SB + h * (16 * GS * 2);
+                row_f32<GS>(at, va[h]);
+                row_f32<GS>(at + 8 * GS * 2, vb[h]);
+                ea[h] = key_exponent<GS>(va[h]);
+                eb[h] = key_exponent<GS>(vb[h]);
+            }
+            bool grow = false;
+            float z[H][NT][4];
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        z[h][nt][c] = fmaf(s[h][nt][c], f[nt][c & 1], -m[nt][c & 1]);
+                        if (kBorder && s[h][nt][c] == s_hidden) z[h][nt][c] = -INFINITY;
+                        grow |= z[h][nt][c] + (c < 2 ? ea[h] : eb[h]) > kTarget + kLazy;
+                    }
+            if (__any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int h = 0; h < H; ++h) top = fmaxf(top, fmaxf(z[h][nt][c] + ea[h], z[h][nt][2 + c] + eb[h]));
+#pragma unroll
+                        for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+                        if (m[nt][c] == kNoMax) {      // no reference yet: z is the score's distance from nothing
+                            float y = -INFINITY;
+#pragma unroll
+                            for (int h = 0; h < H; ++h) {
+                                const float y0 = kBorder && s[h][nt][c] == s_hidden ? -INFINITY : fmaf(s[h][nt][c], f[nt][c], ea[h]);
+                                const float y1 = kBorder && s[h][nt][2 + c] == s_hidden ? -INFINITY : fmaf(s[h][nt][2 + c], f[nt][c], eb[h]);
+                                y = fmaxf(y, fmaxf(y0, y1));
+                            }
+#pragma unroll
+                            for (int x = 4; x <= 16; x <<= 1) y = fmaxf(y, __shfl_xor_sync(0xFFFFFFFFu, y, x));
+                            if (y > kNoMax) m[nt][c] = y - kTarget;
+                        } else if (top > kTarget) {
+                            const float keep = exp2_approx(kTarget - top);
+                            m[nt][c] += top - kTarget;
                             l[nt][c] *= keep;
 #pragma unroll
                             for (int i = 0; i < GS; ++i) bsum[nt][c][i] *= keep;
 #pragma unroll
                             for (int i = 0; i < S::KS; ++i) o[i][nt][c] *= keep, o[i][nt][2 + c] *= keep;
                         }
-                }
-                // ---- weights times scales as B fragments, weights times biases ----
-                uint32_t pf[kTerms][GS][NT][2];
-                {
-                    float sa[GS], sb[GS], ba[GS], bb[GS];
-                    row_f32<GS>(sc + 2 * S::SB + ra * GS * 2, sa);
-                    row_f32<GS>(sc + 2 * S::SB + (ra + 8) * GS * 2, sb);
-                    row_f32<GS>(sc + 3 * S::SB + ra * GS * 2, ba);
-                    row_f32<GS>(sc + 3 * S::SB + (ra + 8) * GS * 2, bb);
-#pragma unroll
-                    for (int i = 0; i < GS; ++i) {
-                        ba[i] = fmaf(static_cast<float>(1 << (BITS - 1)), sa[i], ba[i]);
-                        bb[i] = fmaf(static_cast<float>(1 << (BITS - 1)), sb[i], bb[i]);
                     }
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float pr[4];
+                for (int h = 0; h < H; ++h)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const float top = m[nt][c & 1];
-                            pr[c] = exp2_approx(s[nt][c] - (top == -INFINITY ? 0.0f : top));
-                        }
-                        l[nt][0] += pr[0] + pr[2];
-                        l[nt][1] += pr[1] + pr[3];
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int i = 0; i < GS; ++i) {
-                            float x[4] = {pr[0] * sa[i], pr[1] * sa[i], pr[2] * sb[i], pr[3] * sb[i]};
+                        for (int c = 0; c < 4; ++c)
+                            z[h][nt][c] = kBorder && s[h][nt][c] == s_hidden ? -INFINITY : fmaf(s[h][nt][c], f[nt][c & 1], -m[nt][c & 1]);
+            }
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                // ---- weights times scales as B fragments, weights times biases ----
+                uint32_t pf[LIMBS][GS][NT][2];
+                float ba[GS], bb[GS];
+                const uint32_t at = kc + s_off + 3 * S::SB + h * (16 * GS * 2);
+                row_f32<GS>(at, ba);
+                row_f32<GS>(at + 8 * GS * 2, bb);
+#pragma unroll
+                for (int i = 0; i < GS; ++i) {
+                    ba[i] = fmaf(static_cast<float>(1 << (BITS - 1)), va[h][i], ba[i]);
+                    bb[i] = fmaf(static_cast<float>(1 << (BITS - 1)), vb[h][i], bb[i]);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float pr[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) pr[c] = exp2_approx(z[h][nt][c]);
+                    l[nt][0] += pr[0] + pr[2];
+                    l[nt][1] += pr[1] + pr[3];
+#pragma unroll
+                    for (int i = 0; i < GS; ++i) {
+                        float x[4] = {pr[0] * va[h][i], pr[1] * va[h][i], pr[2] * vb[h][i], pr[3] * vb[h][i]};
+                        if (kBorder) {   // rows behind the end may hold anything, NaN too
                             float y[4] = {pr[0] * ba[i], pr[1] * ba[i], pr[2] * bb[i], pr[3] * bb[i]};
-                            if (border) {   // rows behind the end may hold anything, NaN too
 #pragma unroll
-                                for (int c = 0; c < 4; ++c)
-                                    if (s[nt][c] == -INFINITY) x[c] = 0.0f, y[c] = 0.0f;
-                            }
+                            for (int c = 0; c < 4; ++c)
+                                if (z[h][nt][c] == -INFINITY) x[c] = 0.0f, y[c] = 0.0f;
                             bsum[nt][0][i] += y[0] + y[2];
                             bsum[nt][1][i] += y[1] + y[3];
+                        } else {
+                            bsum[nt][0][i] = fmaf(pr[0], ba[i], fmaf(pr[2], bb[i], bsum[nt][0][i]));
+                            bsum[nt][1][i] = fmaf(pr[1], ba[i], fmaf(pr[3], bb[i], bsum[nt][1][i]));
+                        }
 #pragma unroll
-                            for (int lb = 0; lb < kTerms; ++lb) {
-                                const uint32_t w0 = pack_bf16x2(x[0], x[1]), w1 = pack_bf16x2(x[2], x[3]);
-                                pf[lb][i][nt][0] = transpose8x8(w0);
-                                pf[lb][i][nt][1] = transpose8x8(w1);
-                                if (lb + 1 < kTerms) {
-                                    x[0] -= bf16_f32(w0), x[1] -= __uint_as_float(w0 & 0xFFFF0000u);
-                                    x[2] -= bf16_f32(w1), x[3] -= __uint_as_float(w1 & 0xFFFF0000u);
-                                }
+                        for (int lb = 0; lb < LIMBS; ++lb) {
+                            const uint32_t w0 = pack_f16x2(x[0], x[1]), w1 = pack_f16x2(x[2], x[3]);
+                            pf[lb][i][nt][0] = transpose8x8(w0);
+                            pf[lb][i][nt][1] = transpose8x8(w1);
+                            if (lb + 1 < LIMBS) {
+                                const float2 y0 = __half22float2(*reinterpret_cast<const __half2 *>(&w0)), y1 = __half22float2(*reinterpret_cast<const __half2 *>(&w1));
+                                x[0] -= y0.x, x[1] -= y0.y, x[2] -= y1.x, x[3] -= y1.y;
                             }
                         }
                     }
@@ -762,19 +832,16 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                 for (int j = 0; j < NP; ++j) {
                     constexpr int kWords = vPiece >= 4 ? vPiece / 4 : 1;
                     uint32_t w[4][kWords];
-                    const uint32_t off = j * (PG * BITS / 8) + g * vPiece;
-                    lds<vPiece>(vc + code_offset<RB>(va, off), w[0]);
-                    lds<vPiece>(vc + code_offset<RB>(vb, off), w[1]);
-                    lds<vPiece>(vc + code_offset<RB>(va + 8, off), w[2]);
-                    lds<vPiece>(vc + code_offset<RB>(vb + 8, off), w[3]);
+                    lds<vPiece>(kc + v_off[j][0] + h * (16 * RB), w[0]);
+                    lds<vPiece>(kc + v_off[j][1] + h * (16 * RB), w[1]);
+                    lds<vPiece>(kc + v_off[j][0] + h * (16 * RB) + 8 * RB, w[2]);
+                    lds<vPiece>(kc + v_off[j][1] + h * (16 * RB) + 8 * RB, w[3]);
 #pragma unroll
                     for (int i = 0; i < PG / 16; ++i) {
                         uint32_t a[4];
                         if (BITS == 8) {
-                            a[0] = v_codes8(w[0][i >> 1], w[1][i >> 1], 2 * (i & 1));
-                            a[1] = v_codes8(w[0][i >> 1], w[1][i >> 1], 2 * (i & 1) + 1);
-                            a[2] = v_codes8(w[2][i >> 1], w[3][i >> 1], 2 * (i & 1));
-                            a[3] = v_codes8(w[2][i >> 1], w[3][i >> 1], 2 * (i & 1) + 1);
+                            v_codes8(w[0][i >> 1], w[1][i >> 1], 2 * (i & 1), a[0], a[1]);
+                            v_codes8(w[2][i >> 1], w[3][i >> 1], 2 * (i & 1), a[2], a[3]);
                         } else {
                             const uint32_t x = prmt(w[0][0], w[1][0], i < 2 ? 0x5410u : 0x7632u);
                             const uint32_t y = prmt(w[2][0], w[3][0], i < 2 ? 0x5410u : 0x7632u);
@@ -786,11 +853,26 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int lb = 0; lb < kTerms; ++lb)
-                                mma_bf16(o[j * (PG / 16) + i][nt], a, pf[lb][j * PG / GROUP][nt][0], pf[lb][j * PG / GROUP][nt][1]);
+                            for (int lb = 0; lb < LIMBS; ++lb)
+                                mma_f16(o[j * (PG / 16) + i][nt], a, pf[lb][j * PG / GROUP][nt][0], pf[lb][j * PG / GROUP][nt][1]);
                     }
                 }
             }
+        };
+        for (uint32_t tile = tile0; tile < tile0 + count; ++tile, ++it) {
+            const uint32_t stage = it % S::STAGES;
+            if (!mbar_wait(smem_u32(&s_full[stage]), (it / S::STAGES) & 1u, &s_abort, p.a.error_word)) failed = true;
+            if (S::TURNS > 1 && (it % S::TURNS) != turn) {
+                // another pair's unit: every warp follows every fill of a stage and hands it back, or the parity that it waits
+                // for next could be that of an older fill
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s_empty[stage]));
+                continue;
+            }
+            const int32_t key0 = static_cast<int32_t>(tile * kKeys);
+            const uint32_t bad = s_bad[stage];
+            if (key0 + kKeys <= item.first_seen && bad == 0u) unit(std::false_type(), base + stage * S::STAGE, key0, 0u);
+            else if (key0 + static_cast<int32_t>(wrow) < item.keys) unit(std::true_type(), base + stage * S::STAGE, key0, bad);
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&s_empty[stage]));
         }
@@ -942,7 +1024,7 @@ cudaError_t launch(const Params &p, const CUtensorMap &tmap, int sm_count, cudaS
     return cudaGetLastError();
 }
 
-// `nt`: 1, 2 or 4 row tiles of 8
+// `nt`: 1 to 4 row tiles of 8 (limbs = 2: 1 or 2)
 cudaError_t launch_d64_b4(const Params &p, const CUtensorMap &tmap, int nt, int limbs, int sm_count, cudaStream_t stream);
 cudaError_t launch_d64_b8(const Params &p, const CUtensorMap &tmap, int nt, int limbs, int sm_count, cudaStream_t stream);
 cudaError_t launch_d128_b4(const Params &p, const CUtensorMap &tmap, int nt, int limbs, int sm_count, cudaStream_t stream);
@@ -953,6 +1035,7 @@ cudaError_t launch_rows(const Params &p, const CUtensorMap &tmap, int nt, int li
     if (limbs == 2) return nt == 1 ? launch<D, BITS, GROUP, 1, 2>(p, tmap, sm_count, stream) : launch<D, BITS, GROUP, 2, 2>(p, tmap, sm_count, stream);
     if (nt == 1) return launch<D, BITS, GROUP, 1, 1>(p, tmap, sm_count, stream);
     if (nt == 2) return launch<D, BITS, GROUP, 2, 1>(p, tmap, sm_count, stream);
+    if (nt == 3) return launch<D, BITS, GROUP, 3, 1>(p, tmap, sm_count, stream);
     return launch<D, BITS, GROUP, 4, 1>(p, tmap, sm_count, stream);
 }
 

@@ -459,7 +459,7 @@ cudaError_t attention(const AttnArgs &a, const CUtensorMap &tmap, const AttnWork
             return attend::launch_wide(p, tmap, sm_count, stream);
         }
         // 8 rows a tile cost least where they suffice; more rows read the cache less often
-        const int nt = rows <= 8u ? 1 : rows <= 16u || f32 ? 2 : 4;
+        const int nt = rows <= 8u ? 1 : rows <= 16u || f32 ? 2 : rows <= 24u ? 3 : 4;
         p.row_tiles = static_cast<uint32_t>((rows + 8u * nt - 1u) / (8u * nt));
         p.elements = p.prefix_pass ? p.row_tiles : p.row_tiles * a.seqs.batch;
         const int limbs = f32 ? 2 : 1;
