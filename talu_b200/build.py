@@ -6,6 +6,7 @@ next to this file.  nvcc cross-compiles, so this runs on a machine without a GPU
 from __future__ import annotations
 
 import os
+import re
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -27,14 +28,20 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
-def _deps_mtime() -> float:
-    hdrs = list(CSRC.glob("*.h")) + list(CSRC.glob("*.cuh")) + list((ROOT / "include").glob("*.h"))
-    return max(h.stat().st_mtime for h in hdrs)
+def _newest(path: Path, seen: set[Path]) -> float:
+    """Newest modification time of a source and of the files that it includes by relative path, directly or not."""
+    seen.add(path)
+    times = [path.stat().st_mtime]
+    for name in re.findall(r'^\s*#\s*include\s+"([^"]+)"', path.read_text(), re.M):
+        inc = (path.parent / name).resolve()
+        if inc.exists() and inc not in seen:
+            times.append(_newest(inc, seen))
+    return max(times)
 
 
 def _compile(src: Path, verbose_ptxas: bool) -> tuple[Path, str]:
     obj = OBJ_DIR / (src.stem + ".o")
-    newest = max(src.stat().st_mtime, _deps_mtime())
+    newest = _newest(src, set())
     if obj.exists() and obj.stat().st_mtime >= newest:
         return obj, ""
     cmd = [NVCC, *ARCH, *CFLAGS, "-c", str(src), "-o", str(obj)]

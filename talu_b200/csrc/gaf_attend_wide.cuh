@@ -16,8 +16,10 @@
 //   warp 13          TMA of codes, bulk copies of scales and biases
 // K and V tiles share a ring of three 32 KB buffers, their codes one of three stages: K(i), V(i), K(i+1), ...
 //
-// The maximum follows lazily, as in the narrow kernel: weights are formed against the last maximum in one pass over the
-// scores; only when a row of the warp exceeds it by 2^8 is the pass repeated and O rescaled in tensor memory.
+// The maximum follows lazily, as in the narrow kernel: only when a row of the warp exceeds it by 2^8 is O rescaled in tensor
+// memory.  The scores are read twice (maximum, weights), 64 at a time in loops that are not unrolled: a single unrolled
+// pass that was repeated when the maximum had to follow ran out of the instruction cache (387 against 314 us for two
+// sequences of 768 and 1024 new tokens over 3750 and 5000 cached ones, 32 heads on 8).
 // What bounds it: 2 x 128 x 128 exponentials per unit (16 per clock and SM) and as many clocks of tensor work.
 #pragma once
 #include "gaf_attend.cuh"
@@ -456,8 +458,9 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                     for (int i = 0; i < D / 2; ++i) top = max(top, max((x[i] << 16) & 0x7FFFFFFFu, x[i] & 0x7FFF0000u));
                     int e = static_cast<int>(top >> 23) - 127;
                     e = e < -100 ? -100 : e > 127 ? 127 : e;
-                    const float mul = pow2(13 - e);
-                    f = pow2(e - 13) * (p.a.scale * 1.4426950408889634f);
+                    // the sign of the scale goes to q, so that the largest raw score is the largest score
+                    const float mul = p.a.scale < 0.0f ? -pow2(13 - e) : pow2(13 - e);
+                    f = pow2(e - 13) * (fabsf(p.a.scale) * 1.4426950408889634f);
                     const uint32_t dst = q_base + t * W::TILE + r * 128u;
 #pragma unroll
                     for (int c = 0; c < D / 8; ++c) {
@@ -479,6 +482,18 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                 int32_t seen = p.prefix_pass ? item.seen0 : item.seen0 + static_cast<int32_t>(row / p.per_kv);
                 seen = seen < item.keys ? seen : item.keys;
 
+                auto rescale = [&](float keep) {
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t raw[32];
+                        tmem_ld32(tm_o + 32u * c, raw);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) raw[k] = __float_as_uint(__uint_as_float(raw[k]) * keep);
+                        tmem_st32(tm_o + 32u * c, raw);
+                    }
+                    tmem_wait_st();
+                };
                 for (uint32_t i = 0; i < count; ++i) {
                     const int32_t key0 = static_cast<int32_t>((tile0 + i) * kWideKeys);
                     wait(s_score[t], scores_seen++ & 1u);
@@ -487,76 +502,64 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                     const uint32_t ki = (kx + 2u * i) % kInfo, vi = (kx + 2u * i + 1u) % kInfo;
                     const uint32_t bad = s_lost[ki];
                     const bool border = key0 + kWideKeys > item.first_seen || bad != 0u;
-                    const float fk = f * pow2(s_exp[ki] < -126 ? -126 : s_exp[ki]);
-                    uint32_t w[kWideKeys / 2];
-                    float top, sum;
-                    // scores of 32 keys, with what the row does not see taken out
-                    auto scores = [&](int c, float (&x)[32]) {
-                        uint32_t raw[32];
-                        tmem_ld32(tm_s + 32u * c, raw);
+                    const float fk = fmaxf(f * pow2(s_exp[ki]), 1.0e-37f);     // not 0: hidden scores are -inf
+                    // what the row does not see is taken out of 64 raw scores
+                    auto scores = [&](int c, uint32_t (&raw)[64]) {
+                        tmem_ld32(tm_s + 64u * c, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
+                        tmem_ld32(tm_s + 64u * c + 32u, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
                         tmem_wait_ld();
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) x[k] = __uint_as_float(raw[k]) * fk;
                         if (border) {
+                            const int32_t left = seen - key0 - 64 * c;
 #pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                if (key0 + 32 * c + k >= seen || ((bad >> (2 * c + k / 16)) & 1u)) x[k] = -INFINITY;
+                            for (int k = 0; k < 64; ++k)
+                                if (k >= left || ((bad >> (4 * c + k / 16)) & 1u)) raw[k] = 0xFF800000u;
                         }
                     };
-                    auto pass = [&]() {
-                        const float use = m == -INFINITY ? 0.0f : m;
-                        top = -INFINITY;
-                        sum = 0.0f;
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < kWideKeys / 64; ++c) {
+                        uint32_t raw[64];
+                        scores(c, raw);
+                        float t0 = __uint_as_float(raw[0]), t1 = __uint_as_float(raw[1]);
 #pragma unroll
-                        for (int c = 0; c < kWideKeys / 32; ++c) {
-                            float x[32];
-                            scores(c, x);
-#pragma unroll
-                            for (int k = 0; k < 32; k += 2) {
-                                top = fmaxf(top, fmaxf(x[k], x[k + 1]));
-                                const float p0 = exp2_approx(x[k] - use), p1 = exp2_approx(x[k + 1] - use);
-                                sum += p0 + p1;
-                                w[16 * c + k / 2] = pack_f16x2(p0, p1);
-                            }
+                        for (int k = 2; k < 64; k += 2) {
+                            t0 = fmaxf(t0, __uint_as_float(raw[k]));
+                            t1 = fmaxf(t1, __uint_as_float(raw[k + 1]));
                         }
-                    };
-                    pass();
+                        top = fmaxf(top, fmaxf(t0, t1));
+                    }
+                    top *= fk;
                     if (__any_sync(0xFFFFFFFFu, top > m + kLazy)) {
                         const float m1 = fmaxf(m, top);
                         const float keep = m1 == m ? 1.0f : exp2_approx(m - m1);
                         m = m1;
                         l *= keep;
-                        if (i > 0) {
-#pragma unroll 1
-                            for (int c = 0; c < D / 32; ++c) {
-                                uint32_t raw[32];
-                                tmem_ld32(tm_o + 32u * c, raw);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int k = 0; k < 32; ++k) raw[k] = __float_as_uint(__uint_as_float(raw[k]) * keep);
-                                tmem_st32(tm_o + 32u * c, raw);
-                            }
-                            tmem_wait_st();
-                        }
-                        pass();
+                        if (i > 0) rescale(keep);
                     }
-                    l += sum;
+                    const float use = m == -INFINITY ? 0.0f : m;
+                    float sum0 = 0.0f, sum1 = 0.0f;
+                    // the weights of 64 keys take half of the columns that their scores had
+#pragma unroll 1
+                    for (int c = 0; c < kWideKeys / 64; ++c) {
+                        uint32_t raw[64];
+                        scores(c, raw);
+#pragma unroll
+                        for (int k = 0; k < 64; k += 2) {
+                            const float p0 = exp2_approx(fmaf(__uint_as_float(raw[k]), fk, -use)), p1 = exp2_approx(fmaf(__uint_as_float(raw[k + 1]), fk, -use));
+                            sum0 += p0;
+                            sum1 += p1;
+                            raw[k / 2] = pack_f16x2(p0, p1);
+                        }
+                        tmem_st32(tm_s + 32u * c, raw);
+                    }
+                    l += sum0 + sum1;
                     // the values' side: K of this unit was ready before V, whose information is needed now
                     const uint32_t vx = kx + 2u * i + 1u;
                     wait(s_tile_full[vx % W::TILES], (vx / W::TILES) & 1u);
                     __syncwarp();
                     const int ve = s_exp[vi];
                     if (i > 0 && ve != v_exp) {
-                        const float keep = pow2(v_exp - ve < -126 ? -126 : v_exp - ve);
-#pragma unroll 1
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t raw[32];
-                            tmem_ld32(tm_o + 32u * c, raw);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) raw[k] = __float_as_uint(__uint_as_float(raw[k]) * keep);
-                            tmem_st32(tm_o + 32u * c, raw);
-                        }
+                        rescale(pow2(v_exp - ve < -126 ? -126 : v_exp - ve));
                     }
                     v_exp = ve;
                     if (s_lost[vi]) {
@@ -564,8 +567,6 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                             if (key0 + k < seen) poison |= s_poison[(vx / 2u) % (kInfo / 2)][k];
                     }
                     __syncwarp();
-                    tmem_st32(tm_s, w);
-                    tmem_st32(tm_s + 32u, w + 32);
                     tmem_wait_st();
                     fence_before();
                     mbar_arrive(smem_u32(&s_weights[t]));
