@@ -1,11 +1,12 @@
 // Attention over the quantised KV cache on tcgen05, for many query rows per cached head (prompts, shared prefixes).
 //
-// Mathematics.  Keys and values are dequantised to f16, each unit of 128 keys with one power of two that brings its largest
-// magnitude to 2^14..2^15 (keys) or keeps it below 2^15 (values, one running power per segment): 11 bits of every element
-// that is within 2^-29 of the unit's largest.  bf16 would hold any range as it is, but its 8 bits on keys and values alone put
-// the result 3e-3 off; f16 leaves them at 2^-12.  q is f16 with a power of two per row (exact), the weights are f16 (2^-12 of each),
-// all statistics and sums f32.
-//   w 2^e = (c - h) (s 2^e) + (b + h s) 2^e,   h = 2^(bits - 1): the centred code and s 2^e are exact in f16
+// Mathematics.  Keys and values are dequantised to f16, 32 keys at a time with one power of two that brings their largest
+// magnitude to 2^14..2^15: 11 bits of every element that is within 2^-29 of that.  bf16 would hold any range as it is, but its
+// 8 bits on keys and values alone put the result 3e-3 off; f16 leaves them at 2^-12.
+//   w 2^-e = (c - h) (s 2^-e) + (b + h s) 2^-e,   h = 2^(bits - 1): the centred code and s 2^-e are exact in f16
+// q is f16 with a power of two per row (exact), the weights are f16 (2^-12 of each), all statistics and sums f32.  The keys'
+// power goes into the scores' factor, the values' into the weights: they are formed as 2^(y + e - m) (y: scores in base
+// 2), where m follows the largest y + e instead of the largest y, and leave it again in the row's sum.
 //
 // One CTA per SM, 256 query rows (two MMA tiles of 128) against units of 128 keys:
 //   warps 0-3, 4-7   softmax of tile 0 and 1, one row per thread: scores from tensor memory, weights (f16) back into the
@@ -16,11 +17,13 @@
 //   warp 13          TMA of codes, bulk copies of scales and biases
 // K and V tiles share a ring of three 32 KB buffers, their codes one of three stages: K(i), V(i), K(i+1), ...
 //
-// The maximum follows lazily, as in the narrow kernel: only when a row of the warp exceeds it by 2^8 is O rescaled in tensor
+// The reference follows lazily, as in the narrow kernel: only when a row of the warp exceeds it by 2^8 is O rescaled in tensor
 // memory.  The scores are read twice (maximum, weights), 64 at a time in loops that are not unrolled: a single unrolled
 // pass that was repeated when the maximum had to follow ran out of the instruction cache (387 against 314 us for two
 // sequences of 768 and 1024 new tokens over 3750 and 5000 cached ones, 32 heads on 8).
-// What bounds it: 2 x 128 x 128 exponentials per unit (16 per clock and SM) and as many clocks of tensor work.
+// What bounds it: 2 x 128 x 128 exponentials per unit (16 per clock and SM) and as many clocks of tensor work; what keeps it
+// from there is the way of one tile's unit through scores, softmax, weights and second product, which the other tile
+// covers only in part.
 #pragma once
 #include "gaf_attend.cuh"
 
@@ -29,9 +32,11 @@ namespace attend {
 
 constexpr int kWideKeys = 128;
 constexpr int kWideRows = 256;
-constexpr int kWideThreads = 14 * 32;
-constexpr int kDequantWarp0 = 8, kMmaWarp = 12, kLoadWarp = 13;
-constexpr int kInfo = 8;             // half units whose side information is kept
+constexpr int kWideThreads = 14 * 32;    // 128 registers each
+constexpr int kDequantWarp0 = 8, kDequantWarps = 4, kMmaWarp = 12, kLoadWarp = 13;
+constexpr int kInfo = 4;             // units whose side information is kept
+constexpr float kMinFactor = 1.0e-37f;   // of raw scores: not 0, since hidden ones are -inf
+constexpr int kMinExp = -50;         // values below 2^-36 lose bits instead of pushing the weights out of f32
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
     uint64_t d = 0;
@@ -129,10 +134,10 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
     __shared__ __align__(8) uint64_t s_tile_full[W::TILES], s_tile_empty[W::TILES];
     __shared__ __align__(8) uint64_t s_q_ready[2], s_score[2], s_weights[2], s_done[2], s_idle;
     __shared__ uint32_t s_bad[W::STAGES];           // bit x: keys 16x.. of the unit are in no page
-    __shared__ int32_t s_exp[kInfo];                // tile = stored value x 2^-exp
-    __shared__ uint32_t s_lost[kInfo];              // s_bad of a K tile; of a V tile: some group is not finite
-    __shared__ uint8_t s_poison[kInfo / 2][kWideKeys];   // groups of a V row that are not finite
-    __shared__ uint32_t s_top[2][4];
+    // by unit and 32 keys: factor of the keys' scores, exponent of the values, 2^-exponent, groups of values that are not finite
+    __shared__ float s_kmul[kInfo][4], s_vexp[kInfo][4], s_vinv[kInfo][4];
+    __shared__ uint32_t s_kbad[kInfo], s_lost[kInfo][4];
+    __shared__ uint8_t s_poison[kInfo][kWideKeys];  // by key
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_abort;
     __shared__ uint32_t s_scan[kWideThreads / 32];
@@ -148,10 +153,10 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
         s_abort = 0u;
         for (int i = 0; i < W::STAGES; ++i) {
             mbar_init(smem_u32(&s_code_full[i]), 1);
-            mbar_init(smem_u32(&s_code_empty[i]), 4);
+            mbar_init(smem_u32(&s_code_empty[i]), kDequantWarps);
         }
         for (int i = 0; i < W::TILES; ++i) {
-            mbar_init(smem_u32(&s_tile_full[i]), 4);
+            mbar_init(smem_u32(&s_tile_full[i]), kDequantWarps);
             mbar_init(smem_u32(&s_tile_empty[i]), 1);
         }
         mbar_init(smem_u32(&s_idle), 1);
@@ -181,8 +186,7 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
     // data, so that they still meet at their barriers and leave together.
     bool ok = true;
     auto wait = [&](uint64_t &bar, uint32_t parity) {
-        if (ok && !s_abort) ok = mbar_wait(smem_u32(&bar), parity, &s_abort, p.a.error_word);
-        else ok = false;
+        if (ok) ok = mbar_wait(smem_u32(&bar), parity, &s_abort, p.a.error_word);
     };
 
     if (warp == kLoadWarp) {
@@ -253,6 +257,7 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
         constexpr uint32_t kIdesc = (1u << 4) | ((128u >> 4) << 24);                       // f16 x f16 -> f32, M = 128
         constexpr uint32_t kIdescS = kIdesc | ((kWideKeys >> 3) << 17);                    // N = 128 keys, both K-major
         constexpr uint32_t kIdescO = kIdesc | (1u << 16) | ((static_cast<uint32_t>(D) >> 3) << 17);   // N = D, V is N-major
+        const uint64_t q_desc = desc_sw128(q_base, 16u, 1024u), k_desc = desc_sw128(tile_base, 16u, 1024u), v_desc = desc_sw128(tile_base, W::PANEL, 1024u);
         uint32_t kx = 0, weights_seen[2] = {0u, 0u}, q_seen[2] = {0u, 0u};
         for (uint64_t u = u0; u < u1;) {
             const Item item = next_item<kWideRows, kWideKeys>(p, head, elem);
@@ -263,34 +268,42 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
             auto second = [&](uint32_t t, uint32_t i) {
                 const uint32_t vx = kx + 2u * i + 1u, buf = vx % W::TILES;
                 if (t == 0u) wait(s_tile_full[buf], (vx / W::TILES) & 1u);
+                const uint64_t vd = v_desc + ((buf * W::TILE) >> 4);
+                const uint32_t out = tmem + 256u + 128u * t, in = tmem + 128u * t;
+                const uint32_t add = i > 0u ? 1u : 0u, free_bar = smem_u32(&s_tile_empty[buf]), done_bar = smem_u32(&s_done[t]);
+                const bool last_tile = t + 1u == tiles, last_unit = i + 1u == count;
                 wait(s_weights[t], weights_seen[t]++ & 1u);
                 fence_after();
                 if (elect_one()) {
+                    umma_ts(out, in, vd, kIdescO, add);
 #pragma unroll
-                    for (int k = 0; k < kWideKeys / 16; ++k)
-                        umma_ts(tmem + 256u + 128u * t, tmem + 128u * t + k * 8u,
-                                desc_sw128(tile_base + buf * W::TILE + k * 2048u, W::PANEL, 1024u), kIdescO, i > 0u || k > 0);
-                    if (t + 1u == tiles) umma_commit(smem_u32(&s_tile_empty[buf]));
-                    if (i + 1u == count) umma_commit(smem_u32(&s_done[t]));
+                    for (int k = 1; k < kWideKeys / 16; ++k) umma_ts(out, in + k * 8u, vd + k * 128u, kIdescO, 1u);
+                    if (last_tile) umma_commit(free_bar);
+                    if (last_unit) umma_commit(done_bar);
                 }
                 __syncwarp();
             };
             for (uint32_t i = 0; i < count; ++i) {
-                const uint32_t buf = (kx + 2u * i) % W::TILES;
+                const uint32_t kxi = kx + 2u * i, buf = kxi % W::TILES;
+                const uint64_t kd = k_desc + ((buf * W::TILE) >> 4);
+                const uint32_t free_bar = smem_u32(&s_tile_empty[buf]);
                 for (uint32_t t = 0; t < tiles; ++t) {
                     if (i > 0) second(t, i - 1u);
                     else wait(s_q_ready[t], q_seen[t]++ & 1u);
-                    if (t == 0u) wait(s_tile_full[buf], ((kx + 2u * i) / W::TILES) & 1u);
+                    const uint64_t qd = q_desc + ((t * W::TILE) >> 4);
+                    const uint32_t out = tmem + 128u * t, score_bar = smem_u32(&s_score[t]);
+                    const bool last_tile = t + 1u == tiles;
+                    if (t == 0u) wait(s_tile_full[buf], (kxi / W::TILES) & 1u);
                     fence_after();
                     if (elect_one()) {
+                        umma_ss(out, qd, kd, kIdescS, 0u);
 #pragma unroll
-                        for (int k = 0; k < D / 16; ++k) {
-                            const uint32_t off = (k / 4) * W::PANEL + (k % 4) * 32u;
-                            umma_ss(tmem + 128u * t, desc_sw128(q_base + t * W::TILE + off, 16u, 1024u), desc_sw128(tile_base + buf * W::TILE + off, 16u, 1024u),
-                                    kIdescS, k > 0);
+                        for (int k = 1; k < D / 16; ++k) {
+                            constexpr uint32_t kStep = W::PANEL >> 4;
+                            umma_ss(out, qd + (k / 4) * kStep + (k % 4) * 2u, kd + (k / 4) * kStep + (k % 4) * 2u, kIdescS, 1u);
                         }
-                        if (t + 1u == tiles) umma_commit(smem_u32(&s_tile_empty[buf]));
-                        umma_commit(smem_u32(&s_score[t]));
+                        if (last_tile) umma_commit(free_bar);
+                        umma_commit(score_bar);
                     }
                     __syncwarp();
                 }
@@ -309,21 +322,23 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
         __syncwarp();
     } else if (warp >= kDequantWarp0) {
         // ---------------- dequantise: thread = cached row ----------------
-        const uint32_t row = (warp - kDequantWarp0) * 32 + lane;
+        const uint32_t part = warp - kDequantWarp0;
+        const uint32_t row = part * 32u + lane;
         const uint32_t swz = RB == 128 ? (row & 7u) : RB == 64 ? ((row >> 1) & 3u) : ((row >> 2) & 1u);
         constexpr float kHalf = static_cast<float>(1 << (BITS - 1)), kMost = static_cast<float>((1 << BITS) - 1);
         constexpr uint32_t kCentre = BITS == 8 ? 0xE480E480u : 0xE408E408u;     // -(1024 + h)
+        constexpr uint32_t kCentreHigh = 0xD480D480u;                           // -(64 + 8)
         uint32_t hx = 0;
         for (uint64_t u = u0; u < u1;) {
             const Item item = next_item<kWideRows, kWideKeys>(p, head, elem);
             const uint32_t left = item.tiles - tile0;
             const uint32_t count = u1 - u < left ? static_cast<uint32_t>(u1 - u) : left;
-            int v_exp = 0;
-            bool v_first = true;
             for (uint32_t tile = tile0; tile < tile0 + count; ++tile) {
-                for (int which = 0; which < 2; ++which, ++hx) {
-                    const uint32_t stage = hx % W::STAGES, buf = hx % W::TILES;
+#pragma unroll 1
+                for (uint32_t which = 0; which < 2u; ++which, ++hx) {
+                    const uint32_t stage = hx % W::STAGES, buf = hx % W::TILES, info = (hx >> 1) % kInfo;
                     wait(s_code_full[stage], (hx / W::STAGES) & 1u);
+                    __syncwarp();
                     const uint32_t src = code_base + stage * W::STAGE;
                     const uint32_t bad = s_bad[stage];
                     const bool valid = static_cast<int32_t>(tile * kWideKeys + row) < item.keys && !((bad >> (row >> 4)) & 1u);
@@ -339,54 +354,46 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                         else poison |= 1u << i;
                     }
                     top = __reduce_max_sync(0xFFFFFFFFu, top);
-                    if (lane == 0) s_top[hx & 1u][warp - kDequantWarp0] = top;
-                    const bool lost = __any_sync(0xFFFFFFFFu, poison != 0u);
-                    asm volatile("bar.sync 2, 128;" ::: "memory");
-                    top = max(max(s_top[hx & 1u][0], s_top[hx & 1u][1]), max(s_top[hx & 1u][2], s_top[hx & 1u][3]));
-                    int e = static_cast<int>(top >> 23) - 127;
-                    e = e < -100 ? -100 : e;
-                    if (which == 0) {
-                        e -= 14;
+                    int e = static_cast<int>(top >> 23) - 127 - 14;
+                    if (which == 0u) {
+                        e = e < -114 ? -114 : e;
+                        if (lane == 0) {
+                            s_kmul[info][part] = pow2(e);
+                            if (part == 0u) s_kbad[info] = bad;
+                        }
                     } else {
-                        if (v_first || e - v_exp > 14) v_exp = e - 10;     // room for 2^4 before O is rescaled
-                        v_first = false;
-                        e = v_exp;
-                    }
-                    if (row == 0) s_exp[hx % kInfo] = e;
-                    if (which == 0) {
-                        if (row == 0) s_lost[hx % kInfo] = bad;
-                    } else {
+                        e = e < kMinExp ? kMinExp : e;
                         // a value that is not finite must not reach rows that do not see its key: it is stored as zero, and rows
                         // that see it learn of it here
-                        s_poison[(hx / 2u) % (kInfo / 2)][row] = static_cast<uint8_t>(poison);
-                        const uint32_t any = lost ? 1u : 0u;
-                        uint32_t all;
-                        asm volatile(
-                            "{\n\t.reg .pred p, q;\n\t"
-                            "setp.ne.u32 p, %1, 0;\n\t"
-                            "bar.red.or.pred q, 2, 128, p;\n\t"
-                            "selp.u32 %0, 1, 0, q;\n\t}"
-                            : "=r"(all)
-                            : "r"(any)
-                            : "memory");
-                        if (row == 0) s_lost[hx % kInfo] = all;
+                        const uint32_t lost = __ballot_sync(0xFFFFFFFFu, poison != 0u);
+                        if (lost) s_poison[info][row] = static_cast<uint8_t>(poison);
+                        if (lane == 0) {
+                            s_vexp[info][part] = static_cast<float>(e);
+                            s_vinv[info][part] = pow2(-e);
+                            s_lost[info][part] = lost;
+                        }
                     }
-                    const float mul = pow2(-e);     // -127 < -e: e >= -114, e <= 117
+                    const float mul = pow2(-e);          // e between -114 and 114
                     uint32_t sh[GS], bh[GS];
 #pragma unroll
                     for (int i = 0; i < GS; ++i) {
-                        if (which == 1 && ((poison >> i) & 1u)) s[i] = b[i] = 0.0f;
+                        if (which == 1u && ((poison >> i) & 1u)) s[i] = b[i] = 0.0f;
                         const float sc = s[i] * mul, bc = fmaf(kHalf, s[i], b[i]) * mul;
                         sh[i] = pack_f16x2(sc, sc);
                         bh[i] = pack_f16x2(bc, bc);
                     }
+                    constexpr int kChunks = RB / 16;                 // 16-byte chunks of codes in a row
+                    constexpr int kOut = BITS == 8 ? 2 : 4;          // 16-byte chunks of f16 that 16 bytes of codes make
+                    uint32_t w[kChunks][4];
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c) lds<16>(src + row * RB + ((c ^ swz) << 4), w[c]);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&s_code_empty[stage]));
                     if (hx >= static_cast<uint32_t>(W::TILES)) wait(s_tile_empty[buf], (hx / W::TILES - 1u) & 1u);
+                    __syncwarp();
                     const uint32_t dst = tile_base + buf * W::TILE + row * 128u;
 #pragma unroll
-                    for (int c = 0; c < RB / 16; ++c) {
-                        uint32_t w[4];
-                        lds<16>(src + row * RB + ((c ^ swz) << 4), w);
-                        constexpr int kOut = BITS == 8 ? 2 : 4;          // 16-byte chunks of f16 that 16 bytes of codes make
+                    for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
                         for (int x = 0; x < kOut; ++x) {
                             const int chunk = c * kOut + x, gi = chunk * 8 / GROUP;
@@ -394,9 +401,13 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 uint32_t code;
-                                if (BITS == 8) code = prmt(w[2 * x + (i >> 1)], 0x64646464u, (i & 1) ? 0x4342u : 0x4140u);
-                                else code = ((w[x] >> (4 * i)) & 0x000F000Fu) | 0x64006400u;
-                                y[i] = fma_f16x2(add_f16x2(code, kCentre), sh[gi], bh[gi]);
+                                if (BITS == 8) {
+                                    code = add_f16x2(prmt(w[c][2 * x + (i >> 1)], 0x64646464u, (i & 1) ? 0x4342u : 0x4140u), kCentre);
+                                } else {
+                                    const uint32_t n = i >= 2 ? w[c][x] >> 8 : w[c][x];
+                                    code = (i & 1) ? f16_high(n, kCentreHigh) : f16_low(n, kCentre);
+                                }
+                                y[i] = fma_f16x2(code, sh[gi], bh[gi]);
                             }
                             const uint32_t at = dst + (chunk / 8) * W::PANEL + (((chunk & 7) ^ (row & 7u)) << 4);
                             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
@@ -404,10 +415,7 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                     }
                     fence_async_smem();
                     __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(smem_u32(&s_code_empty[stage]));
-                        mbar_arrive(smem_u32(&s_tile_full[buf]));
-                    }
+                    if (lane == 0) mbar_arrive(smem_u32(&s_tile_full[buf]));
                 }
             }
             u += count;
@@ -427,9 +435,8 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
             const bool active = t == 0u || item.rows - item.row0 > 128u;
             const uint32_t row = item.row0 + t * 128u + r;
             const bool have = row < item.rows;
-            float m = -INFINITY, l = 0.0f;
+            float m = kNoMax, l = 0.0f;
             uint32_t poison = 0u;
-            int v_exp = 0;
             const bool whole = tile0 == 0u && count == item.tiles;
             float *const part = p.partials + static_cast<uint64_t>(2u * blockIdx.x + (tile0 == 0u ? 1u : 0u)) * W::PART;
             if (active) {
@@ -482,28 +489,17 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                 int32_t seen = p.prefix_pass ? item.seen0 : item.seen0 + static_cast<int32_t>(row / p.per_kv);
                 seen = seen < item.keys ? seen : item.keys;
 
-                auto rescale = [&](float keep) {
-#pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t raw[32];
-                        tmem_ld32(tm_o + 32u * c, raw);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) raw[k] = __float_as_uint(__uint_as_float(raw[k]) * keep);
-                        tmem_st32(tm_o + 32u * c, raw);
-                    }
-                    tmem_wait_st();
-                };
                 for (uint32_t i = 0; i < count; ++i) {
                     const int32_t key0 = static_cast<int32_t>((tile0 + i) * kWideKeys);
+                    // values are ready before the scores as a rule: waiting for them first takes that wait out of the way
+                    const uint32_t vx = kx + 2u * i + 1u, info = (vx >> 1) % kInfo;
+                    wait(s_tile_full[vx % W::TILES], (vx / W::TILES) & 1u);
                     wait(s_score[t], scores_seen++ & 1u);
                     __syncwarp();
                     fence_after();
-                    const uint32_t ki = (kx + 2u * i) % kInfo, vi = (kx + 2u * i + 1u) % kInfo;
-                    const uint32_t bad = s_lost[ki];
+                    const uint32_t bad = s_kbad[info];
                     const bool border = key0 + kWideKeys > item.first_seen || bad != 0u;
-                    const float fk = fmaxf(f * pow2(s_exp[ki]), 1.0e-37f);     // not 0: hidden scores are -inf
-                    // what the row does not see is taken out of 64 raw scores
+                    // 64 raw scores, those that the row does not see taken out
                     auto scores = [&](int c, uint32_t (&raw)[64]) {
                         tmem_ld32(tm_s + 64u * c, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
                         tmem_ld32(tm_s + 64u * c + 32u, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
@@ -520,51 +516,57 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                     for (int c = 0; c < kWideKeys / 64; ++c) {
                         uint32_t raw[64];
                         scores(c, raw);
-                        float t0 = __uint_as_float(raw[0]), t1 = __uint_as_float(raw[1]);
 #pragma unroll
-                        for (int k = 2; k < 64; k += 2) {
-                            t0 = fmaxf(t0, __uint_as_float(raw[k]));
-                            t1 = fmaxf(t1, __uint_as_float(raw[k + 1]));
+                        for (int x = 0; x < 2; ++x) {
+                            float t0 = __uint_as_float(raw[32 * x]), t1 = __uint_as_float(raw[32 * x + 1]);
+#pragma unroll
+                            for (int k = 2; k < 32; k += 2) {
+                                t0 = fmaxf(t0, __uint_as_float(raw[32 * x + k]));
+                                t1 = fmaxf(t1, __uint_as_float(raw[32 * x + k + 1]));
+                            }
+                            top = fmaxf(top, fmaf(fmaxf(t0, t1), fmaxf(f * s_kmul[info][2 * c + x], kMinFactor), s_vexp[info][2 * c + x]));
                         }
-                        top = fmaxf(top, fmaxf(t0, t1));
                     }
-                    top *= fk;
                     if (__any_sync(0xFFFFFFFFu, top > m + kLazy)) {
                         const float m1 = fmaxf(m, top);
                         const float keep = m1 == m ? 1.0f : exp2_approx(m - m1);
                         m = m1;
                         l *= keep;
-                        if (i > 0) rescale(keep);
+                        if (i > 0) {
+#pragma unroll 1
+                            for (int c = 0; c < D / 32; ++c) {
+                                uint32_t raw[32];
+                                tmem_ld32(tm_o + 32u * c, raw);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) raw[k] = __float_as_uint(__uint_as_float(raw[k]) * keep);
+                                tmem_st32(tm_o + 32u * c, raw);
+                            }
+                        }
                     }
-                    const float use = m == -INFINITY ? 0.0f : m;
-                    float sum0 = 0.0f, sum1 = 0.0f;
                     // the weights of 64 keys take half of the columns that their scores had
 #pragma unroll 1
                     for (int c = 0; c < kWideKeys / 64; ++c) {
                         uint32_t raw[64];
                         scores(c, raw);
 #pragma unroll
-                        for (int k = 0; k < 64; k += 2) {
-                            const float p0 = exp2_approx(fmaf(__uint_as_float(raw[k]), fk, -use)), p1 = exp2_approx(fmaf(__uint_as_float(raw[k + 1]), fk, -use));
-                            sum0 += p0;
-                            sum1 += p1;
-                            raw[k / 2] = pack_f16x2(p0, p1);
+                        for (int x = 0; x < 2; ++x) {
+                            const float fk = fmaxf(f * s_kmul[info][2 * c + x], kMinFactor), use = s_vexp[info][2 * c + x] - m;
+                            float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                            for (int k = 32 * x; k < 32 * x + 32; k += 2) {
+                                const float p0 = exp2_approx(fmaf(__uint_as_float(raw[k]), fk, use)), p1 = exp2_approx(fmaf(__uint_as_float(raw[k + 1]), fk, use));
+                                sum0 += p0;
+                                sum1 += p1;
+                                raw[k / 2] = pack_f16x2(p0, p1);
+                            }
+                            l = fmaf(sum0 + sum1, s_vinv[info][2 * c + x], l);
                         }
                         tmem_st32(tm_s + 32u * c, raw);
                     }
-                    l += sum0 + sum1;
-                    // the values' side: K of this unit was ready before V, whose information is needed now
-                    const uint32_t vx = kx + 2u * i + 1u;
-                    wait(s_tile_full[vx % W::TILES], (vx / W::TILES) & 1u);
-                    __syncwarp();
-                    const int ve = s_exp[vi];
-                    if (i > 0 && ve != v_exp) {
-                        rescale(pow2(v_exp - ve < -126 ? -126 : v_exp - ve));
-                    }
-                    v_exp = ve;
-                    if (s_lost[vi]) {
+                    if (s_lost[info][0] | s_lost[info][1] | s_lost[info][2] | s_lost[info][3]) {
                         for (int k = 0; k < kWideKeys; ++k)
-                            if (key0 + k < seen) poison |= s_poison[(vx / 2u) % (kInfo / 2)][k];
+                            if (key0 + k < seen && ((s_lost[info][k >> 5] >> (k & 31)) & 1u)) poison |= s_poison[info][k];
                     }
                     __syncwarp();
                     tmem_wait_st();
@@ -575,7 +577,6 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                 wait(s_done[t], done_seen++ & 1u);
                 __syncwarp();
                 fence_after();
-                const float back = pow2(v_exp);
                 if (!whole && have) {
                     __stcg(part + kWideRows * D + t * 128u + r, m);
                     __stcg(part + kWideRows * (D + 1) + t * 128u + r, l);
@@ -593,7 +594,7 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                         for (int k = 0; k < 4; ++k) {
                             // value 4x + k of the 32 stands at the place that its eight keep it
                             const int in = (4 * x + k) % 8, place = BITS == 8 ? in : ((in & 3) * 2 + (in >> 2));
-                            v[k] = __uint_as_float(raw[(4 * x + k) / 8 * 8 + place]) * back;
+                            v[k] = __uint_as_float(raw[(4 * x + k) / 8 * 8 + place]);
                         }
                         if ((poison >> (c * 32 / GROUP)) & 1u) v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7FC00000u);
                         const uint32_t d = 32u * c + 4u * x;
