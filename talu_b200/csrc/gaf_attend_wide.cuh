@@ -9,18 +9,19 @@
 // 2), where m follows the largest y + e instead of the largest y, and leave it again in the row's sum.
 //
 // One CTA per SM, 256 query rows (two MMA tiles of 128) against units of 128 keys:
-//   warps 0-3, 4-7   softmax of tile 0 and 1, one row per thread: scores from tensor memory, weights (f16) back into the
-//                    scores' columns, where the second product takes them as its A operand
-//   warps 8-11       dequantise, one cached row per thread; K (K-major) and V (N-major) tiles have the same image
-//   warp 12          issues the MMAs: per unit S_t = Q_t K^T and O_t += P_t V for both tiles; while one tile's softmax
+//   warps 0-7, 8-15  softmax of tile 0 and 1, two threads per row with 64 keys each: scores from tensor memory, weights (f16)
+//                    back into the scores' columns, where the second product takes them as its A operand
+//   warps 16-19      dequantise, one cached row per thread; K (K-major) and V (N-major) tiles have the same image
+//   warp 20          issues the MMAs: per unit S_t = Q_t K^T and O_t += P_t V for both tiles; while one tile's softmax
 //                    runs, the tensor core works for the other
-//   warp 13          TMA of codes, bulk copies of scales and biases
+//   warp 21          TMA of codes, bulk copies of scales and biases
 // K and V tiles share a ring of three 32 KB buffers, their codes one of three stages: K(i), V(i), K(i+1), ...
 //
 // The reference follows lazily, as in the narrow kernel: only when a row of the warp exceeds it by 2^8 is O rescaled in tensor
-// memory.  The scores are read twice (maximum, weights), 64 at a time in loops that are not unrolled: a single unrolled
-// pass that was repeated when the maximum had to follow ran out of the instruction cache (387 against 314 us for two
-// sequences of 768 and 1024 new tokens over 3750 and 5000 cached ones, 32 heads on 8).
+// memory.  The scores are read twice (maximum, weights), 32 at a time in loops that are not unrolled.  A chunk of two
+// prompts (768 and 1024 new tokens over 3750 and 5000 cached ones, 32 heads on 8): 387 us with one unrolled pass that was
+// repeated when the reference had to follow (it ran out of the instruction cache), 262 with two passes and one thread a
+// row, TTT with two threads a row.
 // What bounds it: 2 x 128 x 128 exponentials per unit (16 per clock and SM) and as many clocks of tensor work; what keeps it
 // from there is the way of one tile's unit through scores, softmax, weights and second product, which the other tile
 // covers only in part.
@@ -32,8 +33,8 @@ namespace attend {
 
 constexpr int kWideKeys = 128;
 constexpr int kWideRows = 256;
-constexpr int kWideThreads = 14 * 32;    // 128 registers each
-constexpr int kDequantWarp0 = 8, kDequantWarps = 4, kMmaWarp = 12, kLoadWarp = 13;
+constexpr int kWideThreads = 22 * 32;    // 80 registers each
+constexpr int kDequantWarp0 = 16, kDequantWarps = 4, kMmaWarp = 20, kLoadWarp = 21;
 constexpr int kInfo = 4;             // units whose side information is kept
 constexpr float kMinFactor = 1.0e-37f;   // of raw scores: not 0, since hidden ones are -inf
 constexpr int kMinExp = -50;         // values below 2^-36 lose bits instead of pushing the weights out of f32
@@ -138,6 +139,7 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
     __shared__ float s_kmul[kInfo][4], s_vexp[kInfo][4], s_vinv[kInfo][4];
     __shared__ uint32_t s_kbad[kInfo], s_lost[kInfo][4];
     __shared__ uint8_t s_poison[kInfo][kWideKeys];  // by key
+    __shared__ float s_pair[2][2][128];             // what the two threads of a row tell each other
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_abort;
     __shared__ uint32_t s_scan[kWideThreads / 32];
@@ -161,9 +163,9 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
         }
         mbar_init(smem_u32(&s_idle), 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&s_q_ready[i]), 128);
+            mbar_init(smem_u32(&s_q_ready[i]), 256);
             mbar_init(smem_u32(&s_score[i]), 1);
-            mbar_init(smem_u32(&s_weights[i]), 128);
+            mbar_init(smem_u32(&s_weights[i]), 256);
             mbar_init(smem_u32(&s_done[i]), 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -287,13 +289,13 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                 const uint32_t kxi = kx + 2u * i, buf = kxi % W::TILES;
                 const uint64_t kd = k_desc + ((buf * W::TILE) >> 4);
                 const uint32_t free_bar = smem_u32(&s_tile_empty[buf]);
+                wait(s_tile_full[buf], (kxi / W::TILES) & 1u);     // ready long before the weights as a rule
                 for (uint32_t t = 0; t < tiles; ++t) {
                     if (i > 0) second(t, i - 1u);
                     else wait(s_q_ready[t], q_seen[t]++ & 1u);
                     const uint64_t qd = q_desc + ((t * W::TILE) >> 4);
                     const uint32_t out = tmem + 128u * t, score_bar = smem_u32(&s_score[t]);
                     const bool last_tile = t + 1u == tiles;
-                    if (t == 0u) wait(s_tile_full[buf], (kxi / W::TILES) & 1u);
                     fence_after();
                     if (elect_one()) {
                         umma_ss(out, qd, kd, kIdescS, 0u);
@@ -423,10 +425,19 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
             if (++elem == p.elements) elem = 0, ++head;
         }
     } else {
-        // ---------------- softmax: thread = query row ----------------
-        const uint32_t t = warp >> 2, r = threadIdx.x & 127u;       // row r of tile t
+        // ---------------- softmax: two threads per query row ----------------
+        const uint32_t t = warp >> 3, half = (warp >> 2) & 1u, r = (warp & 3u) * 32u + lane;       // row r of tile t, keys 64 half ..
         const uint32_t tm = tmem + ((static_cast<uint32_t>(warp) & 3u) << 21);     // this warp's lanes
-        const uint32_t tm_s = tm + 128u * t, tm_o = tm + 256u + 128u * t;
+        const uint32_t tm_s = tm + 128u * t + 64u * half, tm_w = tm + 128u * t + 32u * half, tm_o = tm + 256u + 128u * t + (D / 2) * half;
+        const uint32_t pair_bar = 1u + t * 4u + (warp & 3u);
+        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory"); };
+        // the other thread's value; the barrier in front of the write keeps the last exchange's values until they are read
+        auto exchange = [&](float v) {
+            pair_sync();
+            s_pair[t][half][r] = v;
+            pair_sync();
+            return s_pair[t][half ^ 1u][r];
+        };
         uint32_t kx = 0, scores_seen = 0, done_seen = 0;
         for (uint64_t u = u0; u < u1;) {
             const Item item = next_item<kWideRows, kWideKeys>(p, head, elem);
@@ -440,37 +451,39 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
             const bool whole = tile0 == 0u && count == item.tiles;
             float *const part = p.partials + static_cast<uint64_t>(2u * blockIdx.x + (tile0 == 0u ? 1u : 0u)) * W::PART;
             if (active) {
-                // ---- q: scaled by a power of two, f16 ----
+                // ---- q: scaled by a power of two, f16; each thread half of the row ----
                 float f;
                 {
-                    uint32_t x[D / 2];      // bf16 pairs
+                    uint32_t x[D / 4];      // bf16 pairs
 #pragma unroll
-                    for (int i = 0; i < D / 2; ++i) x[i] = 0u;
+                    for (int i = 0; i < D / 4; ++i) x[i] = 0u;
                     if (have) {
                         const uint16_t *src = static_cast<const uint16_t *>(p.a.q) + static_cast<uint64_t>(item.token0 + row / p.per_kv) * p.a.qs.token +
-                                              static_cast<uint64_t>(head * p.per_kv + row % p.per_kv) * p.a.qs.head;
+                                              static_cast<uint64_t>(head * p.per_kv + row % p.per_kv) * p.a.qs.head + half * (D / 2);
                         if (p.q_vec) {
 #pragma unroll
-                            for (int i = 0; i < D / 8; ++i) {
+                            for (int i = 0; i < D / 16; ++i) {
                                 const uint4 y = *reinterpret_cast<const uint4 *>(src + 8 * i);
                                 x[4 * i] = y.x, x[4 * i + 1] = y.y, x[4 * i + 2] = y.z, x[4 * i + 3] = y.w;
                             }
                         } else {
 #pragma unroll
-                            for (int i = 0; i < D / 2; ++i) x[i] = src[2 * i] | (static_cast<uint32_t>(src[2 * i + 1]) << 16);
+                            for (int i = 0; i < D / 4; ++i) x[i] = src[2 * i] | (static_cast<uint32_t>(src[2 * i + 1]) << 16);
                         }
                     }
                     uint32_t top = 0u;
 #pragma unroll
-                    for (int i = 0; i < D / 2; ++i) top = max(top, max((x[i] << 16) & 0x7FFFFFFFu, x[i] & 0x7FFF0000u));
+                    for (int i = 0; i < D / 4; ++i) top = max(top, max((x[i] << 16) & 0x7FFFFFFFu, x[i] & 0x7FFF0000u));
+                    __syncwarp();
+                    top = max(top, __float_as_uint(exchange(__uint_as_float(top))));
                     int e = static_cast<int>(top >> 23) - 127;
                     e = e < -100 ? -100 : e > 127 ? 127 : e;
                     // the sign of the scale goes to q, so that the largest raw score is the largest score
                     const float mul = p.a.scale < 0.0f ? -pow2(13 - e) : pow2(13 - e);
                     f = pow2(e - 13) * (fabsf(p.a.scale) * 1.4426950408889634f);
-                    const uint32_t dst = q_base + t * W::TILE + r * 128u;
+                    const uint32_t dst = q_base + t * W::TILE + r * 128u + (D == 128 ? half * W::PANEL : 0u);
 #pragma unroll
-                    for (int c = 0; c < D / 8; ++c) {
+                    for (int c = 0; c < D / 16; ++c) {
                         uint32_t y[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -479,7 +492,8 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                             y[i] = pack_f16x2(((d0 & 1) ? __uint_as_float(w0 & 0xFFFF0000u) : bf16_f32(w0)) * mul,
                                               ((d1 & 1) ? __uint_as_float(w1 & 0xFFFF0000u) : bf16_f32(w1)) * mul);
                         }
-                        const uint32_t at = dst + (c / 8) * W::PANEL + (((c & 7) ^ (r & 7u)) << 4);
+                        const uint32_t chunk = D == 128 ? c : half * (D / 16) + c;
+                        const uint32_t at = dst + ((chunk ^ (r & 7u)) << 4);
                         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
                     }
                 }
@@ -498,94 +512,104 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                     __syncwarp();
                     fence_after();
                     const uint32_t bad = s_kbad[info];
-                    const bool border = key0 + kWideKeys > item.first_seen || bad != 0u;
-                    // 64 raw scores, those that the row does not see taken out
-                    auto scores = [&](int c, uint32_t (&raw)[64]) {
-                        tmem_ld32(tm_s + 64u * c, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
-                        tmem_ld32(tm_s + 64u * c + 32u, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
+                    // 32 raw scores; kBorder: those that the row does not see taken out
+                    auto scores = [&](auto border_tag, int c, uint32_t (&raw)[32]) {
+                        tmem_ld32(tm_s + 32u * c, raw);
                         tmem_wait_ld();
-                        if (border) {
-                            const int32_t left = seen - key0 - 64 * c;
+                        if (decltype(border_tag)::value) {
+                            const int32_t left = seen - key0 - 64 * static_cast<int32_t>(half) - 32 * c;
+                            const uint32_t gone = bad >> (4u * half + 2u * c);
 #pragma unroll
-                            for (int k = 0; k < 64; ++k)
-                                if (k >= left || ((bad >> (4 * c + k / 16)) & 1u)) raw[k] = 0xFF800000u;
+                            for (int k = 0; k < 32; ++k)
+                                if (k >= left || ((gone >> (k / 16)) & 1u)) raw[k] = 0xFF800000u;
                         }
                     };
-                    float top = -INFINITY;
+                    auto unit = [&](auto border_tag) {
+                        float top = -INFINITY;
 #pragma unroll 1
-                    for (int c = 0; c < kWideKeys / 64; ++c) {
-                        uint32_t raw[64];
-                        scores(c, raw);
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            float t0 = __uint_as_float(raw[32 * x]), t1 = __uint_as_float(raw[32 * x + 1]);
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t raw[32];
+                            scores(border_tag, c, raw);
+                            float t0 = __uint_as_float(raw[0]), t1 = __uint_as_float(raw[1]);
 #pragma unroll
                             for (int k = 2; k < 32; k += 2) {
-                                t0 = fmaxf(t0, __uint_as_float(raw[32 * x + k]));
-                                t1 = fmaxf(t1, __uint_as_float(raw[32 * x + k + 1]));
+                                t0 = fmaxf(t0, __uint_as_float(raw[k]));
+                                t1 = fmaxf(t1, __uint_as_float(raw[k + 1]));
                             }
-                            top = fmaxf(top, fmaf(fmaxf(t0, t1), fmaxf(f * s_kmul[info][2 * c + x], kMinFactor), s_vexp[info][2 * c + x]));
+                            top = fmaxf(top, fmaf(fmaxf(t0, t1), fmaxf(f * s_kmul[info][2 * half + c], kMinFactor), s_vexp[info][2 * half + c]));
                         }
-                    }
-                    if (__any_sync(0xFFFFFFFFu, top > m + kLazy)) {
-                        const float m1 = fmaxf(m, top);
-                        const float keep = m1 == m ? 1.0f : exp2_approx(m - m1);
-                        m = m1;
-                        l *= keep;
-                        if (i > 0) {
+                        top = fmaxf(top, exchange(top));
+                        if (__any_sync(0xFFFFFFFFu, top > m + kLazy)) {
+                            const float m1 = fmaxf(m, top);
+                            const float keep = m1 == m ? 1.0f : exp2_approx(m - m1);
+                            m = m1;
+                            l *= keep;
+                            if (i > 0) {
 #pragma unroll 1
-                            for (int c = 0; c < D / 32; ++c) {
-                                uint32_t raw[32];
-                                tmem_ld32(tm_o + 32u * c, raw);
-                                tmem_wait_ld();
+                                for (int c = 0; c < D / 64; ++c) {
+                                    uint32_t raw[32];
+                                    tmem_ld32(tm_o + 32u * c, raw);
+                                    tmem_wait_ld();
 #pragma unroll
-                                for (int k = 0; k < 32; ++k) raw[k] = __float_as_uint(__uint_as_float(raw[k]) * keep);
-                                tmem_st32(tm_o + 32u * c, raw);
+                                    for (int k = 0; k < 32; ++k) raw[k] = __float_as_uint(__uint_as_float(raw[k]) * keep);
+                                    tmem_st32(tm_o + 32u * c, raw);
+                                }
                             }
                         }
-                    }
-                    // the weights of 64 keys take half of the columns that their scores had
-#pragma unroll 1
-                    for (int c = 0; c < kWideKeys / 64; ++c) {
-                        uint32_t raw[64];
-                        scores(c, raw);
+                        // the weights of 32 keys take 16 of the row's first 64 columns.  The other thread may still be reading
+                        // scores there: its weights wait until both are through (the loop writes after its last read)
+                        uint32_t w[32];
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const float fk = fmaxf(f * s_kmul[info][2 * c + x], kMinFactor), use = s_vexp[info][2 * c + x] - m;
-                            float sum0 = 0.0f, sum1 = 0.0f;
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t raw[32];
+                            scores(border_tag, c, raw);
+                            const float fk = fmaxf(f * s_kmul[info][2 * half + c], kMinFactor), use = s_vexp[info][2 * half + c] - m;
+                            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                            for (int k = 32 * x; k < 32 * x + 32; k += 2) {
-                                const float p0 = exp2_approx(fmaf(__uint_as_float(raw[k]), fk, use)), p1 = exp2_approx(fmaf(__uint_as_float(raw[k + 1]), fk, use));
-                                sum0 += p0;
-                                sum1 += p1;
-                                raw[k / 2] = pack_f16x2(p0, p1);
+                            for (int y = 0; y < 2; ++y) {
+                                float e[16];
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) e[k] = fmaf(__uint_as_float(raw[16 * y + k]), fk, use);
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) e[k] = exp2_approx(e[k]);
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) sum[k & 3] += e[k];
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) w[16 * c + 8 * y + k] = pack_f16x2(e[2 * k], e[2 * k + 1]);
                             }
-                            l = fmaf(sum0 + sum1, s_vinv[info][2 * c + x], l);
+                            l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), s_vinv[info][2 * half + c], l);
                         }
-                        tmem_st32(tm_s + 32u * c, raw);
+                        pair_sync();
+                        tmem_st32(tm_w, w);
+                    };
+                    if (key0 + kWideKeys > item.first_seen || bad != 0u) unit(std::true_type());
+                    else unit(std::false_type());
+                    if (s_lost[info][2 * half] | s_lost[info][2 * half + 1]) {
+                        for (uint32_t k = 64u * half; k < 64u * half + 64u; ++k)
+                            if (key0 + static_cast<int32_t>(k) < seen && ((s_lost[info][k >> 5] >> (k & 31u)) & 1u)) poison |= s_poison[info][k];
+                        __syncwarp();
                     }
-                    if (s_lost[info][0] | s_lost[info][1] | s_lost[info][2] | s_lost[info][3]) {
-                        for (int k = 0; k < kWideKeys; ++k)
-                            if (key0 + k < seen && ((s_lost[info][k >> 5] >> (k & 31)) & 1u)) poison |= s_poison[info][k];
-                    }
-                    __syncwarp();
                     tmem_wait_st();
                     fence_before();
                     mbar_arrive(smem_u32(&s_weights[t]));
                 }
                 // ---- end of the segment ----
+                l += exchange(l);
+                poison |= __float_as_uint(exchange(__uint_as_float(poison)));
                 wait(s_done[t], done_seen++ & 1u);
                 __syncwarp();
                 fence_after();
-                if (!whole && have) {
+                if (!whole && have && half == 0u) {
                     __stcg(part + kWideRows * D + t * 128u + r, m);
                     __stcg(part + kWideRows * (D + 1) + t * 128u + r, l);
                 }
 #pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
+                for (int c = 0; c < D / 64; ++c) {
                     uint32_t raw[32];
                     tmem_ld32(tm_o + 32u * c, raw);
                     tmem_wait_ld();
+                    const uint32_t d0 = half * (D / 2) + 32u * c;
+                    const bool lost = (poison >> (d0 / GROUP)) & 1u;
 #pragma unroll
                     for (int x = 0; x < 8; ++x) {
                         if (!have) break;
@@ -594,10 +618,9 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                         for (int k = 0; k < 4; ++k) {
                             // value 4x + k of the 32 stands at the place that its eight keep it
                             const int in = (4 * x + k) % 8, place = BITS == 8 ? in : ((in & 3) * 2 + (in >> 2));
-                            v[k] = __uint_as_float(raw[(4 * x + k) / 8 * 8 + place]);
+                            v[k] = lost ? __uint_as_float(0x7FC00000u) : __uint_as_float(raw[(4 * x + k) / 8 * 8 + place]);
                         }
-                        if ((poison >> (c * 32 / GROUP)) & 1u) v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7FC00000u);
-                        const uint32_t d = 32u * c + 4u * x;
+                        const uint32_t d = d0 + 4u * x;
                         if (whole) finish_row<D, false>(p, item, head, t * 128u + r, d, m, l, make_float4(v[0], v[1], v[2], v[3]));
                         else __stcg(reinterpret_cast<float4 *>(part + (static_cast<uint64_t>(d / 4u) * kWideRows + t * 128u + r) * 4u), make_float4(v[0], v[1], v[2], v[3]));
                     }
@@ -611,35 +634,39 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                 const uint32_t c0 = static_cast<uint32_t>(((first_unit + 1) * range.ctas - 1) / range.units);
                 const uint32_t c1 = static_cast<uint32_t>(((first_unit + item.tiles) * range.ctas - 1) / range.units);
                 __threadfence();
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                asm volatile("bar.sync 9, 512;" ::: "memory");
                 if (threadIdx.x == 0) {
                     const uint32_t seen = atomicAdd(p.tickets + c0, 1u);
                     s_last = seen == c1 - c0;
                     if (s_last) p.tickets[c0] = 0u;
                 }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                asm volatile("bar.sync 9, 512;" ::: "memory");
                 if (s_last && have) {
                     __threadfence();
                     const uint32_t rr = t * 128u + r;
                     auto part_of = [&](uint32_t c) { return p.partials + static_cast<uint64_t>(2u * c + (c == c0 ? 1u : 0u)) * W::PART; };
-                    float top = -INFINITY, sum = 0.0f;
+                    float top = kNoMax, sum = 0.0f;
                     for (uint32_t c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(part_of(c) + kWideRows * D + rr));
                     for (uint32_t c = c0; c <= c1; ++c) {
                         const float mc = __ldcg(part_of(c) + kWideRows * D + rr);
                         sum += __ldcg(part_of(c) + kWideRows * (D + 1) + rr) * (mc == top ? 1.0f : exp2_approx(mc - top));
                     }
-                    for (uint32_t d = 0; d < static_cast<uint32_t>(D); d += 4u) {
-                        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (uint32_t d = half * (D / 2); d < (half + 1u) * (D / 2); d += 8u) {
+                        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f), w = v;
                         for (uint32_t c = c0; c <= c1; ++c) {
-                            const float mc = __ldcg(part_of(c) + kWideRows * D + rr);
+                            const float *src = part_of(c);
+                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(src + (static_cast<uint64_t>(d / 4u) * kWideRows + rr) * 4u));
+                            const float4 y = __ldcg(reinterpret_cast<const float4 *>(src + (static_cast<uint64_t>(d / 4u + 1u) * kWideRows + rr) * 4u));
+                            const float mc = __ldcg(src + kWideRows * D + rr);
                             const float wc = mc == top ? 1.0f : exp2_approx(mc - top);
-                            const float4 y = __ldcg(reinterpret_cast<const float4 *>(part_of(c) + (static_cast<uint64_t>(d / 4u) * kWideRows + rr) * 4u));
-                            v = make_float4(fmaf(y.x, wc, v.x), fmaf(y.y, wc, v.y), fmaf(y.z, wc, v.z), fmaf(y.w, wc, v.w));
+                            v = make_float4(fmaf(x.x, wc, v.x), fmaf(x.y, wc, v.y), fmaf(x.z, wc, v.z), fmaf(x.w, wc, v.w));
+                            w = make_float4(fmaf(y.x, wc, w.x), fmaf(y.y, wc, w.y), fmaf(y.z, wc, w.z), fmaf(y.w, wc, w.w));
                         }
                         finish_row<D, false>(p, item, head, rr, d, top, sum, v);
+                        finish_row<D, false>(p, item, head, rr, d + 4u, top, sum, w);
                     }
                 }
-                asm volatile("bar.sync 1, 256;" ::: "memory");   // s_last is free again
+                asm volatile("bar.sync 9, 512;" ::: "memory");   // s_last is free again
             }
             u += count;
             tile0 = 0;
