@@ -172,6 +172,7 @@ struct Params {
     float *prefix_lse;      // [rows], base 2
     float *partials;        // [2 * gridDim.x][R * (D + 2)]
     unsigned int *tickets;  // [gridDim.x], zero between launches
+    struct Cut *cuts;       // [gridDim.x] of the wide kernel
     uint32_t q_vec, o_vec;  // rows of q / out can be read / written by vectors
 };
 
@@ -185,6 +186,12 @@ struct Item {
     int32_t seen0;       // keys that the sequence's first new token sees
     int64_t token0;      // packed row of the sequence's first new token
     int32_t seq;
+};
+
+// An item that begins in a CTA of the wide kernel and goes on in the next `parts` - 1; parts = 0: none.
+struct Cut {
+    Item item;
+    uint32_t head, parts;
 };
 
 template <int R, int KEYS>
@@ -1053,8 +1060,8 @@ cudaError_t launch_rows(const Params &p, const CUtensorMap &tmap, int nt, int li
 // tcgen05, bf16 rows (gaf_attend_wide.cuh): 256 rows a tile
 cudaError_t launch_wide(const Params &p, const CUtensorMap &tmap, int sm_count, cudaStream_t stream);
 
-constexpr int kMaxCtas = 3;             // per SM, of any instance
-constexpr int kMaxPartRows = 256 * 2;   // rows of the partial results of an SM's CTAs (3 CTAs x 2 slots x 32 rows; 1 x 2 x 256)
+constexpr int kMaxCtas = 4;             // per SM, of any instance
+constexpr int kMaxPartRows = 256 * 2;   // rows of the partial results of an SM's CTAs (4 CTAs x 2 slots x 32 rows; 1 x 2 x 256)
 constexpr int kMaxDim = 128;
 
 }  // namespace attend

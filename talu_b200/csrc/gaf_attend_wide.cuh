@@ -9,19 +9,20 @@
 // 2), where m follows the largest y + e instead of the largest y, and leave it again in the row's sum.
 //
 // One CTA per SM, 256 query rows (two MMA tiles of 128) against units of 128 keys:
-//   warps 0-7, 8-15  softmax of tile 0 and 1, two threads per row with 64 keys each: scores from tensor memory, weights (f16)
-//                    back into the scores' columns, where the second product takes them as its A operand
-//   warps 16-19      dequantise, one cached row per thread; K (K-major) and V (N-major) tiles have the same image
-//   warp 20          issues the MMAs: per unit S_t = Q_t K^T and O_t += P_t V for both tiles; while one tile's softmax
+//   warps 0-3, 4-7   softmax of tile 0 and 1, one row per thread: scores from tensor memory, weights (f16) back into the
+//                    scores' columns, where the second product takes them as its A operand
+//   warps 8-11       dequantise, one cached row per thread; K (K-major) and V (N-major) tiles have the same image
+//   warp 12          issues the MMAs: per unit S_t = Q_t K^T and O_t += P_t V for both tiles; while one tile's softmax
 //                    runs, the tensor core works for the other
-//   warp 21          TMA of codes, bulk copies of scales and biases
+//   warp 13          TMA of codes, bulk copies of scales and biases
 // K and V tiles share a ring of three 32 KB buffers, their codes one of three stages: K(i), V(i), K(i+1), ...
 //
-// The reference follows lazily, as in the narrow kernel: only when a row of the warp exceeds it by 2^8 is O rescaled in tensor
-// memory.  The scores are read twice (maximum, weights), 32 at a time in loops that are not unrolled.  A chunk of two
-// prompts (768 and 1024 new tokens over 3750 and 5000 cached ones, 32 heads on 8): 387 us with one unrolled pass that was
-// repeated when the reference had to follow (it ran out of the instruction cache), 262 with two passes and one thread a
-// row, TTT with two threads a row.
+// The reference follows lazily, as in the narrow kernel: only when a row of the warp exceeds it by 2^8 are O (and the weights
+// of the unit that are formed already) rescaled in tensor memory.  A row's thread takes 32 scores at a time, the next 32 on
+// their way, and puts their weights into columns whose scores it has read.  Measured on a chunk of two prompts (768 and
+// 1024 new tokens over 3750 and 5000 cached ones, 32 heads on 8): TTT us; 262 with a pass of its own for the maximum,
+// 256 with that and two threads a row, 334 with two buffers of 64 keys for the scores (twice the MMAs, of half the
+// width: the issuing warp does not keep up), 387 with everything unrolled (instruction cache).
 // What bounds it: 2 x 128 x 128 exponentials per unit (16 per clock and SM) and as many clocks of tensor work; what keeps it
 // from there is the way of one tile's unit through scores, softmax, weights and second product, which the other tile
 // covers only in part.
@@ -33,8 +34,8 @@ namespace attend {
 
 constexpr int kWideKeys = 128;
 constexpr int kWideRows = 256;
-constexpr int kWideThreads = 22 * 32;    // 80 registers each
-constexpr int kDequantWarp0 = 16, kDequantWarps = 4, kMmaWarp = 20, kLoadWarp = 21;
+constexpr int kWideThreads = 14 * 32;    // 128 registers each
+constexpr int kDequantWarp0 = 8, kDequantWarps = 4, kMmaWarp = 12, kLoadWarp = 13;
 constexpr int kInfo = 4;             // units whose side information is kept
 constexpr float kMinFactor = 1.0e-37f;   // of raw scores: not 0, since hidden ones are -inf
 constexpr int kMinExp = -50;         // values below 2^-36 lose bits instead of pushing the weights out of f32
@@ -84,6 +85,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr)
         : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
     asm volatile(
@@ -139,12 +153,10 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
     __shared__ float s_kmul[kInfo][4], s_vexp[kInfo][4], s_vinv[kInfo][4];
     __shared__ uint32_t s_kbad[kInfo], s_lost[kInfo][4];
     __shared__ uint8_t s_poison[kInfo][kWideKeys];  // by key
-    __shared__ float s_pair[2][2][128];             // what the two threads of a row tell each other
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_abort;
     __shared__ uint32_t s_scan[kWideThreads / 32];
     __shared__ uint32_t s_begin[3];
-    __shared__ uint32_t s_last;
 
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_base = base, tile_base = q_base + 2 * W::TILE, code_base = tile_base + W::TILES * W::TILE;
@@ -163,15 +175,19 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
         }
         mbar_init(smem_u32(&s_idle), 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&s_q_ready[i]), 256);
+            mbar_init(smem_u32(&s_q_ready[i]), 128);
             mbar_init(smem_u32(&s_score[i]), 1);
-            mbar_init(smem_u32(&s_weights[i]), 256);
+            mbar_init(smem_u32(&s_weights[i]), 128);
             mbar_init(smem_u32(&s_done[i]), 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     Range range;
-    if (!cta_range<kWideRows, kWideKeys, kWideThreads>(p, s_scan, s_begin, range)) return;
+    if (!cta_range<kWideRows, kWideKeys, kWideThreads>(p, s_scan, s_begin, range)) {
+        if (threadIdx.x == 0) p.cuts[blockIdx.x].parts = 0u;
+        return;
+    }
+    if (threadIdx.x == 0) p.cuts[blockIdx.x].parts = 0u;     // until a segment says otherwise
     const uint64_t u0 = range.u0, u1 = range.u1;
     uint32_t head = s_begin[0], elem = s_begin[1], tile0 = s_begin[2];
     if (warp == kMmaWarp) {
@@ -376,45 +392,47 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                         }
                     }
                     const float mul = pow2(-e);          // e between -114 and 114
-                    uint32_t sh[GS], bh[GS];
-#pragma unroll
-                    for (int i = 0; i < GS; ++i) {
-                        if (which == 1u && ((poison >> i) & 1u)) s[i] = b[i] = 0.0f;
-                        const float sc = s[i] * mul, bc = fmaf(kHalf, s[i], b[i]) * mul;
-                        sh[i] = pack_f16x2(sc, sc);
-                        bh[i] = pack_f16x2(bc, bc);
-                    }
-                    constexpr int kChunks = RB / 16;                 // 16-byte chunks of codes in a row
-                    constexpr int kOut = BITS == 8 ? 2 : 4;          // 16-byte chunks of f16 that 16 bytes of codes make
-                    uint32_t w[kChunks][4];
-#pragma unroll
-                    for (int c = 0; c < kChunks; ++c) lds<16>(src + row * RB + ((c ^ swz) << 4), w[c]);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&s_code_empty[stage]));
                     if (hx >= static_cast<uint32_t>(W::TILES)) wait(s_tile_empty[buf], (hx / W::TILES - 1u) & 1u);
                     __syncwarp();
-                    const uint32_t dst = tile_base + buf * W::TILE + row * 128u;
+                    constexpr int kChunks = RB / 16;                 // 16-byte chunks of codes in a row
+                    constexpr int kOut = BITS == 8 ? 2 : 4;          // 16-byte chunks of f16 that 16 bytes of codes make
+                    const uint32_t dst = tile_base + buf * W::TILE + row * 128u, from = src + row * RB, scale_at = src + W::CODES + row * GS * 2;
+                    // not unrolled: the roles share the instruction cache
+#pragma unroll 1
+                    for (uint32_t g = 0; g < static_cast<uint32_t>(GS); ++g) {
+                        uint32_t si, bi;
+                        lds<2>(scale_at + g * 2u, &si);
+                        lds<2>(scale_at + W::SB + g * 2u, &bi);
+                        const bool none = !valid || (which == 1u && ((poison >> g) & 1u));
+                        const float sg = none ? 0.0f : bf16_f32(si), bg = none ? 0.0f : bf16_f32(bi);
+                        const float sc = sg * mul, bc = fmaf(kHalf, sg, bg) * mul;
+                        const uint32_t sh = pack_f16x2(sc, sc), bh = pack_f16x2(bc, bc);
+#pragma unroll 1
+                        for (uint32_t c = g * (kChunks / GS); c < (g + 1u) * (kChunks / GS); ++c) {
+                            uint32_t w[4];
+                            lds<16>(from + ((c ^ swz) << 4), w);
 #pragma unroll
-                    for (int c = 0; c < kChunks; ++c) {
+                            for (int x = 0; x < kOut; ++x) {
+                                const uint32_t to = c * kOut + x;
+                                uint32_t y[4];
 #pragma unroll
-                        for (int x = 0; x < kOut; ++x) {
-                            const int chunk = c * kOut + x, gi = chunk * 8 / GROUP;
-                            uint32_t y[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                uint32_t code;
-                                if (BITS == 8) {
-                                    code = add_f16x2(prmt(w[c][2 * x + (i >> 1)], 0x64646464u, (i & 1) ? 0x4342u : 0x4140u), kCentre);
-                                } else {
-                                    const uint32_t n = i >= 2 ? w[c][x] >> 8 : w[c][x];
-                                    code = (i & 1) ? f16_high(n, kCentreHigh) : f16_low(n, kCentre);
+                                for (int i = 0; i < 4; ++i) {
+                                    uint32_t code;
+                                    if (BITS == 8) {
+                                        code = add_f16x2(prmt(w[2 * x + (i >> 1)], 0x64646464u, (i & 1) ? 0x4342u : 0x4140u), kCentre);
+                                    } else {
+                                        const uint32_t n = i >= 2 ? w[x] >> 8 : w[x];
+                                        code = (i & 1) ? f16_high(n, kCentreHigh) : f16_low(n, kCentre);
+                                    }
+                                    y[i] = fma_f16x2(code, sh, bh);
                                 }
-                                y[i] = fma_f16x2(code, sh[gi], bh[gi]);
+                                const uint32_t at = dst + (to / 8u) * W::PANEL + (((to & 7u) ^ (row & 7u)) << 4);
+                                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
                             }
-                            const uint32_t at = dst + (chunk / 8) * W::PANEL + (((chunk & 7) ^ (row & 7u)) << 4);
-                            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
                         }
                     }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&s_code_empty[stage]));
                     fence_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&s_tile_full[buf]));
@@ -425,19 +443,10 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
             if (++elem == p.elements) elem = 0, ++head;
         }
     } else {
-        // ---------------- softmax: two threads per query row ----------------
-        const uint32_t t = warp >> 3, half = (warp >> 2) & 1u, r = (warp & 3u) * 32u + lane;       // row r of tile t, keys 64 half ..
+        // ---------------- softmax: thread = query row ----------------
+        const uint32_t t = warp >> 2, r = threadIdx.x & 127u;       // row r of tile t
         const uint32_t tm = tmem + ((static_cast<uint32_t>(warp) & 3u) << 21);     // this warp's lanes
-        const uint32_t tm_s = tm + 128u * t + 64u * half, tm_w = tm + 128u * t + 32u * half, tm_o = tm + 256u + 128u * t + (D / 2) * half;
-        const uint32_t pair_bar = 1u + t * 4u + (warp & 3u);
-        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory"); };
-        // the other thread's value; the barrier in front of the write keeps the last exchange's values until they are read
-        auto exchange = [&](float v) {
-            pair_sync();
-            s_pair[t][half][r] = v;
-            pair_sync();
-            return s_pair[t][half ^ 1u][r];
-        };
+        const uint32_t tm_s = tm + 128u * t, tm_o = tm + 256u + 128u * t;
         uint32_t kx = 0, scores_seen = 0, done_seen = 0;
         for (uint64_t u = u0; u < u1;) {
             const Item item = next_item<kWideRows, kWideKeys>(p, head, elem);
@@ -451,39 +460,37 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
             const bool whole = tile0 == 0u && count == item.tiles;
             float *const part = p.partials + static_cast<uint64_t>(2u * blockIdx.x + (tile0 == 0u ? 1u : 0u)) * W::PART;
             if (active) {
-                // ---- q: scaled by a power of two, f16; each thread half of the row ----
+                // ---- q: scaled by a power of two, f16 ----
                 float f;
                 {
-                    uint32_t x[D / 4];      // bf16 pairs
+                    uint32_t x[D / 2];      // bf16 pairs
 #pragma unroll
-                    for (int i = 0; i < D / 4; ++i) x[i] = 0u;
+                    for (int i = 0; i < D / 2; ++i) x[i] = 0u;
                     if (have) {
                         const uint16_t *src = static_cast<const uint16_t *>(p.a.q) + static_cast<uint64_t>(item.token0 + row / p.per_kv) * p.a.qs.token +
-                                              static_cast<uint64_t>(head * p.per_kv + row % p.per_kv) * p.a.qs.head + half * (D / 2);
+                                              static_cast<uint64_t>(head * p.per_kv + row % p.per_kv) * p.a.qs.head;
                         if (p.q_vec) {
 #pragma unroll
-                            for (int i = 0; i < D / 16; ++i) {
+                            for (int i = 0; i < D / 8; ++i) {
                                 const uint4 y = *reinterpret_cast<const uint4 *>(src + 8 * i);
                                 x[4 * i] = y.x, x[4 * i + 1] = y.y, x[4 * i + 2] = y.z, x[4 * i + 3] = y.w;
                             }
                         } else {
 #pragma unroll
-                            for (int i = 0; i < D / 4; ++i) x[i] = src[2 * i] | (static_cast<uint32_t>(src[2 * i + 1]) << 16);
+                            for (int i = 0; i < D / 2; ++i) x[i] = src[2 * i] | (static_cast<uint32_t>(src[2 * i + 1]) << 16);
                         }
                     }
                     uint32_t top = 0u;
 #pragma unroll
-                    for (int i = 0; i < D / 4; ++i) top = max(top, max((x[i] << 16) & 0x7FFFFFFFu, x[i] & 0x7FFF0000u));
-                    __syncwarp();
-                    top = max(top, __float_as_uint(exchange(__uint_as_float(top))));
+                    for (int i = 0; i < D / 2; ++i) top = max(top, max((x[i] << 16) & 0x7FFFFFFFu, x[i] & 0x7FFF0000u));
                     int e = static_cast<int>(top >> 23) - 127;
                     e = e < -100 ? -100 : e > 127 ? 127 : e;
                     // the sign of the scale goes to q, so that the largest raw score is the largest score
                     const float mul = p.a.scale < 0.0f ? -pow2(13 - e) : pow2(13 - e);
                     f = pow2(e - 13) * (fabsf(p.a.scale) * 1.4426950408889634f);
-                    const uint32_t dst = q_base + t * W::TILE + r * 128u + (D == 128 ? half * W::PANEL : 0u);
+                    const uint32_t dst = q_base + t * W::TILE + r * 128u;
 #pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
+                    for (int c = 0; c < D / 8; ++c) {
                         uint32_t y[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -492,8 +499,7 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                             y[i] = pack_f16x2(((d0 & 1) ? __uint_as_float(w0 & 0xFFFF0000u) : bf16_f32(w0)) * mul,
                                               ((d1 & 1) ? __uint_as_float(w1 & 0xFFFF0000u) : bf16_f32(w1)) * mul);
                         }
-                        const uint32_t chunk = D == 128 ? c : half * (D / 16) + c;
-                        const uint32_t at = dst + ((chunk ^ (r & 7u)) << 4);
+                        const uint32_t at = dst + (c / 8) * W::PANEL + (((c & 7) ^ (r & 7u)) << 4);
                         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
                     }
                 }
@@ -505,88 +511,87 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
 
                 for (uint32_t i = 0; i < count; ++i) {
                     const int32_t key0 = static_cast<int32_t>((tile0 + i) * kWideKeys);
-                    // values are ready before the scores as a rule: waiting for them first takes that wait out of the way
                     const uint32_t vx = kx + 2u * i + 1u, info = (vx >> 1) % kInfo;
-                    wait(s_tile_full[vx % W::TILES], (vx / W::TILES) & 1u);
+                    // in this order: the scores are proof that the fill before the values' in their buffer is over, without which
+                    // the parity could be that of an older one (a tile that rests in a segment runs ahead of the other)
                     wait(s_score[t], scores_seen++ & 1u);
                     __syncwarp();
                     fence_after();
                     const uint32_t bad = s_kbad[info];
-                    // 32 raw scores; kBorder: those that the row does not see taken out
-                    auto scores = [&](auto border_tag, int c, uint32_t (&raw)[32]) {
-                        tmem_ld32(tm_s + 32u * c, raw);
-                        tmem_wait_ld();
-                        if (decltype(border_tag)::value) {
-                            const int32_t left = seen - key0 - 64 * static_cast<int32_t>(half) - 32 * c;
-                            const uint32_t gone = bad >> (4u * half + 2u * c);
+                    const bool border = key0 + kWideKeys > item.first_seen || bad != 0u;
+                    // 32 keys: scores to weights, which take half of the columns of scores that have been read
+                    auto chunk = [&](int c, uint32_t (&x)[32]) {
+                        const float fk = fmaxf(f * s_kmul[info][c], kMinFactor), ve = s_vexp[info][c];
+                        float tops[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
 #pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                if (k >= left || ((gone >> (k / 16)) & 1u)) raw[k] = 0xFF800000u;
-                        }
-                    };
-                    auto unit = [&](auto border_tag) {
-                        float top = -INFINITY;
-#pragma unroll 1
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t raw[32];
-                            scores(border_tag, c, raw);
-                            float t0 = __uint_as_float(raw[0]), t1 = __uint_as_float(raw[1]);
-#pragma unroll
-                            for (int k = 2; k < 32; k += 2) {
-                                t0 = fmaxf(t0, __uint_as_float(raw[k]));
-                                t1 = fmaxf(t1, __uint_as_float(raw[k + 1]));
-                            }
-                            top = fmaxf(top, fmaf(fmaxf(t0, t1), fmaxf(f * s_kmul[info][2 * half + c], kMinFactor), s_vexp[info][2 * half + c]));
-                        }
-                        top = fmaxf(top, exchange(top));
+                        for (int k = 4; k < 32; ++k) tops[k & 3] = fmaxf(tops[k & 3], __uint_as_float(x[k]));
+                        const float top = fmaf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fk, ve);
                         if (__any_sync(0xFFFFFFFFu, top > m + kLazy)) {
                             const float m1 = fmaxf(m, top);
                             const float keep = m1 == m ? 1.0f : exp2_approx(m - m1);
                             m = m1;
                             l *= keep;
-                            if (i > 0) {
 #pragma unroll 1
-                                for (int c = 0; c < D / 64; ++c) {
-                                    uint32_t raw[32];
-                                    tmem_ld32(tm_o + 32u * c, raw);
-                                    tmem_wait_ld();
+                            for (int y = i > 0 ? 0 : D / 16; y < D / 16 + c; ++y) {     // O, then this unit's weights so far
+                                uint32_t z[16];
+                                const uint32_t at = y < D / 16 ? tm_o + 16u * y : tm_s + 16u * (y - D / 16);
+                                tmem_ld16(at, z);
+                                tmem_wait_ld();
 #pragma unroll
-                                    for (int k = 0; k < 32; ++k) raw[k] = __float_as_uint(__uint_as_float(raw[k]) * keep);
-                                    tmem_st32(tm_o + 32u * c, raw);
+                                for (int k = 0; k < 16; ++k) {
+                                    if (y < D / 16) {
+                                        z[k] = __float_as_uint(__uint_as_float(z[k]) * keep);
+                                    } else {
+                                        const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&z[k]));
+                                        z[k] = pack_f16x2(v.x * keep, v.y * keep);
+                                    }
                                 }
+                                tmem_st16(at, z);
                             }
+                            tmem_wait_st();
                         }
-                        // the weights of 32 keys take 16 of the row's first 64 columns.  The other thread may still be reading
-                        // scores there: its weights wait until both are through (the loop writes after its last read)
-                        uint32_t w[32];
+                        const float use = ve - m;
+                        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        uint32_t w[16];
+                        float e[32];
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t raw[32];
-                            scores(border_tag, c, raw);
-                            const float fk = fmaxf(f * s_kmul[info][2 * half + c], kMinFactor), use = s_vexp[info][2 * half + c] - m;
-                            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        for (int k = 0; k < 32; ++k) e[k] = fmaf(__uint_as_float(x[k]), fk, use);
 #pragma unroll
-                            for (int y = 0; y < 2; ++y) {
-                                float e[16];
+                        for (int k = 0; k < 32; ++k) e[k] = exp2_approx(e[k]);
 #pragma unroll
-                                for (int k = 0; k < 16; ++k) e[k] = fmaf(__uint_as_float(raw[16 * y + k]), fk, use);
+                        for (int k = 0; k < 32; ++k) sum[k & 3] += e[k];
 #pragma unroll
-                                for (int k = 0; k < 16; ++k) e[k] = exp2_approx(e[k]);
-#pragma unroll
-                                for (int k = 0; k < 16; ++k) sum[k & 3] += e[k];
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) w[16 * c + 8 * y + k] = pack_f16x2(e[2 * k], e[2 * k + 1]);
-                            }
-                            l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), s_vinv[info][2 * half + c], l);
-                        }
-                        pair_sync();
-                        tmem_st32(tm_w, w);
+                        for (int k = 0; k < 16; ++k) w[k] = pack_f16x2(e[2 * k], e[2 * k + 1]);
+                        l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), s_vinv[info][c], l);
+                        tmem_st16(tm_s + 16u * c, w);
                     };
-                    if (key0 + kWideKeys > item.first_seen || bad != 0u) unit(std::true_type());
-                    else unit(std::false_type());
-                    if (s_lost[info][2 * half] | s_lost[info][2 * half + 1]) {
-                        for (uint32_t k = 64u * half; k < 64u * half + 64u; ++k)
-                            if (key0 + static_cast<int32_t>(k) < seen && ((s_lost[info][k >> 5] >> (k & 31u)) & 1u)) poison |= s_poison[info][k];
+                    if (border) {            // what the row does not see is taken out
+#pragma unroll 1
+                        for (int c = 0; c < 8; ++c) {
+                            const int32_t left = (bad >> c) & 1u ? 0 : seen - key0 - 16 * c;
+                            if (__all_sync(0xFFFFFFFFu, left >= 16)) continue;
+                            uint32_t x[16];
+                            tmem_ld16(tm_s + 16u * c, x);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 16; ++k)
+                                if (k >= left) x[k] = 0xFF800000u;
+                            tmem_st16(tm_s + 16u * c, x);
+                        }
+                        tmem_wait_st();
+                    }
+                    wait(s_tile_full[vx % W::TILES], (vx / W::TILES) & 1u);
+                    __syncwarp();
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t x[32];
+                        tmem_ld32(tm_s + 32u * c, x);
+                        tmem_wait_ld();
+                        chunk(c, x);
+                    }
+                    if (s_lost[info][0] | s_lost[info][1] | s_lost[info][2] | s_lost[info][3]) {
+                        for (int k = 0; k < kWideKeys; ++k)
+                            if (key0 + k < seen && ((s_lost[info][k >> 5] >> (k & 31)) & 1u)) poison |= s_poison[info][k];
                         __syncwarp();
                     }
                     tmem_wait_st();
@@ -594,22 +599,18 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                     mbar_arrive(smem_u32(&s_weights[t]));
                 }
                 // ---- end of the segment ----
-                l += exchange(l);
-                poison |= __float_as_uint(exchange(__uint_as_float(poison)));
                 wait(s_done[t], done_seen++ & 1u);
                 __syncwarp();
                 fence_after();
-                if (!whole && have && half == 0u) {
+                if (!whole && have) {
                     __stcg(part + kWideRows * D + t * 128u + r, m);
                     __stcg(part + kWideRows * (D + 1) + t * 128u + r, l);
                 }
 #pragma unroll 1
-                for (int c = 0; c < D / 64; ++c) {
+                for (int c = 0; c < D / 32; ++c) {
                     uint32_t raw[32];
                     tmem_ld32(tm_o + 32u * c, raw);
                     tmem_wait_ld();
-                    const uint32_t d0 = half * (D / 2) + 32u * c;
-                    const bool lost = (poison >> (d0 / GROUP)) & 1u;
 #pragma unroll
                     for (int x = 0; x < 8; ++x) {
                         if (!have) break;
@@ -618,9 +619,10 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                         for (int k = 0; k < 4; ++k) {
                             // value 4x + k of the 32 stands at the place that its eight keep it
                             const int in = (4 * x + k) % 8, place = BITS == 8 ? in : ((in & 3) * 2 + (in >> 2));
-                            v[k] = lost ? __uint_as_float(0x7FC00000u) : __uint_as_float(raw[(4 * x + k) / 8 * 8 + place]);
+                            v[k] = __uint_as_float(raw[(4 * x + k) / 8 * 8 + place]);
                         }
-                        const uint32_t d = d0 + 4u * x;
+                        if ((poison >> (c * 32 / GROUP)) & 1u) v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7FC00000u);
+                        const uint32_t d = 32u * c + 4u * x;
                         if (whole) finish_row<D, false>(p, item, head, t * 128u + r, d, m, l, make_float4(v[0], v[1], v[2], v[3]));
                         else __stcg(reinterpret_cast<float4 *>(part + (static_cast<uint64_t>(d / 4u) * kWideRows + t * 128u + r) * 4u), make_float4(v[0], v[1], v[2], v[3]));
                     }
@@ -629,44 +631,13 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                 fence_before();
             }
             kx += 2u * count;
-            if (!whole) {
-                const uint64_t first_unit = u - tile0;
-                const uint32_t c0 = static_cast<uint32_t>(((first_unit + 1) * range.ctas - 1) / range.units);
-                const uint32_t c1 = static_cast<uint32_t>(((first_unit + item.tiles) * range.ctas - 1) / range.units);
-                __threadfence();
-                asm volatile("bar.sync 9, 512;" ::: "memory");
-                if (threadIdx.x == 0) {
-                    const uint32_t seen = atomicAdd(p.tickets + c0, 1u);
-                    s_last = seen == c1 - c0;
-                    if (s_last) p.tickets[c0] = 0u;
-                }
-                asm volatile("bar.sync 9, 512;" ::: "memory");
-                if (s_last && have) {
-                    __threadfence();
-                    const uint32_t rr = t * 128u + r;
-                    auto part_of = [&](uint32_t c) { return p.partials + static_cast<uint64_t>(2u * c + (c == c0 ? 1u : 0u)) * W::PART; };
-                    float top = kNoMax, sum = 0.0f;
-                    for (uint32_t c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(part_of(c) + kWideRows * D + rr));
-                    for (uint32_t c = c0; c <= c1; ++c) {
-                        const float mc = __ldcg(part_of(c) + kWideRows * D + rr);
-                        sum += __ldcg(part_of(c) + kWideRows * (D + 1) + rr) * (mc == top ? 1.0f : exp2_approx(mc - top));
-                    }
-                    for (uint32_t d = half * (D / 2); d < (half + 1u) * (D / 2); d += 8u) {
-                        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f), w = v;
-                        for (uint32_t c = c0; c <= c1; ++c) {
-                            const float *src = part_of(c);
-                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(src + (static_cast<uint64_t>(d / 4u) * kWideRows + rr) * 4u));
-                            const float4 y = __ldcg(reinterpret_cast<const float4 *>(src + (static_cast<uint64_t>(d / 4u + 1u) * kWideRows + rr) * 4u));
-                            const float mc = __ldcg(src + kWideRows * D + rr);
-                            const float wc = mc == top ? 1.0f : exp2_approx(mc - top);
-                            v = make_float4(fmaf(x.x, wc, v.x), fmaf(x.y, wc, v.y), fmaf(x.z, wc, v.z), fmaf(x.w, wc, v.w));
-                            w = make_float4(fmaf(y.x, wc, w.x), fmaf(y.y, wc, w.y), fmaf(y.z, wc, w.z), fmaf(y.w, wc, w.w));
-                        }
-                        finish_row<D, false>(p, item, head, rr, d, top, sum, v);
-                        finish_row<D, false>(p, item, head, rr, d + 4u, top, sum, w);
-                    }
-                }
-                asm volatile("bar.sync 9, 512;" ::: "memory");   // s_last is free again
+            if (tile0 == 0u && !whole && threadIdx.x == 0) {
+                // the item goes on in the next CTAs: the pass that joins their results finds it here
+                const uint32_t last = static_cast<uint32_t>(((u + item.tiles) * range.ctas - 1) / range.units);
+                Cut &cut = p.cuts[blockIdx.x];
+                cut.item = item;
+                cut.head = head;
+                cut.parts = last - blockIdx.x + 1u;
             }
             u += count;
             tile0 = 0;
@@ -679,6 +650,41 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
+// Joins the results of items that were cut across CTAs: grid (CTAs of the wide kernel) x (blocks of 32 rows), thread = a row and
+// every eighth four of its values, so that a warp reads 32 rows' neighbours of the partial results.
+template <int D>
+__global__ void __launch_bounds__(256) gaf_attend_join_kernel(const __grid_constant__ Params p) {
+    constexpr int kPart = kWideRows * (D + 2);
+    const Cut &cut = p.cuts[blockIdx.x];
+    const uint32_t parts = cut.parts;
+    if (parts == 0u) return;
+    const Item item = cut.item;
+    const uint32_t r = blockIdx.y * 32u + (threadIdx.x & 31u);
+    if (item.row0 + r >= item.rows) return;
+    auto part_of = [&](uint32_t c) { return p.partials + static_cast<uint64_t>(2u * (blockIdx.x + c) + (c == 0u ? 1u : 0u)) * kPart; };
+    float top = kNoMax, sum = 0.0f;
+    for (uint32_t c = 0; c < parts; ++c) top = fmaxf(top, part_of(c)[kWideRows * D + r]);
+    for (uint32_t c = 0; c < parts; ++c) {
+        const float mc = part_of(c)[kWideRows * D + r];
+        sum += part_of(c)[kWideRows * (D + 1) + r] * (mc == top ? 1.0f : exp2_approx(mc - top));
+    }
+    float4 v[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t c = 0; c < parts; ++c) {
+        const float *src = part_of(c);
+        const float mc = src[kWideRows * D + r];
+        const float wc = mc == top ? 1.0f : exp2_approx(mc - top);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const float4 x = *reinterpret_cast<const float4 *>(src + (static_cast<uint64_t>((threadIdx.x >> 5) + 8u * i) * kWideRows + r) * 4u);
+            v[i] = make_float4(fmaf(x.x, wc, v[i].x), fmaf(x.y, wc, v[i].y), fmaf(x.z, wc, v[i].z), fmaf(x.w, wc, v[i].w));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) finish_row<D, false>(p, item, cut.head, r, ((threadIdx.x >> 5) + 8u * i) * 4u, top, sum, v[i]);
+}
+
 template <int D, int BITS, int GROUP>
 cudaError_t launch_wide(const Params &p, const CUtensorMap &tmap, int sm_count, cudaStream_t stream) {
     using W = Wide<D, BITS, GROUP>;
@@ -687,6 +693,7 @@ cudaError_t launch_wide(const Params &p, const CUtensorMap &tmap, int sm_count, 
     const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W::SMEM); });
     if (e != cudaSuccess) return e;
     kernel<<<sm_count, kWideThreads, W::SMEM, stream>>>(p, tmap);
+    gaf_attend_join_kernel<D><<<dim3(sm_count, kWideRows / 32), 256, 0, stream>>>(p);
     return cudaGetLastError();
 }
 

@@ -431,7 +431,11 @@ cudaError_t attention_generic(const AttnArgs &a, bool f32, cudaStream_t stream) 
 constexpr uint64_t kNarrowRows = 32;
 
 bool attention_fast(const KvView &kv) { return kv.head_dim == 64u || kv.head_dim == 128u; }
-size_t attention_ticket_count(int sm_count) { return static_cast<size_t>(sm_count) * attend::kMaxCtas; }
+// the tickets of the narrow kernel, then the cuts of the wide one
+size_t attention_ticket_count(int sm_count) {
+    static_assert(sizeof(attend::Cut) % sizeof(unsigned int) == 0 && attend::kMaxCtas % 2 == 0, "the cuts are 8-byte aligned");
+    return static_cast<size_t>(sm_count) * (attend::kMaxCtas + sizeof(attend::Cut) / sizeof(unsigned int));
+}
 size_t attention_partial_bytes(int sm_count) {
     return static_cast<size_t>(sm_count) * attend::kMaxPartRows * (attend::kMaxDim + 2) * sizeof(float);
 }
@@ -448,6 +452,7 @@ cudaError_t attention(const AttnArgs &a, const CUtensorMap &tmap, const AttnWork
     p.per_kv = a.q_heads / a.kv.kv_heads;
     p.partials = ws.partials;
     p.tickets = ws.tickets;
+    p.cuts = reinterpret_cast<attend::Cut *>(ws.tickets + static_cast<size_t>(sm_count) * attend::kMaxCtas);
     p.prefix_o = ws.prefix;
     p.prefix_lse = ws.prefix ? ws.prefix + static_cast<uint64_t>(a.seqs.total) * a.q_heads * a.kv.head_dim : nullptr;
     p.o_vec = reinterpret_cast<uintptr_t>(a.out) % (f32 ? 16u : 8u) == 0u && a.os.token % 4u == 0u && a.os.head % 4u == 0u;
