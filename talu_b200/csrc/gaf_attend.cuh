@@ -21,8 +21,10 @@
 //
 // What bounds it: the cache is read once (HBM), and every code is unpacked once (2 to 3 instructions per pair).  A unit is 64
 // keys of one (head, sequence, row tile): codes by TMA (swizzled, so that the fragment reads below hit every bank once),
-// scales and biases by bulk copies into the same ring stage.  A consumer warp owns 16 keys of every unit, or (8 rows) 32 keys of
-// every other unit, for both products, with its own reference and sum: no barrier between warps but at the end of a segment.  The units of
+// scales and biases by bulk copies into the same ring stage.  Each of the four consumer warps owns 16 keys of the unit for
+// both products, with its own reference and sum: no barrier between warps but at the end of a segment.  (32 keys a warp and
+// units in turns: 85 against 78 us for 64 sequences of 2048 to 4096 tokens, 32 heads on 8, 8 bits: the code grows, and what is
+// executed once a segment comes from far.)  The units of
 // all items are cut into equal contiguous ranges over a grid that fills the GPU once, whatever the lengths are; an item cut
 // across CTAs is joined by the last CTA to finish, in CTA order (the result does not depend on timing).
 #pragma once
@@ -253,6 +255,10 @@ __device__ __forceinline__ Item next_item(const Params &p, uint32_t &head, uint3
     return item;
 }
 
+// 64-bit quotients of numbers that hardly ever need 64 bits (a division in them costs some 150 clocks).
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) {
+    return ((a | b) >> 32) == 0u ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
+}
 // The CTA's share of all units: equal contiguous ranges, in the order cached head, element, unit.  A sum over the elements
 // that every CTA forms alike; false: nothing to do.
 struct Range {
@@ -284,9 +290,10 @@ __device__ __forceinline__ bool cta_range(const Params &p, uint32_t *s_scan, uin
     if (out.units == 0) return false;
     out.ctas = out.units < gridDim.x ? out.units : gridDim.x;
     if (blockIdx.x >= out.ctas) return false;
-    out.u0 = out.units * blockIdx.x / out.ctas;
-    out.u1 = out.units * (blockIdx.x + 1u) / out.ctas;
-    const uint32_t start = static_cast<uint32_t>(out.u0 % per_head);
+    out.u0 = quotient(out.units * blockIdx.x, out.ctas);
+    out.u1 = quotient(out.units * (blockIdx.x + 1u), out.ctas);
+    const uint32_t first_head = static_cast<uint32_t>(quotient(out.u0, per_head));
+    const uint32_t start = static_cast<uint32_t>(out.u0 - static_cast<uint64_t>(first_head) * per_head);
     if (start >= pre && start < pre + mine) {
         uint32_t n = n_lo, at = pre;
         for (;; ++n) {
@@ -294,7 +301,7 @@ __device__ __forceinline__ bool cta_range(const Params &p, uint32_t *s_scan, uin
             if (start < at + t) break;
             at += t;
         }
-        s_begin[0] = static_cast<uint32_t>(out.u0 / per_head);
+        s_begin[0] = first_head;
         s_begin[1] = n;
         s_begin[2] = start - at;
     }
@@ -355,8 +362,6 @@ struct Shape {
     static constexpr int HALVES = NT >= 2 && NP >= 2 ? 2 : 1;   // the warps' sums are joined D / HALVES values at a time
     static constexpr int OW = D / HALVES + 4;              // pitch of a joined row (floats)
     static constexpr int JOIN = kConsumers * R * OW * 4;
-    static constexpr int H = NT == 1 && LIMBS == 1 ? 2 : 1;    // 16-key tiles of a warp in a unit
-    static constexpr int TURNS = H;                        // units among which the warps take turns
     static constexpr int CTAS = NT >= 2 ? 2 : 3;           // per SM
     static constexpr int FIXED = QF + JOIN + 1024;
     static constexpr int FIT = (226 * 1024 / CTAS - 2048 - FIXED) / STAGE;
@@ -557,12 +562,10 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
 
     // ---------------- consumers ----------------
     const uint32_t g = lane >> 2, t = lane & 3;
-    constexpr int H = S::H;
-    const uint32_t turn = S::TURNS == 1 ? 0u : static_cast<uint32_t>(warp) >> 1;         // units it % TURNS == turn are this warp's
-    const uint32_t wrow = (S::TURNS == 1 ? warp : (warp & 1)) * (16 * H);              // its first key of a unit
+    const uint32_t wrow = warp * 16u;                             // this warp's first key of a unit
     constexpr int kPiece = PG / 4 * BITS / 8, vPiece = PG / 8 * BITS / 8;   // bytes of a row that a lane reads per step
-    const uint32_t ra = wrow + key_row<RB>(g);                    // this lane's rows in the score product: ra, ra + 8 (+ 16)
-    // offsets in a stage; rows 8 and 16 further on lie 8 and 16 row lengths further on under every swizzle
+    const uint32_t ra = wrow + key_row<RB>(g);                    // this lane's rows in the score product: ra, ra + 8
+    // offsets in a stage; a row 8 further on lies 8 row lengths further on under every swizzle
     uint32_t k_off[NP], v_off[NP][2];
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
@@ -676,12 +679,11 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
         // One unit.  kBorder: some row of the tile does not see all its keys, or some of its keys are in no page.
         auto unit = [&](auto border_tag, uint32_t kc, int32_t key0, uint32_t bad) {
             constexpr bool kBorder = decltype(border_tag)::value;
-            // ---- scores, transposed: [16 H keys][8 NT rows] ----
-            float s[H][NT][4];
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
+            // ---- scores, transposed: [16 keys][8 NT rows] ----
+            float s[NT][4];
+            {
                 float sa[GS], sb[GS], ba[GS], bb[GS];
-                const uint32_t at = kc + s_off + h * (16 * GS * 2);
+                const uint32_t at = kc + s_off;
                 row_f32<GS>(at, sa);
                 row_f32<GS>(at + 8 * GS * 2, sb);
                 row_f32<GS>(at + S::SB, ba);
@@ -690,8 +692,8 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                 for (int j = 0; j < NP; ++j) {
                     constexpr int kWords = kPiece >= 4 ? kPiece / 4 : 1;
                     uint32_t wa[kWords], wb[kWords];
-                    lds<kPiece>(kc + k_off[j] + h * (16 * RB), wa);
-                    lds<kPiece>(kc + k_off[j] + h * (16 * RB) + 8 * RB, wb);
+                    lds<kPiece>(kc + k_off[j], wa);
+                    lds<kPiece>(kc + k_off[j] + 8 * RB, wb);
                     float acc[NT][4];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
@@ -719,114 +721,93 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            s[h][nt][c] = j == 0 ? sa[0] * acc[nt][c] : fmaf(sa[j / kPer], acc[nt][c], s[h][nt][c]);
-                            s[h][nt][2 + c] = j == 0 ? sb[0] * acc[nt][2 + c] : fmaf(sb[j / kPer], acc[nt][2 + c], s[h][nt][2 + c]);
-                            s[h][nt][c] = fmaf(ba[j / kPer], qsum[nt][c][j], s[h][nt][c]);
-                            s[h][nt][2 + c] = fmaf(bb[j / kPer], qsum[nt][c][j], s[h][nt][2 + c]);
+                            s[nt][c] = j == 0 ? sa[0] * acc[nt][c] : fmaf(sa[j / kPer], acc[nt][c], s[nt][c]);
+                            s[nt][2 + c] = j == 0 ? sb[0] * acc[nt][2 + c] : fmaf(sb[j / kPer], acc[nt][2 + c], s[nt][2 + c]);
+                            s[nt][c] = fmaf(ba[j / kPer], qsum[nt][c][j], s[nt][c]);
+                            s[nt][2 + c] = fmaf(bb[j / kPer], qsum[nt][c][j], s[nt][2 + c]);
                         }
                 }
                 if (kBorder) {
-                    const int32_t pa = key0 + static_cast<int32_t>(ra) + 16 * h, pb = pa + 8;
-                    const bool gone = (bad >> (wrow / 16 + h)) & 1u;
+                    const int32_t pa = key0 + static_cast<int32_t>(ra), pb = pa + 8;
+                    const bool gone = (bad >> warp) & 1u;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
                             const int32_t seen = gone ? 0 : s_seen[nt * 8 + 2 * t + c];
-                            if (pa >= seen) s[h][nt][c] = s_hidden;
-                            if (pb >= seen) s[h][nt][2 + c] = s_hidden;
+                            if (pa >= seen) s[nt][c] = s_hidden;
+                            if (pb >= seen) s[nt][2 + c] = s_hidden;
                         }
                 }
             }
             // ---- weights: against the row's reference; it follows lazily ----
-            float va[H][GS], vb[H][GS], ea[H], eb[H];     // scales of the values and the exponents that they lend the weights
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
-                const uint32_t at = kc + s_off + 2 * S::SB + h * (16 * GS * 2);
-                row_f32<GS>(at, va[h]);
-                row_f32<GS>(at + 8 * GS * 2, vb[h]);
-                ea[h] = key_exponent<GS>(va[h]);
-                eb[h] = key_exponent<GS>(vb[h]);
-            }
+            float va[GS], vb[GS];     // scales of the values, and the exponents that they lend the weights
+            row_f32<GS>(kc + s_off + 2 * S::SB, va);
+            row_f32<GS>(kc + s_off + 2 * S::SB + 8 * GS * 2, vb);
+            const float ea = key_exponent<GS>(va), eb = key_exponent<GS>(vb);
             bool grow = false;
-            float z[H][NT][4];
-#pragma unroll
-            for (int h = 0; h < H; ++h)
+            float z[NT][4];
+            auto weigh = [&]() {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        z[h][nt][c] = fmaf(s[h][nt][c], f[nt][c & 1], -m[nt][c & 1]);
-                        if (kBorder && s[h][nt][c] == s_hidden) z[h][nt][c] = -INFINITY;
-                        grow |= z[h][nt][c] + (c < 2 ? ea[h] : eb[h]) > kTarget + kLazy;
-                    }
+                    for (int c = 0; c < 4; ++c)
+                        z[nt][c] = kBorder && s[nt][c] == s_hidden ? -INFINITY : fmaf(s[nt][c], f[nt][c & 1], -m[nt][c & 1]);
+            };
+            weigh();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) grow |= z[nt][c] + (c < 2 ? ea : eb) > kTarget + kLazy;
             if (__any_sync(0xFFFFFFFFu, grow)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        float top = -INFINITY;
-#pragma unroll
-                        for (int h = 0; h < H; ++h) top = fmaxf(top, fmaxf(z[h][nt][c] + ea[h], z[h][nt][2 + c] + eb[h]));
+                        // largest score and exponent of the row, not of its distance from the present reference, which may be none
+                        const float ya = kBorder && s[nt][c] == s_hidden ? -INFINITY : fmaf(s[nt][c], f[nt][c], ea);
+                        const float yb = kBorder && s[nt][2 + c] == s_hidden ? -INFINITY : fmaf(s[nt][2 + c], f[nt][c], eb);
+                        float top = fmaxf(ya, yb);
 #pragma unroll
                         for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-                        if (m[nt][c] == kNoMax) {      // no reference yet: z is the score's distance from nothing
-                            float y = -INFINITY;
+                        const float next = fmaxf(m[nt][c], top - kTarget);
+                        const float keep = next == m[nt][c] ? 1.0f : exp2_approx(m[nt][c] - next);
+                        m[nt][c] = next;
+                        l[nt][c] *= keep;
 #pragma unroll
-                            for (int h = 0; h < H; ++h) {
-                                const float y0 = kBorder && s[h][nt][c] == s_hidden ? -INFINITY : fmaf(s[h][nt][c], f[nt][c], ea[h]);
-                                const float y1 = kBorder && s[h][nt][2 + c] == s_hidden ? -INFINITY : fmaf(s[h][nt][2 + c], f[nt][c], eb[h]);
-                                y = fmaxf(y, fmaxf(y0, y1));
-                            }
+                        for (int i = 0; i < GS; ++i) bsum[nt][c][i] *= keep;
 #pragma unroll
-                            for (int x = 4; x <= 16; x <<= 1) y = fmaxf(y, __shfl_xor_sync(0xFFFFFFFFu, y, x));
-                            if (y > kNoMax) m[nt][c] = y - kTarget;
-                        } else if (top > kTarget) {
-                            const float keep = exp2_approx(kTarget - top);
-                            m[nt][c] += top - kTarget;
-                            l[nt][c] *= keep;
-#pragma unroll
-                            for (int i = 0; i < GS; ++i) bsum[nt][c][i] *= keep;
-#pragma unroll
-                            for (int i = 0; i < S::KS; ++i) o[i][nt][c] *= keep, o[i][nt][2 + c] *= keep;
-                        }
+                        for (int i = 0; i < S::KS; ++i) o[i][nt][c] *= keep, o[i][nt][2 + c] *= keep;
                     }
-#pragma unroll
-                for (int h = 0; h < H; ++h)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            z[h][nt][c] = kBorder && s[h][nt][c] == s_hidden ? -INFINITY : fmaf(s[h][nt][c], f[nt][c & 1], -m[nt][c & 1]);
+                weigh();
             }
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
+            {
                 // ---- weights times scales as B fragments, weights times biases ----
                 uint32_t pf[LIMBS][GS][NT][2];
                 float ba[GS], bb[GS];
-                const uint32_t at = kc + s_off + 3 * S::SB + h * (16 * GS * 2);
+                const uint32_t at = kc + s_off + 3 * S::SB;
                 row_f32<GS>(at, ba);
                 row_f32<GS>(at + 8 * GS * 2, bb);
 #pragma unroll
                 for (int i = 0; i < GS; ++i) {
-                    ba[i] = fmaf(static_cast<float>(1 << (BITS - 1)), va[h][i], ba[i]);
-                    bb[i] = fmaf(static_cast<float>(1 << (BITS - 1)), vb[h][i], bb[i]);
+                    ba[i] = fmaf(static_cast<float>(1 << (BITS - 1)), va[i], ba[i]);
+                    bb[i] = fmaf(static_cast<float>(1 << (BITS - 1)), vb[i], bb[i]);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float pr[4];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) pr[c] = exp2_approx(z[h][nt][c]);
+                    for (int c = 0; c < 4; ++c) pr[c] = exp2_approx(z[nt][c]);
                     l[nt][0] += pr[0] + pr[2];
                     l[nt][1] += pr[1] + pr[3];
 #pragma unroll
                     for (int i = 0; i < GS; ++i) {
-                        float x[4] = {pr[0] * va[h][i], pr[1] * va[h][i], pr[2] * vb[h][i], pr[3] * vb[h][i]};
+                        float x[4] = {pr[0] * va[i], pr[1] * va[i], pr[2] * vb[i], pr[3] * vb[i]};
                         if (kBorder) {   // rows behind the end may hold anything, NaN too
                             float y[4] = {pr[0] * ba[i], pr[1] * ba[i], pr[2] * bb[i], pr[3] * bb[i]};
 #pragma unroll
                             for (int c = 0; c < 4; ++c)
-                                if (z[h][nt][c] == -INFINITY) x[c] = 0.0f, y[c] = 0.0f;
+                                if (z[nt][c] == -INFINITY) x[c] = 0.0f, y[c] = 0.0f;
                             bsum[nt][0][i] += y[0] + y[2];
                             bsum[nt][1][i] += y[1] + y[3];
                         } else {
@@ -850,10 +831,10 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                 for (int j = 0; j < NP; ++j) {
                     constexpr int kWords = vPiece >= 4 ? vPiece / 4 : 1;
                     uint32_t w[4][kWords];
-                    lds<vPiece>(kc + v_off[j][0] + h * (16 * RB), w[0]);
-                    lds<vPiece>(kc + v_off[j][1] + h * (16 * RB), w[1]);
-                    lds<vPiece>(kc + v_off[j][0] + h * (16 * RB) + 8 * RB, w[2]);
-                    lds<vPiece>(kc + v_off[j][1] + h * (16 * RB) + 8 * RB, w[3]);
+                    lds<vPiece>(kc + v_off[j][0], w[0]);
+                    lds<vPiece>(kc + v_off[j][1], w[1]);
+                    lds<vPiece>(kc + v_off[j][0] + 8 * RB, w[2]);
+                    lds<vPiece>(kc + v_off[j][1] + 8 * RB, w[3]);
 #pragma unroll
                     for (int i = 0; i < PG / 16; ++i) {
                         uint32_t a[4];
@@ -880,13 +861,6 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
         for (uint32_t tile = tile0; tile < tile0 + count; ++tile, ++it) {
             const uint32_t stage = it % S::STAGES;
             if (!mbar_wait(smem_u32(&s_full[stage]), (it / S::STAGES) & 1u, &s_abort, p.a.error_word)) failed = true;
-            if (S::TURNS > 1 && (it % S::TURNS) != turn) {
-                // another pair's unit: every warp follows every fill of a stage and hands it back, or the parity that it waits
-                // for next could be that of an older fill
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&s_empty[stage]));
-                continue;
-            }
             const int32_t key0 = static_cast<int32_t>(tile * kKeys);
             const uint32_t bad = s_bad[stage];
             if (key0 + kKeys <= item.first_seen && bad == 0u) unit(std::false_type(), base + stage * S::STAGE, key0, 0u);

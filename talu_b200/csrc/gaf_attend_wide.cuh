@@ -151,7 +151,8 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
     __shared__ uint32_t s_bad[W::STAGES];           // bit x: keys 16x.. of the unit are in no page
     // by unit and 32 keys: factor of the keys' scores, exponent of the values, 2^-exponent, groups of values that are not finite
     __shared__ float s_kmul[kInfo][4], s_vexp[kInfo][4], s_vinv[kInfo][4];
-    __shared__ uint32_t s_kbad[kInfo], s_lost[kInfo][4];
+    __shared__ uint32_t s_kbad[kInfo];
+    __shared__ __align__(16) uint32_t s_lost[kInfo][4];
     __shared__ uint8_t s_poison[kInfo][kWideKeys];  // by key
     __shared__ uint32_t s_tmem;
     __shared__ volatile uint32_t s_abort;
@@ -580,16 +581,19 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                         }
                         tmem_wait_st();
                     }
-                    wait(s_tile_full[vx % W::TILES], (vx / W::TILES) & 1u);
-                    __syncwarp();
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         uint32_t x[32];
                         tmem_ld32(tm_s + 32u * c, x);
+                        if (c == 0) {
+                            wait(s_tile_full[vx % W::TILES], (vx / W::TILES) & 1u);
+                            __syncwarp();
+                        }
                         tmem_wait_ld();
                         chunk(c, x);
                     }
-                    if (s_lost[info][0] | s_lost[info][1] | s_lost[info][2] | s_lost[info][3]) {
+                    const uint4 lost = *reinterpret_cast<const uint4 *>(s_lost[info]);
+                    if (lost.x | lost.y | lost.z | lost.w) {
                         for (int k = 0; k < kWideKeys; ++k)
                             if (key0 + k < seen && ((s_lost[info][k >> 5] >> (k & 31)) & 1u)) poison |= s_poison[info][k];
                         __syncwarp();
