@@ -177,6 +177,13 @@ __device__ __forceinline__ uint64_t element_of(const KvRows &x, const Place &p, 
     return (first_token + p.token) * token_stride + p.head * head_stride + p.vec * 8u;
 }
 
+// a / b, rounded to nearest, for r = 1 / b rounded to nearest: the product a r and one correction by its exact remainder
+// (Markstein's theorem).  The codes are those of a division, ties included, at two instructions more than a product.
+__device__ __forceinline__ float rounded_quotient(float a, float b, float r) {
+    const float q = a * r;
+    return fmaf(fmaf(-q, b, a), r, q);
+}
+
 // The group's lanes (G / 8 neighbours) share minimum and maximum.
 template <bool F32, bool VEC, bool FIXED>
 __global__ void __launch_bounds__(kThreadsKv) gaf_kv_append_kernel(const KvView kv, const KvSeqs seqs, const KvRows in, uint32_t tokens,
@@ -186,7 +193,7 @@ __global__ void __launch_bounds__(kThreadsKv) gaf_kv_append_kernel(const KvView 
     Walk<FIXED> walk(kv, tokens, s_row);
     const uint64_t first_token = static_cast<uint64_t>(blockIdx.x) * tokens;
     const uint32_t steps = (tokens * walk.per_token + kThreadsKv - 1u) / kThreadsKv;
-    const float maxq = kv.bits == 4u ? 15.0f : 255.0f;
+    const float maxq = kv.bits == 4u ? 15.0f : 255.0f, inv_maxq = __frcp_rn(0.5f * maxq);
     for (uint32_t step = 0; step < steps; step += kUnroll) {
         Place pl[kUnroll];
         float x[kUnroll][8];
@@ -214,7 +221,7 @@ __global__ void __launch_bounds__(kThreadsKv) gaf_kv_append_kernel(const KvView 
                 hi = max_nan(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
             }
             const float range = 0.5f * hi - 0.5f * lo;             // of halves: finite for finite values
-            uint32_t sraw = f32_bf16(__fdiv_rn(range, 0.5f * maxq)), braw = f32_bf16(lo);
+            uint32_t sraw = f32_bf16(rounded_quotient(range, 0.5f * maxq, inv_maxq)), braw = f32_bf16(lo);
             if ((braw & 0x7FFFu) == 0x7F80u) braw -= 1u;           // f32 values beyond the largest bf16
             float s = bf16_f32(sraw);
             if (s < FLT_MIN) s = 0.0f, sraw = 0u;
@@ -224,31 +231,24 @@ __global__ void __launch_bounds__(kThreadsKv) gaf_kv_append_kernel(const KvView 
             const float r = s > 0.0f ? __frcp_rn(half_s) : 0.0f;
             // adding 1.5 * 2^23 rounds to an integer (ties to even) and leaves it in the low bits
             constexpr float kMagic = 12582912.0f;
-            uint32_t q[8];
-            float off = 0.0f;
+            float y[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float c = fminf(fmaxf(fmaf(0.5f, x[k][i], -half_b) * r, 0.0f), maxq);
-                const float y = c + kMagic;
-                off = fmaxf(off, fabsf(c - (y - kMagic)));
-                q[i] = __float_as_uint(y) & 0xFFu;
+                const float c = rounded_quotient(fmaf(0.5f, x[k][i], -half_b), half_s, r);
+                y[i] = fminf(fmaxf(c, 0.0f), maxq) + kMagic;
             }
-            if (off > 0.49996f) {
-                // the product is within 2^-15 (3.1e-5) of the quotient: only next to a tie does the division decide the code
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    q[i] = __float_as_uint(fminf(fmaxf(__fdiv_rn(fmaf(0.5f, x[k][i], -half_b), half_s), 0.0f), maxq) + kMagic) & 0xFFu;
-            }
-            if (!finite) q[0] = q[1] = q[2] = q[3] = q[4] = q[5] = q[6] = q[7] = 0u;
             if (pl[k].row < 0) continue;
             uint8_t *dst = kv.packed + pl[k].row * kv.row_bytes + pl[k].vec * kv.bits;   // 8 codes are `bits` bytes
+            auto bytes = [](float a, float b, float c, float d) {      // the low bytes of four numbers
+                return attend::prmt(attend::prmt(__float_as_uint(a), __float_as_uint(b), 0x0040u), attend::prmt(__float_as_uint(c), __float_as_uint(d), 0x0040u), 0x5410u);
+            };
             if (kv.bits == 8u) {
-                *reinterpret_cast<uint2 *>(dst) = make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
+                *reinterpret_cast<uint2 *>(dst) = make_uint2(bytes(y[0], y[1], y[2], y[3]), bytes(y[4], y[5], y[6], y[7]));
             } else {
-                uint32_t w = 0u;
+                float z[4];       // code + 16 code' + 1.5 * 2^23, exact
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w |= q[i] << (4 * i);
-                *reinterpret_cast<uint32_t *>(dst) = w;
+                for (int i = 0; i < 4; ++i) z[i] = fmaf(y[2 * i + 1] - kMagic, 16.0f, y[2 * i]);
+                *reinterpret_cast<uint32_t *>(dst) = bytes(z[0], z[1], z[2], z[3]);
             }
             if ((pl[k].vec & ((kv.group >> 3) - 1u)) == 0u) {
                 const int64_t g = pl[k].row * kv.groups + (pl[k].vec * 8u >> kv.group_shift);
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kThreadsKv) gaf_kv_read_kernel(const KvView kv
                     x[i] = fmaf(__uint_as_float(attend::prmt(i < 4 ? code[k].x : code[k].y, 0x4B000000u, 0x7650u | (i & 3))) - 8388608.0f, s[k], b[k]);
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = fmaf(static_cast<float>((code[k].x >> (4 * i)) & 15u), s[k], b[k]);
+                for (int i = 0; i < 8; ++i) x[i] = fmaf(__uint_as_float(((code[k].x >> (4 * i)) & 15u) | 0x4B000000u) - 8388608.0f, s[k], b[k]);
             }
             store8<F32, VEC>(const_cast<void *>(tensor_of(out, pl[k])), element_of(out, pl[k], first_token), x);
         }
