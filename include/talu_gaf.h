@@ -279,13 +279,13 @@ int32_t tgaf_embedding_lookup_f32(tgaf_ctx *ctx, const tgaf_weight *w, const uin
  *   biases  u16 [pages][2][kv_heads][page_tokens][head_dim/group]     bf16
  *   value = f32(code) * f32(scale) + f32(bias)                        one rounding (fused multiply-add)
  *
- * The quantiser of a group of values x: bias = bf16(min x), scale = bf16((max x - min x) / (2^bits - 1)), 0 where that is
- * below the smallest normal number, code = clamp(rint((x - bias) / scale), 0, 2^bits - 1), all in f32 with ties to even;
+ * The quantiser of a group of values x: bias = bf16(min x), scale = bf16((max x - min x) * f32(1 / (2^bits - 1))), 0 where
+ * that is below the smallest normal number, code = clamp(rint((x - bias) / scale), 0, 2^bits - 1), all in f32 with ties to even;
  * the codes are taken against the stored (rounded) scale and bias, so a value is off by half a step at most wherever the
  * rounded scale reaches it.  A group that holds an infinity or a NaN reads back as NaN.
  * bits in {4, 8}; group in {32, 64, 128}; head_dim a multiple of group, at most 256; page_tokens in {16, 32, 64, 128, 256};
  * pages * 2 * kv_heads * page_tokens < 2^31.  The three buffers are the caller's device memory (16-byte aligned), are not
- * copied and must outlive the cache; the kernels read nothing of rows that no sequence reaches. */
+ * copied and must outlive the cache; what lies in rows that no sequence reaches never matters. */
 typedef struct tgaf_kv_cache tgaf_kv_cache;
 int32_t tgaf_kv_cache_wrap_device(tgaf_ctx *ctx, void *d_packed, void *d_scales, void *d_biases, uint64_t pages,
                                   uint32_t kv_heads, uint32_t page_tokens, uint32_t head_dim, uint32_t group_size,

@@ -565,7 +565,7 @@ const char *tgaf_status_string(int32_t status) {
         case TGAF_ERR_NCCL: return "NCCL error";
         case TGAF_ERR_UNSUPPORTED: return "unsupported";
         case TGAF_ERR_TIMEOUT: return "timeout";
-        case TGAF_ERR_DEVICE_FLAG: return "device-side wait ran out";
+        case TGAF_ERR_DEVICE_FLAG: return "device-side wait ran out or bad block table";
         default: return "unknown status";
     }
 }

@@ -2,7 +2,7 @@
 // sizes that the tensor-core kernel does not take.
 //
 // A group of G values x along head_dim is stored as codes q, a bf16 scale s and a bf16 bias b:
-//   b = bf16(min x),  s = bf16((max x - min x) / maxq),  q = clamp(rint((x - b) / s), 0, maxq),  value = q s + b
+//   b = bf16(min x),  s = bf16((max x - min x) f32(1 / maxq)),  q = clamp(rint((x - b) / s), 0, maxq),  value = q s + b
 // b is exact for bf16 inputs (the minimum is one of them).  s and b are rounded to nearest once, because 16 bits each is
 // what the format stores; the codes are taken against the rounded pair, which makes the rounding of s part of the grid and
 // not an error of every value: only the top value can be off by more than half a step, (max x - min x) 2^-9 + s / 2.
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kThreadsKv) gaf_kv_append_kernel(const KvView 
                 hi = max_nan(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
             }
             const float range = 0.5f * hi - 0.5f * lo;             // of halves: finite for finite values
-            uint32_t sraw = f32_bf16(rounded_quotient(range, 0.5f * maxq, inv_maxq)), braw = f32_bf16(lo);
+            uint32_t sraw = f32_bf16(range * inv_maxq), braw = f32_bf16(lo);
             if ((braw & 0x7FFFu) == 0x7F80u) braw -= 1u;           // f32 values beyond the largest bf16
             float s = bf16_f32(sraw);
             if (s < FLT_MIN) s = 0.0f, sraw = 0u;

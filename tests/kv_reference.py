@@ -12,7 +12,7 @@ def quantise_f32(x, bits, group):
     g = x.float().cpu().unflatten(-1, (-1, group))
     lo, hi = g.amin(-1), g.amax(-1)
     b = lo.to(torch.bfloat16)
-    s = ((hi * 0.5 - lo * 0.5) / (most * 0.5)).to(torch.bfloat16)
+    s = ((hi * 0.5 - lo * 0.5) * (torch.ones(()) / torch.tensor(most * 0.5))).to(torch.bfloat16)
     s = torch.where(s.float() < torch.finfo(torch.float32).tiny, torch.zeros_like(s), s)
     half = (s.float() * 0.5).unsqueeze(-1)
     q = ((g * 0.5 - b.float().unsqueeze(-1) * 0.5) / torch.where(half > 0, half, 1.0)).round().clamp(0.0, most)

@@ -390,3 +390,282 @@ def test_attention_shared_prefix(ctx, shape, dtype, prefix):
     prefix_table = table[-1, :-(-prefix // page)].contiguous()
     q = torch.randn(cu[-1] + 1, kv_heads * per_kv, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(dtype)
     check_attention(ctx, cache, q, table[:-1], lens, cu, max(news), prefix_table, prefix)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(8, 4, 128, 8, 64, 64), (4, 8, 64, 4, 32, 16), (2, 2, 128, 4, 128, 128)])
+def test_attention_of_prompts_over_long_caches(ctx, shape):
+    """Hundreds of new tokens over a thousand cached ones: row tiles that start inside a token's heads, units and tiles at
+    every kind of border, sequences that leave half of a row tile empty."""
+    kv_heads, per_kv, dim, bits, group, page = shape
+    lens, news = [1500, 64, 333, 1100], [300, 64, 1, 129]
+    table, pages, _ = make_tables(lens, page, 7)
+    cache = filled_cache(ctx, pages, kv_heads, dim, page, bits, group)
+    claim(cache, table, lens)
+    cu = cumulate(news)
+    q = torch.randn(cu[-1], kv_heads * per_kv, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).bfloat16()
+    check_attention(ctx, cache, q, table, lens, cu, max(news))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("k_size, v_size, q_size, scale", [(1e-12, 1e-9, 1.0, 1e11), (1e30, 1e30, 1e-30, 0.1), (1.0, 1e20, 0.0, 1.0), (1.0, 1.0, 30.0, 1.0),
+                                                         (1.0, 1.0, 1.0, -0.3), (1.0, 1.0, 1.0, 0.0), (30.0, 1e-6, 3e4, 1e-4)])
+def test_attention_of_large_and_small_values(ctx, dtype, new, k_size, v_size, q_size, scale):
+    """Values of any size that f32 sums hold, scores in the hundreds, scale of either sign or zero, q of zeros."""
+    lens, news = [150, 700], [new, new]
+    table, pages, _ = make_tables(lens, 32, 7)
+    cache = filled_cache(ctx, pages, 2, 128, 32, 8, 64)
+    claim(cache, table, lens)
+    for t in (cache.scales, cache.biases):
+        t[:, 0] *= k_size
+        t[:, 1] *= v_size
+    q = (torch.randn(2 * new, 8, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) * q_size).to(dtype)
+    out = torch.empty_like(q)
+    import talu_b200 as gaf
+    gaf.attention(ctx, cache, q, table, dev(lens), cu=dev(cumulate(news)), max_new=new, scale=scale, out=out)
+    ctx.synchronize()
+    want, mass = ref.attention(cache, q, table, lens, cumulate(news), scale=scale)
+    # a score y is a sum of 128 products: off by 128 2^-24 of their absolute sum in f32, and by 2^-12 sqrt(128) of a product's
+    # size where keys are rounded to f16; it changes its weight, and with it the result, by that share
+    k = torch.cat([ref.values(cache, table[b], lens[b], 0)[0].abs() for b in range(2)], 1)
+    size = abs(scale) * q.double().abs().amax() * k.amax()
+    share = size.item() * (2.0 ** -12 * 12 if dtype == torch.bfloat16 else 2.0 ** -17)
+    tol = mass * (2.0 ** -8 * 3 + 2 * share if dtype == torch.bfloat16 else 2.0 ** -15 + 2 * share) + 2.0 ** -8 * want.abs() * (dtype == torch.bfloat16)
+    assert ((out.double() - want).abs() <= tol + 1e-30).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("per_kv, new", [(1, 5), (4, 5), (4, 60)])
+def test_values_that_are_not_finite(ctx, dtype, per_kv, new):
+    """A NaN group of a key makes every row that sees the key NaN, one of a value only its group's part; rows that do not see
+    it, behind a causal border or in another sequence, are untouched."""
+    import talu_b200 as gaf
+    lens, news, group = [90, 200], [new, new], 32
+    table, pages, _ = make_tables(lens, 16, 7)
+    cache = filled_cache(ctx, pages, 2, 128, 16, 8, group)
+    claim(cache, table, lens)
+    q = torch.randn(2 * new, 2 * per_kv, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(dtype)
+    run = lambda: gaf.attention(ctx, cache, q, table, dev(lens), cu=dev([0, new, 2 * new]), max_new=new)  # noqa: E731
+    clean = run()
+    at = lens[1] - 3                                            # seen by the last three tokens of the second sequence
+    page, row = int(table[1, at // 16]), at % 16
+    saved = cache.scales[page, 1, 1, row, 2].clone()
+    cache.scales[page, 1, 1, row, 2] = float("nan")             # V, head 1, values 64..95
+    bad_v = run()
+    cache.scales[page, 1, 1, row, 2] = saved
+    cache.biases[page, 0, 0, row, 0] = float("nan")             # K, head 0
+    bad_k = run()
+    ctx.synchronize()
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    hit[2 * new - 3:, per_kv:, 64:96] = True
+    assert torch.equal(bad_v.isnan(), hit) and torch.equal(bad_v[~hit], clean[~hit])
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    hit[2 * new - 3:, :per_kv] = True
+    assert torch.equal(bad_k.isnan(), hit) and torch.equal(bad_k[~hit], clean[~hit])
+
+
+@gpu
+@pytest.mark.parametrize("new, per_kv", [(1, 4), (5, 4), (90, 4)])
+def test_captured_calls_follow_their_tables(ctx, new, per_kv):
+    """Append and attention captured once; lengths, tables and rows change between replays.  Equal inputs give equal bits."""
+    import talu_b200 as gaf
+    own = gaf.Context(0, own_stream=True)
+    stream = torch.cuda.Stream()
+    own.set_stream(stream.cuda_stream)
+    batch, kv_heads, dim, page = 3, 2, 128, 32
+    cache = gaf.KvCache.allocate(own, 200, kv_heads, dim, page, 8, 64)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    table = torch.arange(150, device="cuda").view(3, 50).int()
+    lens, cu = dev([new] * 3), dev([new * i for i in range(4)])
+    qkv = torch.randn(batch * new, (per_kv + 2) * kv_heads, dim, device="cuda", generator=gen).bfloat16()
+    q, k, v = qkv.split([per_kv * kv_heads, kv_heads, kv_heads], 1)
+    out = torch.zeros(batch * new, per_kv * kv_heads, dim, device="cuda", dtype=torch.bfloat16)
+
+    def step():
+        gaf.kv_append(own, cache, k, v, table, lens, cu=cu)
+        gaf.attention(own, cache, q, table, lens, cu=cu, max_new=new, out=out)
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        step()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+    for turn in range(5):
+        qkv.copy_(torch.randn(qkv.shape, device="cuda", generator=gen))
+        lens.copy_(dev([new * (turn + 1)] * 3))
+        if turn == 3:                                           # the pages move
+            old = table.clone()
+            table.copy_(199 - table)
+            for t in (cache.packed, cache.scales, cache.biases):
+                t[table.long().flatten()] = t[old.long().flatten()].clone()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        first = out.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(first, out)
+        n = [new * (turn + 1)] * 3
+        want, mass = ref.attention(cache, q, table, n, [new * i for i in range(4)])
+        assert ((out.double() - want).abs() <= 2.0 ** -8 * (3 * mass + want.abs()) + 1e-7).all()
+    own.synchronize()
+    del graph
+    cache.free()
+    own.close()
+
+
+@gpu
+def test_two_contexts_at_once():
+    """Each context has its own workspace: calls of two contexts on two streams may overlap."""
+    import talu_b200 as gaf
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctxs = [gaf.Context(0, stream=s.cuda_stream) for s in streams]
+    jobs = []
+    for i, c in enumerate(ctxs):
+        lens = [3000 + 100 * i, 40, 900]
+        table, pages, _ = make_tables(lens, 64, i)
+        cache = filled_cache(c, pages, 2, 128, 64, 8, 64, seed=i)
+        claim(cache, table, lens, seed=i)
+        q = torch.randn(3, 8, 128, device="cuda").bfloat16()
+        jobs.append((c, cache, q, table, dev(lens), lens))
+    torch.cuda.synchronize()
+    outs = [[gaf.attention(c, cache, q, table, lens) for _ in range(20)] for c, cache, q, table, lens, _ in jobs]
+    torch.cuda.synchronize()
+    for (c, cache, q, table, _, lens), many in zip(jobs, outs):
+        want, mass = ref.attention(cache, q, table, lens, [0, 1, 2, 3])
+        for out in many:
+            assert torch.equal(out, many[0])
+        assert ((many[0].double() - want).abs() <= 2.0 ** -8 * (3 * mass + want.abs()) + 1e-7).all()
+        c.synchronize()
+        cache.free()
+        c.close()
+
+
+@gpu
+def test_prefix_is_the_head_of_every_sequence(ctx):
+    """A prefix that ends with a page gives what tables that begin with its pages give, up to the roundings of the weights."""
+    import talu_b200 as gaf
+    lens, page, prefix = [70, 3, 129, 64], 32, 320
+    table, pages, _ = make_tables(lens + [prefix], page, 1)
+    cache = filled_cache(ctx, pages, 2, 128, page, 8, 64)
+    claim(cache, table, lens + [prefix])
+    head = table[-1, :prefix // page].contiguous()
+    q = torch.randn(4, 16, 128, device="cuda").bfloat16()
+    a = gaf.attention_shared_prefix(ctx, cache, q, head, prefix, table[:-1], dev(lens))
+    whole = torch.cat((head.expand(4, -1), table[:-1, :5]), 1).contiguous()
+    b = gaf.attention(ctx, cache, q, whole, dev([n + prefix for n in lens]))
+    none = gaf.attention_shared_prefix(ctx, cache, q, head, 0, table[:-1], dev(lens))
+    plain = gaf.attention(ctx, cache, q, table[:-1], dev(lens))
+    ctx.synchronize()
+    assert (a.float() - b.float()).norm() <= 2.0 ** -8 * b.float().norm()
+    assert torch.equal(none, plain)
+
+
+@gpu
+@pytest.mark.parametrize("new", [2, 50])
+def test_more_new_tokens_than_announced(ctx, new):
+    """A sequence with more than max_new own tokens: reported, its rows from max_new on left as they were."""
+    import talu_b200 as gaf
+    lens = [100, 80]
+    table, pages, _ = make_tables(lens, 16, 1)
+    cache = filled_cache(ctx, pages, 2, 64, 16, 8, 64)
+    claim(cache, table, lens)
+    q = torch.randn(2 * new, 8, 64, device="cuda").bfloat16()
+    out = torch.full_like(q, 7.0)
+    gaf.attention(ctx, cache, q, table, dev(lens), cu=dev([0, new - 1, 2 * new]), max_new=new - 1, out=out)
+    with pytest.raises(gaf.GafError) as e:
+        ctx.synchronize()
+    assert e.value.status == 7 and "max_new" in e.value.message
+    assert (out[2 * new - 2:] == 7.0).all() and (out[:2 * new - 2] != 7.0).any(-1).all()
+    assert gaf.attention(ctx, cache, q[:0], table, dev(lens), cu=dev([0, 0, 0]), max_new=1).shape == (0, 8, 64)
+    gaf.kv_append(ctx, cache, q[:0, :2], q[:0, :2], table, dev(lens), cu=dev([0, 0, 0]))
+    ctx.synchronize()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new, offset", [(1, 0), (1, 1), (30, 0), (30, 1)])
+def test_attention_with_any_strides(ctx, dtype, new, offset):
+    """Queries and results with odd pitches, heads in front of tokens, and bases that are not 16-byte aligned."""
+    import talu_b200 as gaf
+    lens = [100, 80]
+    table, pages, _ = make_tables(lens, 16, 1)
+    wide = torch.full((2, pages + 5), -1, dtype=torch.int32, device="cuda")      # a table with a pitch of its own
+    wide[:, :table.shape[1]] = table
+    cache = filled_cache(ctx, pages, 2, 128, 16, 8, 64)
+    claim(cache, table, lens)
+    raw = torch.randn(8, 2 * new, 128 + 2 * offset + 1, device="cuda").to(dtype)
+    q = raw[:, :, offset:offset + 128].transpose(0, 1)
+    buf = torch.full((8, 2 * new, 131 + offset), 7.0, device="cuda", dtype=dtype)
+    out = buf[:, :, offset:offset + 128].transpose(0, 1)
+    gaf.attention(ctx, cache, q, wide[:, :table.shape[1]], dev(lens), out=out)
+    dense = gaf.attention(ctx, cache, q.contiguous(), table, dev(lens))
+    ctx.synchronize()
+    assert torch.equal(out, dense)
+    assert (buf[:, :, :offset] == 7.0).all() and (buf[:, :, offset + 128:] == 7.0).all()
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 64])
+def test_pages_beyond_four_gigabytes(ctx, new):
+    """Offsets of codes and of scales that do not fit 32 bits."""
+    import talu_b200 as gaf
+    kv_heads, dim, page = 8, 128, 64
+    pages = (2 ** 32 // (2 * kv_heads * page * dim) + 1) * 2 + 8            # codes: over 8 GB; the last pages are used
+    free, _ = torch.cuda.mem_get_info()
+    if free < 12 * 2 ** 30:
+        pytest.skip("not enough device memory")
+    cache = gaf.KvCache.allocate(ctx, pages, kv_heads, dim, page, 8, 32)
+    lens = [200, 130]
+    table = dev([[pages - 1, 5, pages - 3, pages - 8], [pages - 2, pages // 2 + 1, pages - 4, 0]])
+    q = torch.randn(2 * new, 32, dim, device="cuda").bfloat16()
+    for b, n in enumerate(lens):
+        kv = torch.randn(2, n, kv_heads, dim, device="cuda").bfloat16()
+        gaf.kv_append(ctx, cache, kv[0], kv[1], table[b:b + 1], dev([n]))
+        got = gaf.kv_read(ctx, cache, table[b:b + 1], dev([n]), total=n)
+        step = (kv.float().amax(-1) - kv.float().amin(-1)).amax() / 255
+        assert (got[0].float() - kv[0].float()).abs().amax() <= 1.1 * step + 2.0 ** -8 * 6
+        assert (got[1].float() - kv[1].float()).abs().amax() <= 1.1 * step + 2.0 ** -8 * 6
+    check_attention(ctx, cache, q, table, lens, [0, new, 2 * new], new)
+    cache.free()
+
+
+@gpu
+def test_decoder_layer_from_linears_and_cache(ctx, oracle):
+    """qkv linear, append, attention and o linear as a decoder runs them: a prompt of two sequences, then single tokens, against
+    the same layer in 64 bits on the dequantised weights and the cache's values."""
+    import talu_b200 as gaf
+    from helpers import make_weights
+    heads, kv_heads, dim, hidden = 8, 2, 64, 512
+    parts = {}
+    for i, (name, n, k) in enumerate((("qkv", (heads + 2 * kv_heads) * dim, hidden), ("o", hidden, heads * dim))):
+        packed, scales, biases = make_weights(oracle, n, k, 64, 4, seed=i)
+        parts[name] = gaf.Weight.from_host(ctx, packed, scales, biases, 64, 4)
+    cache = gaf.KvCache.allocate(ctx, 12, kv_heads, dim, 32, 8, 64)
+    table = dev([[3, 7, 1, 0], [2, 9, 11, 4]])
+    lens, gen = [0, 0], torch.Generator(device="cuda").manual_seed(1)
+    for news in ([70, 33], [1, 1], [1, 1]):
+        lens = [a + b for a, b in zip(lens, news)]
+        cu = cumulate(news)
+        x = torch.randn(cu[-1], hidden, device="cuda", generator=gen).bfloat16()
+        qkv = gaf.linear(ctx, parts["qkv"], x).unflatten(1, (-1, dim))
+        q, k, v = qkv.split([heads, kv_heads, kv_heads], 1)
+        gaf.kv_append(ctx, cache, k, v, table, dev(lens), cu=dev(cu))
+        a = gaf.attention(ctx, cache, q, table, dev(lens), cu=dev(cu), max_new=max(news))
+        y = gaf.linear(ctx, parts["o"], a.flatten(1))
+        ctx.synchronize()
+        want, mass = ref.attention(cache, q, table, lens, cu)
+        assert ((a.double() - want).abs() <= 2.0 ** -8 * (3 * mass + want.abs()) + 1e-7).all()
+        w = gaf.dequant_f32(ctx, parts["o"]).double()
+        exact = a.double().flatten(1) @ w.T
+        assert (y.double() - exact).norm() <= 1e-2 * exact.norm()
+        k_back, _ = gaf.kv_read(ctx, cache, table, dev(lens), cu=dev(cu), total=cu[-1])
+        ctx.synchronize()
+        assert (k_back.float() - k.float()).norm() <= 2.0 ** -6 * k.float().norm()   # half a 1/255 step of a range of some six sigma
+    for w in parts.values():
+        w.free()
