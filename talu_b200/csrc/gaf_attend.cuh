@@ -467,6 +467,7 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
     __shared__ int32_t s_seen[R];
     __shared__ float s_ml[kConsumers][R][2];
     __shared__ uint32_t s_last;
+    __shared__ Item s_item;
 
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *const base_ptr = smem_raw + (base - smem_u32(smem_raw));
@@ -578,33 +579,60 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
     const float s_hidden = __uint_as_float(0xFF800000u);      // score of a key that a row does not see
     uint32_t it = 0;
     bool failed = false;
+    // A warp's rows of q as they lie in memory.  Those of the next segment are fetched before the present one's units are worked
+    // on: finding the item and waiting for its rows took a segment's start 1 to 2 us.
+    constexpr int PL = D / 32, kRows = R / kConsumers, kRaw = LIMBS == 2 ? PL : PL / 2;
+    uint32_t raw[kRows][kRaw];
+    auto fetch_q = [&](const Item &item) {
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+            const uint32_t row = item.row0 + warp + j * kConsumers;
+#pragma unroll
+            for (int i = 0; i < kRaw; ++i) raw[j][i] = 0u;
+            if (row >= item.rows) continue;
+            const uint32_t token = row / p.per_kv;
+            const uint64_t at = static_cast<uint64_t>(item.token0 + token) * p.a.qs.token +
+                                static_cast<uint64_t>(head * p.per_kv + row - token * p.per_kv) * p.a.qs.head + lane * PL;
+            if (LIMBS == 2) {
+                const uint32_t *src = static_cast<const uint32_t *>(p.a.q) + at;
+#pragma unroll
+                for (int i = 0; i < kRaw; ++i) raw[j][i] = src[i];
+            } else {
+                const uint16_t *src = static_cast<const uint16_t *>(p.a.q) + at;
+                if (p.q_vec && kRaw == 2) {
+                    const uint2 y = *reinterpret_cast<const uint2 *>(src);
+                    raw[j][0] = y.x, raw[j][kRaw - 1] = y.y;
+                } else if (p.q_vec) {
+                    raw[j][0] = *reinterpret_cast<const uint32_t *>(src);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kRaw; ++i) raw[j][i] = src[2 * i] | (static_cast<uint32_t>(src[2 * i + 1]) << 16);
+                }
+            }
+        }
+    };
+    {
+        const Item first = next_item<R, kKeys>(p, head, elem);
+        if (threadIdx.x == 0) s_item = first;
+        fetch_q(first);
+        bar_consumers();
+    }
     for (uint64_t u = u0; u < u1;) {
-        const Item item = next_item<R, kKeys>(p, head, elem);
+        const Item item = s_item;
         const uint32_t left = item.tiles - tile0;
         const uint32_t count = u1 - u < left ? static_cast<uint32_t>(u1 - u) : left;
 
         // ---- q of the tile's rows: scaled by a power of two, f16, as B fragments; sums per step; scale of the scores ----
-        for (int r = warp; r < R; r += kConsumers) {
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+            const int r = warp + j * kConsumers;
             const uint32_t row = item.row0 + r;
             const bool have = row < item.rows;
-            constexpr int PL = D / 32;
             float x[PL];
-            if (have) {
-                const uint64_t at = static_cast<uint64_t>(item.token0 + row / p.per_kv) * p.a.qs.token +
-                                    static_cast<uint64_t>(head * p.per_kv + row % p.per_kv) * p.a.qs.head + lane * PL;
-                if (LIMBS == 2) {
-                    const float *src = static_cast<const float *>(p.a.q) + at;
 #pragma unroll
-                    for (int i = 0; i < PL; ++i) x[i] = src[i];
-                } else {
-                    const uint16_t *src = static_cast<const uint16_t *>(p.a.q) + at;
-#pragma unroll
-                    for (int i = 0; i < PL; ++i) x[i] = bf16_f32(src[i]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < PL; ++i) x[i] = 0.0f;
-            }
+            for (int i = 0; i < PL; ++i)
+                x[i] = LIMBS == 2 ? __uint_as_float(raw[j][LIMBS == 2 ? i : 0])
+                                  : (i & 1) ? __uint_as_float(raw[j][LIMBS == 2 ? 0 : i / 2] & 0xFFFF0000u) : bf16_f32(raw[j][LIMBS == 2 ? 0 : i / 2]);
             float top = 0.0f;
 #pragma unroll
             for (int i = 0; i < PL; ++i) top = fmaxf(top, fabsf(x[i]));
@@ -640,6 +668,14 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
             }
         }
         bar_consumers();
+        // where this segment lies is kept, and the next one's rows are sent for
+        const uint32_t this_head = head;
+        if (u + count < u1) {
+            if (++elem == p.elements) elem = 0, ++head;
+            const Item next = next_item<R, kKeys>(p, head, elem);
+            if (threadIdx.x == 0) s_item = next;       // read again behind the barriers of the segment's end
+            fetch_q(next);
+        }
         uint32_t qreg[kQReg ? LIMBS : 1][kQReg ? NT : 1][kQReg ? S::KS : 1][2];
         if (kQReg) {
 #pragma unroll
@@ -937,7 +973,7 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                 float top, sum;
                 row_sum(r, top, sum);
                 if (whole) {
-                    finish_row<D, LIMBS == 2>(p, item, head, r, half * kWide + d, top, sum, v);
+                    finish_row<D, LIMBS == 2>(p, item, this_head, r, half * kWide + d, top, sum, v);
                 } else {
                     __stcg(reinterpret_cast<float4 *>(part + r * D + half * kWide + d), v);
                     if (half == 0 && d == 0) {
@@ -950,11 +986,11 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
         if (!whole) {
             // the item's CTAs: the first holds its unit 0
             const uint64_t first_unit = u - tile0;
-            const uint32_t c0 = static_cast<uint32_t>(((first_unit + 1) * ctas - 1) / units);
-            const uint32_t c1 = static_cast<uint32_t>(((first_unit + item.tiles) * ctas - 1) / units);
-            __threadfence();
+            const uint32_t c0 = static_cast<uint32_t>(quotient((first_unit + 1) * ctas - 1, units));
+            const uint32_t c1 = static_cast<uint32_t>(quotient((first_unit + item.tiles) * ctas - 1, units));
             bar_consumers();
             if (threadIdx.x == 0) {
+                __threadfence();      // for the whole CTA, whose writes the barrier puts before it
                 const uint32_t seen = atomicAdd(p.tickets + c0, 1u);
                 s_last = seen == c1 - c0;
                 if (s_last) p.tickets[c0] = 0u;
@@ -978,14 +1014,13 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                         sum = fmaf(sum, wa, lc * wb);
                         v = make_float4(fmaf(v.x, wa, y.x * wb), fmaf(v.y, wa, y.y * wb), fmaf(v.z, wa, y.z * wb), fmaf(v.w, wa, y.w * wb));
                     }
-                    finish_row<D, LIMBS == 2>(p, item, head, r, d, top, sum, v);
+                    finish_row<D, LIMBS == 2>(p, item, this_head, r, d, top, sum, v);
                 }
             }
         }
         bar_consumers();   // s_ml, the joined rows and q are free again
         u += count;
         tile0 = 0;
-        if (++elem == p.elements) elem = 0, ++head;
     }
 }
 
