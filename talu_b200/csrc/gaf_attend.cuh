@@ -1051,7 +1051,7 @@ cudaError_t launch(const Params &p, const CUtensorMap &tmap, int sm_count, cudaS
     return cudaGetLastError();
 }
 
-// `nt`: 1 to 4 row tiles of 8 (limbs = 2: 1 or 2)
+// `nt`: 1 to 4 row tiles of 8 (4 for heads of 64 only; limbs = 2: 1 or 2)
 cudaError_t launch_d64_b4(const Params &p, const CUtensorMap &tmap, int nt, int limbs, int sm_count, cudaStream_t stream);
 cudaError_t launch_d64_b8(const Params &p, const CUtensorMap &tmap, int nt, int limbs, int sm_count, cudaStream_t stream);
 cudaError_t launch_d128_b4(const Params &p, const CUtensorMap &tmap, int nt, int limbs, int sm_count, cudaStream_t stream);
@@ -1062,8 +1062,9 @@ cudaError_t launch_rows(const Params &p, const CUtensorMap &tmap, int nt, int li
     if (limbs == 2) return nt == 1 ? launch<D, BITS, GROUP, 1, 2>(p, tmap, sm_count, stream) : launch<D, BITS, GROUP, 2, 2>(p, tmap, sm_count, stream);
     if (nt == 1) return launch<D, BITS, GROUP, 1, 1>(p, tmap, sm_count, stream);
     if (nt == 2) return launch<D, BITS, GROUP, 2, 1>(p, tmap, sm_count, stream);
-    if (nt == 3) return launch<D, BITS, GROUP, 3, 1>(p, tmap, sm_count, stream);
-    return launch<D, BITS, GROUP, 4, 1>(p, tmap, sm_count, stream);
+    if constexpr (D == 64)
+        if (nt == 4) return launch<D, BITS, GROUP, 4, 1>(p, tmap, sm_count, stream);
+    return launch<D, BITS, GROUP, 3, 1>(p, tmap, sm_count, stream);
 }
 
 // tcgen05, bf16 rows (gaf_attend_wide.cuh): 256 rows a tile

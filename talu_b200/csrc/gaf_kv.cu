@@ -459,8 +459,16 @@ cudaError_t attention_generic(const AttnArgs &a, bool f32, cudaStream_t stream) 
     return cudaGetLastError();
 }
 
-// Up to so many rows of a cached head and sequence the register-path kernel takes bf16 calls.
-constexpr uint64_t kNarrowRows = 32;
+// Up to how many rows of a cached head and sequence the register-path kernel takes bf16 calls; `items`: sequences x cached heads.
+// Its time grows with the rows, the tcgen05 kernel's hardly does; with fewer items than SMs every item is cut across many CTAs,
+// and the larger units of the tcgen05 kernel leave fewer parts to join.  Measured (8 cached heads, 8 bits; register path
+// against tcgen05, us), 24 sequences of 3000 tokens, then 4 of 800:
+//   heads of 128   16 rows 61 / 111, 33 / 27    24 rows 106 / 112, 47 / 27    32 rows 168 / 112, 65 / 27
+//   heads of 64    16 rows 36 / 90, 21 / 22     24 rows 43 / 90, 28 / 22      32 rows 54 / 91, 36 / 22
+uint64_t narrow_rows(uint32_t head_dim, uint64_t items, int sm_count) {
+    const bool few = items < static_cast<uint64_t>(sm_count);
+    return head_dim == 128u ? (few ? 8u : 24u) : (few ? 16u : 32u);
+}
 
 bool attention_fast(const KvView &kv) { return kv.head_dim == 64u || kv.head_dim == 128u; }
 // the tickets of the narrow kernel, then the cuts of the wide one
@@ -490,7 +498,8 @@ cudaError_t attention(const AttnArgs &a, const CUtensorMap &tmap, const AttnWork
     p.o_vec = reinterpret_cast<uintptr_t>(a.out) % (f32 ? 16u : 8u) == 0u && a.os.token % 4u == 0u && a.os.head % 4u == 0u;
     p.q_vec = vec_ok(a.q, a.qs, f32);
     auto run = [&](uint64_t rows) {
-        if (!f32 && rows > kNarrowRows) {
+        const uint64_t items = static_cast<uint64_t>(p.prefix_pass ? 1u : a.seqs.batch) * a.kv.kv_heads;
+        if (!f32 && rows > narrow_rows(a.kv.head_dim, items, sm_count)) {
             p.row_tiles = static_cast<uint32_t>((rows + 255u) / 256u);
             p.elements = p.prefix_pass ? p.row_tiles : p.row_tiles * a.seqs.batch;
             return attend::launch_wide(p, tmap, sm_count, stream);
