@@ -414,6 +414,9 @@ int32_t attend(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const int32_t *prefix_
     if (a.seqs.total == 0) return TGAF_OK;
     if (max_new == 0 || (!a.seqs.cu && a.seqs.per > max_new)) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "max_new %u is below the rows of a sequence", max_new);
     if (static_cast<uint64_t>(a.seqs.total) * q_heads > 0x7FFFFFFFull) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "too many query rows");
+    // row tiles (of 8 rows at least) of all sequences are counted in 32 bits
+    const uint64_t per_kv = q_heads / a.kv.kv_heads, most = max_new < a.seqs.total ? max_new : a.seqs.total;
+    if ((most * per_kv + 7u) / 8u * a.seqs.batch > 0x7FFFFFFFull) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "max_new %u is too large for %u sequences", max_new, a.seqs.batch);
     a.prefix_table = prefix_table;
     a.prefix_len = prefix_len;
     a.q = q;

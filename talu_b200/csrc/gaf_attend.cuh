@@ -4,12 +4,12 @@
 //
 // Mathematics.  The affine map is taken out of the sums, so that the matrix products run on the codes as they are (exact in
 // f16) and neither keys nor values are rounded:
-//   q_r . K_j  = sum_g s_jg (sum_{d in g} q_rd c_jd) + b_jg (sum_{d in g} q_rd)
-//   out_rd     = sum_j (p_rj s_jg) (c_jd - h) + sum_j p_rj (b_jg + h s_jg),   h = 2^(bits - 1)
+//   q_r . K_j  = sum_g s_jg (sum_{d in g} q_rd (c_jd - h)) + (b_jg + h s_jg) (sum_{d in g} q_rd),   h = 2^(bits - 1)
+//   out_rd     = sum_j (p_rj s_jg) (c_jd - h) + sum_j p_rj (b_jg + h s_jg)
 // q is scaled by a power of two per row (so that it fits f16, which holds bf16's 8 bits and the codes) and the products
-// p s are rounded to f16 once (2^-12 of each); everything else is f32.  The values' codes are centred because that
-// rounding is relative to p s |c - h|: with plain codes it is relative to the distance from the group's minimum, some four
-// times the value itself.  f16 and not bf16 for the products, although s is the caller's and of any size: unpacking a
+// p s are rounded to f16 once (2^-12 of each); everything else is f32.  The codes are centred because roundings
+// are relative to s |c - h|: with plain codes they are relative to the distance from the group's minimum, some four times
+// the value itself.  f16 and not bf16 for the products, although s is the caller's and of any size: unpacking a
 // code to f16 takes two instructions a pair, to bf16 (8 bits of code in 8 bits of mantissa) four.  The range is kept
 // by the softmax's own freedom: weights are formed against a reference m that need not be the largest score, so m follows
 // the largest y_j + log2 s_j (y: scores in base 2), and p s stays within 2^-14 and 2^13 for every key that counts.
@@ -413,16 +413,16 @@ __device__ __forceinline__ void row_f32(uint32_t addr, float (&v)[GS]) {
 constexpr uint32_t kF16One16th = 0x2C002C00u;
 __device__ __forceinline__ uint32_t f16_low(uint32_t x, uint32_t minus) { return add_f16x2((x & 0x000F000Fu) | 0x64006400u, minus); }
 __device__ __forceinline__ uint32_t f16_high(uint32_t x, uint32_t minus) { return fma_f16x2((x & 0x00F000F0u) | 0x64006400u, kF16One16th, minus); }
-// K codes of one k step as two A registers.
+// K codes (less 2^(bits - 1)) of one k step as two A registers.
 template <int BITS>
 __device__ __forceinline__ void k_codes(const uint32_t *w, int step, uint32_t &lo, uint32_t &hi) {
     if (BITS == 8) {
-        lo = add_f16x2(prmt(w[step], 0x64646464u, 0x4140u), 0xE400E400u);
-        hi = add_f16x2(prmt(w[step], 0x64646464u, 0x4342u), 0xE400E400u);
+        lo = add_f16x2(prmt(w[step], 0x64646464u, 0x4140u), 0xE480E480u);      // -(1024 + 128)
+        hi = add_f16x2(prmt(w[step], 0x64646464u, 0x4342u), 0xE480E480u);
     } else {
         const uint32_t x = (step & 1) ? w[step >> 1] >> 8 : w[step >> 1];
-        lo = f16_low(x, 0xE400E400u);
-        hi = f16_high(x, 0xD400D400u);       // -64
+        lo = f16_low(x, 0xE408E408u);        // -(1024 + 8)
+        hi = f16_high(x, 0xD480D480u);       // -(64 + 8)
     }
 }
 // Element of q in a k step of the score product: what k_codes pairs with it.
@@ -724,6 +724,11 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                 row_f32<GS>(at + 8 * GS * 2, sb);
                 row_f32<GS>(at + S::SB, ba);
                 row_f32<GS>(at + S::SB + 8 * GS * 2, bb);
+#pragma unroll
+                for (int i = 0; i < GS; ++i) {
+                    ba[i] = fmaf(static_cast<float>(1 << (BITS - 1)), sa[i], ba[i]);
+                    bb[i] = fmaf(static_cast<float>(1 << (BITS - 1)), sb[i], bb[i]);
+                }
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
                     constexpr int kWords = kPiece >= 4 ? kPiece / 4 : 1;

@@ -20,7 +20,7 @@
 // The reference follows lazily, as in the narrow kernel: only when a row of the warp exceeds it by 2^8 are O (and the weights
 // of the unit that are formed already) rescaled in tensor memory.  A row's thread takes 32 scores at a time, the next 32 on
 // their way, and puts their weights into columns whose scores it has read.  Measured on a chunk of two prompts (768 and
-// 1024 new tokens over 3750 and 5000 cached ones, 32 heads on 8): TTT us; 262 with a pass of its own for the maximum,
+// 1024 new tokens over 3750 and 5000 cached ones, 32 heads on 8): 216 us; 262 with a pass of its own for the maximum,
 // 256 with that and two threads a row, 334 with two buffers of 64 keys for the scores (twice the MMAs, of half the
 // width: the issuing warp does not keep up), 387 with everything unrolled (instruction cache).
 // What bounds it: 2 x 128 x 128 exponentials per unit (16 per clock and SM) and as many clocks of tensor work; what keeps it
