@@ -1087,8 +1087,8 @@ cudaError_t launch_rows(const Params &p, const CUtensorMap &tmap, int nt, int li
 // tcgen05, bf16 rows (gaf_attend_wide.cuh): 256 rows a tile
 cudaError_t launch_wide(const Params &p, const CUtensorMap &tmap, int sm_count, cudaStream_t stream);
 
-constexpr int kMaxCtas = 4;             // per SM, of any instance
-constexpr int kMaxPartRows = 256 * 2;   // rows of the partial results of an SM's CTAs (4 CTAs x 2 slots x 32 rows; 1 x 2 x 256)
+constexpr int kMaxCtas = 4;             // per SM, of any instance (even: what follows the tickets is 8-byte aligned)
+constexpr int kMaxPartRows = 256 * 2;   // rows of the partial results of an SM's CTAs (3 CTAs x 2 slots x 32 rows; 1 x 2 x 256)
 constexpr int kMaxDim = 128;
 
 }  // namespace attend

@@ -177,11 +177,27 @@ __device__ __forceinline__ uint64_t element_of(const KvRows &x, const Place &p, 
     return (first_token + p.token) * token_stride + p.head * head_stride + p.vec * 8u;
 }
 
+// Pairs of f32 in one instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 // a / b, rounded to nearest, for r = 1 / b rounded to nearest: the product a r and one correction by its exact remainder
 // (Markstein's theorem).  The codes are those of a division, ties included, at two instructions more than a product.
-__device__ __forceinline__ float rounded_quotient(float a, float b, float r) {
-    const float q = a * r;
-    return fmaf(fmaf(-q, b, a), r, q);
+__device__ __forceinline__ uint64_t rounded_quotient2(uint64_t a, uint64_t minus_b, uint64_t r) {
+    const uint64_t q = mul2(a, r);
+    return fma2(fma2(q, minus_b, a), r, q);
 }
 
 // The group's lanes (G / 8 neighbours) share minimum and maximum.
@@ -232,10 +248,14 @@ __global__ void __launch_bounds__(kThreadsKv) gaf_kv_append_kernel(const KvView 
             // adding 1.5 * 2^23 rounds to an integer (ties to even) and leaves it in the low bits
             constexpr float kMagic = 12582912.0f;
             float y[8];
+            const uint64_t half2 = pair(0.5f, 0.5f), minus_hb2 = pair(-half_b, -half_b), minus_hs2 = pair(-half_s, -half_s), r2 = pair(r, r);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float c = rounded_quotient(fmaf(0.5f, x[k][i], -half_b), half_s, r);
+            for (int i = 0; i < 8; i += 2) {
+                const uint64_t c2 = rounded_quotient2(fma2(pair(x[k][i], x[k][i + 1]), half2, minus_hb2), minus_hs2, r2);
+                float c, d;
+                asm("mov.b64 {%0, %1}, %2;" : "=f"(c), "=f"(d) : "l"(c2));
                 y[i] = fminf(fmaxf(c, 0.0f), maxq) + kMagic;
+                y[i + 1] = fminf(fmaxf(d, 0.0f), maxq) + kMagic;
             }
             if (pl[k].row < 0) continue;
             uint8_t *dst = kv.packed + pl[k].row * kv.row_bytes + pl[k].vec * kv.bits;   // 8 codes are `bits` bytes
