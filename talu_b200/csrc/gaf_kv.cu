@@ -99,7 +99,7 @@ __device__ __forceinline__ void store8(void *p, uint64_t at, const float (&x)[8]
         if (VEC) {
             uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = f32_bf16(x[2 * i]) | (f32_bf16(x[2 * i + 1]) << 16);
+            for (int i = 0; i < 4; ++i) w[i] = attend::pack_bf16x2(x[2 * i], x[2 * i + 1]);
             *reinterpret_cast<uint4 *>(f) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
 #pragma unroll
@@ -485,9 +485,11 @@ cudaError_t attention_generic(const AttnArgs &a, bool f32, cudaStream_t stream) 
 // against tcgen05, us), 24 sequences of 3000 tokens, then 4 of 800:
 //   heads of 128   16 rows 61 / 111, 33 / 27    24 rows 106 / 112, 47 / 27    32 rows 168 / 112, 65 / 27
 //   heads of 64    16 rows 36 / 90, 21 / 22     24 rows 43 / 90, 28 / 22      32 rows 54 / 91, 36 / 22
-uint64_t narrow_rows(uint32_t head_dim, uint64_t items, int sm_count) {
+// (times of captured calls; the tcgen05 kernel's joining pass is a launch of its own, some 4 us more where launches follow one
+// another from the host, which decides for 16 rows against a shared prefix: 35 against 39 us for one of 1111 tokens.)
+uint64_t narrow_rows(uint32_t head_dim, uint64_t items, bool prefix, int sm_count) {
     const bool few = items < static_cast<uint64_t>(sm_count);
-    return head_dim == 128u ? (few ? 8u : 24u) : (few ? 16u : 32u);
+    return head_dim == 128u ? (!few ? 24u : prefix ? 16u : 8u) : (few ? 16u : 32u);
 }
 
 bool attention_fast(const KvView &kv) { return kv.head_dim == 64u || kv.head_dim == 128u; }
@@ -519,7 +521,7 @@ cudaError_t attention(const AttnArgs &a, const CUtensorMap &tmap, const AttnWork
     p.q_vec = vec_ok(a.q, a.qs, f32);
     auto run = [&](uint64_t rows) {
         const uint64_t items = static_cast<uint64_t>(p.prefix_pass ? 1u : a.seqs.batch) * a.kv.kv_heads;
-        if (!f32 && rows > narrow_rows(a.kv.head_dim, items, sm_count)) {
+        if (!f32 && rows > narrow_rows(a.kv.head_dim, items, p.prefix_pass != 0u, sm_count)) {
             p.row_tiles = static_cast<uint32_t>((rows + 255u) / 256u);
             p.elements = p.prefix_pass ? p.row_tiles : p.row_tiles * a.seqs.batch;
             return attend::launch_wide(p, tmap, sm_count, stream);
