@@ -269,14 +269,8 @@ __device__ __forceinline__ bool cta_range(const Params &p, uint32_t *s_scan, uin
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t per_thread = (p.elements + THREADS - 1u) / THREADS;
     const uint32_t n_lo = threadIdx.x * per_thread, n_hi = n_lo + per_thread < p.elements ? n_lo + per_thread : p.elements;
-    const uint32_t usual = item_at<R, KEYS>(p, 0).tiles;
     uint32_t mine = 0;
-    bool alike = true;
-    for (uint32_t n = n_lo; n < n_hi; ++n) {
-        const uint32_t t = item_at<R, KEYS>(p, n).tiles;
-        mine += t;
-        alike = alike && t == usual;
-    }
+    for (uint32_t n = n_lo; n < n_hi; ++n) mine += item_at<R, KEYS>(p, n).tiles;
     uint32_t pre = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -284,7 +278,7 @@ __device__ __forceinline__ bool cta_range(const Params &p, uint32_t *s_scan, uin
         if (lane >= o) pre += v;
     }
     if (lane == 31) s_scan[warp] = pre;
-    alike = __syncthreads_and(alike) != 0;
+    __syncthreads();
     uint32_t per_head = 0;
     pre -= mine;
 #pragma unroll
@@ -294,12 +288,12 @@ __device__ __forceinline__ bool cta_range(const Params &p, uint32_t *s_scan, uin
     }
     out.units = static_cast<uint64_t>(per_head) * p.a.kv.kv_heads;
     if (out.units == 0) return false;
-    // Items of one size that are fewer than the CTAs are cut into as many parts each, where that leaves hardly a CTA idle: a CTA
-    // then has a part of one item and writes one partial result instead of two.  (A prefix of 16384 tokens for 96 sequences, 24
-    // items on 148 CTAs: 85 us for its pass, 93 without.)
-    const uint64_t items = static_cast<uint64_t>(p.elements) * p.a.kv.kv_heads;
+    // The row tiles of a prefix pass are items of one size: where that leaves hardly a CTA idle they are cut into as many parts each,
+    // so that a CTA has a part of one item and writes one partial result instead of two.  (A prefix of 16384 tokens for 96
+    // sequences, 24 items on 148 CTAs: 85 us for its pass, 93 without.)
     out.ctas = gridDim.x;
-    if (alike && items < out.ctas && gridDim.x % static_cast<uint32_t>(items) * 16u <= gridDim.x) out.ctas -= gridDim.x % static_cast<uint32_t>(items);
+    const uint64_t items = static_cast<uint64_t>(p.elements) * p.a.kv.kv_heads;
+    if (p.prefix_pass && items < out.ctas && gridDim.x % static_cast<uint32_t>(items) * 16u <= gridDim.x) out.ctas -= gridDim.x % static_cast<uint32_t>(items);
     if (out.units < out.ctas) out.ctas = out.units;
     if (blockIdx.x >= out.ctas) return false;
     out.u0 = quotient(out.units * blockIdx.x, out.ctas);
