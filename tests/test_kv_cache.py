@@ -669,3 +669,88 @@ def test_decoder_layer_from_linears_and_cache(ctx, oracle):
         assert (k_back.float() - k.float()).norm() <= 2.0 ** -6 * k.float().norm()   # half a 1/255 step of a range of some six sigma
     for w in parts.values():
         w.free()
+
+
+@gpu
+@pytest.mark.parametrize("dtype, new", [(torch.bfloat16, 1), (torch.bfloat16, 70), (torch.float32, 70)])
+def test_a_bad_page_hides_its_keys_only(ctx, dtype, new):
+    """A table entry outside the cache in the middle of a sequence, or of a shared prefix: its 32 keys are not seen, all others are."""
+    import talu_b200 as gaf
+    n, page, hole = 300, 32, slice(64, 96)
+    table, pages, _ = make_tables([n], page, 1)
+    cache = filled_cache(ctx, pages, 2, 128, page, 8, 64)
+    claim(cache, table, [n])
+    q = torch.randn(new, 8, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(dtype)
+    bad = table.clone()
+    bad[0, 2] = pages
+    a = gaf.attention(ctx, cache, q, bad, dev([n]))
+    with pytest.raises(gaf.GafError) as e:
+        ctx.synchronize()
+    assert e.value.status == 7
+    b = gaf.attention_shared_prefix(ctx, cache, q, bad[0], 224, table[:, 7:], dev([n - 224]))
+    with pytest.raises(gaf.GafError):
+        ctx.synchronize()
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[hole] = False
+    k, v = ref.values(cache, table[0], n, 0)[0][:, keep], ref.values(cache, table[0], n, 1)
+    v, vs = v[0][:, keep], v[1][:, keep]
+    seen = (torch.arange(n, device="cuda") <= n - new + torch.arange(new, device="cuda")[:, None])[:, keep]
+    x = q.double().unflatten(1, (2, -1)).permute(1, 2, 0, 3)
+    w = torch.softmax((torch.einsum("hgmd,hnd->hgmn", x, k) / math.sqrt(128)).masked_fill(~seen, -math.inf), -1)
+    want = torch.einsum("hgmn,hnd->mhgd", w, v).flatten(1, 2)
+    mass = torch.einsum("hgmn,hnd->mhgd", w, vs.abs() + v.abs()).flatten(1, 2)
+    tol = (2.0 ** -8 * (3 * mass + want.abs()) if dtype == torch.bfloat16 else 2.0 ** -15 * mass) + 1e-7
+    for out in (a, b):
+        assert ((out.double() - want).abs() <= tol).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_a_generous_bound_and_a_row_that_is_not_finite(ctx, dtype, new):
+    """max_new far above what any sequence has; a NaN or an infinity in q spoils its own row and no other."""
+    import talu_b200 as gaf
+    lens = [100, 260, 31]
+    table, pages, _ = make_tables(lens, 16, 1)
+    cache = filled_cache(ctx, pages, 2, 128, 16, 4, 64)
+    claim(cache, table, lens)
+    cu = [0, new, 2 * new, 2 * new + min(new, 31)]
+    q = torch.randn(cu[-1], 8, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(dtype)
+    clean = check_attention(ctx, cache, q, table, lens, cu, 1000)
+    q[new, 3, 17] = float("nan")
+    q[0, 0, 5] = float("inf")
+    out = gaf.attention(ctx, cache, q, table, dev(lens), cu=dev(cu), max_new=1000)
+    ctx.synchronize()
+    hit = torch.zeros(clean.shape, dtype=torch.bool, device="cuda")
+    hit[new, 3] = hit[0, 0] = True
+    assert out[new, 3].isnan().all() and not out[0, 0].isfinite().any()
+    assert torch.equal(out.double()[~hit], clean[~hit])
+
+
+@gpu
+def test_a_prefix_call_that_outgrows_its_workspace_in_a_capture_is_refused():
+    import talu_b200 as gaf
+    own = gaf.Context(0, own_stream=True)
+    stream = torch.cuda.Stream()
+    own.set_stream(stream.cuda_stream)
+    cache = gaf.KvCache.allocate(own, 8, 8, 128, 16, 8, 64)
+    table, lens = dev([[0]] * 3), dev([1] * 3)
+    small, large = (torch.zeros(n, 64, 128, dtype=torch.bfloat16, device="cuda") for n in (3, 1200))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        call = lambda q: gaf.attention_shared_prefix(own, cache, q, dev_prefix, 40, table, lens, cu=cu, max_new=400)  # noqa: E731
+        dev_prefix, cu = dev([1, 2, 3]), dev([0, 1, 2, 3])
+        call(small)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call(small)
+            with pytest.raises(gaf.GafError) as e:
+                call(large)
+        assert e.value.status == 5
+        graph.replay()
+        call(large)
+    own.synchronize()
+    del graph
+    cache.free()
+    own.close()
