@@ -18,8 +18,6 @@ import torch
 
 own = False
 
-_contexts = []   # the framework's context: a program has one, whatever its inputs
-
 DTYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
 
 
@@ -242,10 +240,8 @@ def prepare(case, seed):
     }
     if own:
         import talu_b200 as gaf
-        if not _contexts:
-            _contexts.append(gaf.Context(0))
-        state["ctx"] = _contexts[0]
-        state["cache"] = gaf.KvCache.wrap_device(state["ctx"], packed, scales, biases, group, bits)
+        ctx = gaf.Context(0)
+        state["ctx"], state["cache"] = ctx, gaf.KvCache.wrap_device(ctx, packed, scales, biases, group, bits)
     return state
 
 
