@@ -532,6 +532,7 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                             const float keep = m1 == m ? 1.0f : exp2_approx(m - m1);
                             m = m1;
                             l *= keep;
+                            tmem_wait_st();      // the weights of the chunk before may still be on their way to the columns read here
 #pragma unroll 1
                             for (int y = i > 0 ? 0 : D / 16; y < D / 16 + c; ++y) {     // O, then this unit's weights so far
                                 uint32_t z[16];
