@@ -285,7 +285,9 @@ int32_t tgaf_embedding_lookup_f32(tgaf_ctx *ctx, const tgaf_weight *w, const uin
  * rounded scale reaches it.  A group that holds an infinity or a NaN reads back as NaN.
  * bits in {4, 8}; group in {32, 64, 128}; head_dim a multiple of group, at most 256; page_tokens in {16, 32, 64, 128, 256};
  * pages * 2 * kv_heads * page_tokens < 2^31.  The three buffers are the caller's device memory (16-byte aligned), are not
- * copied and must outlive the cache; what lies in rows that no sequence reaches never matters. */
+ * copied and must outlive the cache; what lies in rows that no sequence reaches never matters.  The cache may be used with
+ * every context of the device that it was wrapped for, and must not be wrapped while the context's stream is captured unless the
+ * context has a cache already. */
 typedef struct tgaf_kv_cache tgaf_kv_cache;
 int32_t tgaf_kv_cache_wrap_device(tgaf_ctx *ctx, void *d_packed, void *d_scales, void *d_biases, uint64_t pages,
                                   uint32_t kv_heads, uint32_t page_tokens, uint32_t head_dim, uint32_t group_size,
@@ -328,7 +330,8 @@ int32_t tgaf_kv_read(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_se
  * [total, q_heads, head_dim], strides in elements, head_dim contiguous; out must not overlap q.  f32 statistics and sums.
  * max_new: an upper bound of the own tokens of any sequence (the launch is sized by it; a sequence with more sets the
  * error word and its rows from max_new on are left as they were).  A row that sees no key gives 0.
- * The partial results of long sequences lie in a workspace of the context, made with its first cache: calls captured into
+ * The partial results of long sequences lie in a workspace of the context, made with its first cache (or by its first call,
+ * where the cache is another context's; such a call cannot be captured): calls captured into
  * graphs must not be replayed at the same time as other attention calls of the same context (one context per stream). */
 int32_t tgaf_attention(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *seqs, uint32_t dtype, const void *q,
                        uint64_t q_token_stride, uint64_t q_head_stride, uint32_t q_heads, uint32_t max_new, float scale,

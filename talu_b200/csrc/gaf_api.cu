@@ -165,6 +165,7 @@ struct tgaf_host_batch {
 
 struct tgaf_kv_cache {
     KvView v;
+    int device = 0;     // any context of this device may use the cache
     CUtensorMap tmap;   // the codes' rows
     bool fast = false;  // the tensor-core attention kernels take this head size
 };
@@ -386,6 +387,7 @@ int32_t kv_seqs(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *i
                 KvSeqs *out) {
     if (!ctx) return TGAF_ERR_INVALID_ARGUMENT;
     if (!cache || !in) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "null cache or sequences");
+    if (cache->device != ctx->device) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "the cache is on device %d, the context on %d", cache->device, ctx->device);
     if (dtype != TGAF_DTYPE_F32 && dtype != TGAF_DTYPE_BF16) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "bad dtype %u", dtype);
     *out = {in->d_table, in->table_stride, in->table_width, in->batch, in->d_lens, in->d_cu, in->total, 1u};
     if (in->total == 0) return TGAF_OK;
@@ -398,6 +400,36 @@ int32_t kv_seqs(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *i
         if (in->total % in->batch != 0) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "%u rows are no equal share of %u sequences", in->total, in->batch);
         out->per = in->total / in->batch;
     }
+    return TGAF_OK;
+}
+
+// Refuses (with `what` to do) to allocate while the context's stream is being captured.
+int32_t may_allocate(tgaf_ctx *ctx, const char *what) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    TGAF_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &cap));
+    return cap == cudaStreamCaptureStatusNone ? TGAF_OK : fail(ctx, TGAF_ERR_UNSUPPORTED, "the attention's workspace cannot be made in a capture: %s", what);
+}
+
+// The attention's workspace of a context: one size for all calls, so that captured calls may go on using it.  Made with the
+// context's first cache, or by its first attention call where the caches are another context's.
+int32_t ensure_attention(tgaf_ctx *ctx) {
+    if (ctx->attn_partials && ctx->attn_tickets) return TGAF_OK;
+    const int32_t st = may_allocate(ctx, "make a cache with this context, or an attention call, before it");
+    if (st != TGAF_OK) return st;
+    if (!ctx->attn_partials) {
+        float *b = nullptr;
+        TGAF_CUDA(ctx, cudaMalloc(reinterpret_cast<void **>(&b), attention_partial_bytes(ctx->sm_count)));
+        ctx->attn_partials = b;
+    }
+    unsigned int *t = nullptr;
+    const size_t bytes = attention_ticket_count(ctx->sm_count) * sizeof(unsigned int);
+    TGAF_CUDA(ctx, cudaMalloc(reinterpret_cast<void **>(&t), bytes));
+    const cudaError_t e = cudaMemsetAsync(t, 0, bytes, ctx->stream);   // a change of the stream waits for the old one
+    if (e != cudaSuccess) {
+        cudaFree(t);
+        return cuda_fail(ctx, e, "attention workspace");
+    }
+    ctx->attn_tickets = t;
     return TGAF_OK;
 }
 
@@ -430,14 +462,14 @@ int32_t attend(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const int32_t *prefix_
     TGAF_CUDA(ctx, cudaSetDevice(ctx->device));
     cudaError_t e;
     if (cache->fast) {
+        const int32_t made = ensure_attention(ctx);
+        if (made != TGAF_OK) return made;
         const uint64_t rows = static_cast<uint64_t>(a.seqs.total) * q_heads;
         if (prefix_table) {
             const size_t need = rows * (a.kv.head_dim + 1u) * sizeof(float);
             if (need > ctx->attn_prefix_bytes) {
-                cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-                TGAF_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &cap));
-                if (cap != cudaStreamCaptureStatusNone)
-                    return fail(ctx, TGAF_ERR_UNSUPPORTED, "the workspace must grow to %zu bytes: make a call of this size before the capture", need);
+                const int32_t may = may_allocate(ctx, "make a call of this size before it");
+                if (may != TGAF_OK) return may;
                 float *b = nullptr;
                 const size_t want = need < (size_t(8) << 20) ? size_t(8) << 20 : need;
                 TGAF_CUDA(ctx, cudaMalloc(reinterpret_cast<void **>(&b), want));
@@ -1658,21 +1690,18 @@ int32_t tgaf_kv_cache_wrap_device(tgaf_ctx *ctx, void *d_packed, void *d_scales,
     v.groups = head_dim / group_size;
     v.bits = bits;
     v.row_bytes = head_dim * bits / 8;
+    c->device = ctx->device;
+    int32_t st = TGAF_OK;
     cudaError_t e = cudaSetDevice(ctx->device);
     if (e == cudaSuccess && attention_fast(v)) {
-        // the workspace has one size for all calls: captured calls may go on using it
-        if (!ctx->attn_partials) e = cudaMalloc(reinterpret_cast<void **>(&ctx->attn_partials), attention_partial_bytes(ctx->sm_count));
-        if (e == cudaSuccess && !ctx->attn_tickets) {
-            const size_t bytes = attention_ticket_count(ctx->sm_count) * sizeof(unsigned int);
-            e = cudaMalloc(reinterpret_cast<void **>(&ctx->attn_tickets), bytes);
-            if (e == cudaSuccess) e = cudaMemsetAsync(ctx->attn_tickets, 0, bytes, ctx->stream);
-        }
-        if (e == cudaSuccess) e = make_kv_tmap(v, &c->tmap);
-        c->fast = e == cudaSuccess;
+        st = ensure_attention(ctx);
+        if (st == TGAF_OK) e = make_kv_tmap(v, &c->tmap);
+        c->fast = st == TGAF_OK && e == cudaSuccess;
     }
-    if (e != cudaSuccess) {
+    if (st == TGAF_OK && e != cudaSuccess) st = cuda_fail(ctx, e, "kv cache set-up");
+    if (st != TGAF_OK) {
         delete c;
-        return cuda_fail(ctx, e, "kv cache set-up");
+        return st;
     }
     *out_cache = c;
     return TGAF_OK;

@@ -43,6 +43,11 @@ def _tag(name: str, dtype) -> int:
     return DTYPE_F32
 
 
+def _of_device(ctx: Context, cache: KvCache):
+    if cache.ctx.device != ctx.device:
+        _refuse(f"the cache is on cuda:{cache.ctx.device}, the context on cuda:{ctx.device}")
+
+
 def _rows(ctx: Context, name: str, t, heads: int, head_dim: int, written: bool = False):
     """Rows of `t` and its pointer, token stride and head stride, if it is [rows, heads, head_dim] on the context's device."""
     shape, stride = t.shape, t.stride()
@@ -63,7 +68,7 @@ def _rows(ctx: Context, name: str, t, heads: int, head_dim: int, written: bool =
 
 
 class KvCache:
-    """A paged cache of grouped-affine K / V rows in device memory (tgaf_kv_cache).
+    """A paged cache of grouped-affine K / V rows in device memory (tgaf_kv_cache).  Any context of its device may use it.
 
     packed: int32 [pages, 2, kv_heads, page_tokens, head_dim * bits / 32], K at index 0 of the second axis, V at 1;
     scales, biases: 2-byte tensors [pages, 2, kv_heads, page_tokens, head_dim / group] of bf16 values."""
@@ -150,6 +155,7 @@ def _seqs(ctx: Context, table, lens, cu, total: int) -> _capi.KvSeqs:
 def kv_append(ctx: Context, cache: KvCache, k, v, table, lens, cu=None) -> None:
     """Quantises the call's own rows k, v [tokens, kv_heads, head_dim] (bf16 or f32, any token and head strides) into the
     sequences' pages (tgaf_kv_append).  lens counts them already; without cu every sequence has tokens / batch of them."""
+    _of_device(ctx, cache)
     tag = _tag("k", k.dtype)
     total, k_args = _rows(ctx, "k", k, cache.kv_heads, cache.head_dim)
     v_rows, v_args = _rows(ctx, "v", v, cache.kv_heads, cache.head_dim)
@@ -167,6 +173,7 @@ def kv_read(ctx: Context, cache: KvCache, table, lens, cu=None, total: int | Non
     are cu = cumulated lens.  Rows that lie in no sequence are left as they were (undefined in new tensors)."""
     if _BF16 is None:
         _torch()
+    _of_device(ctx, cache)
     if out is None:
         if total is None:
             _refuse("total (or out) is needed")
@@ -190,6 +197,7 @@ def kv_read(ctx: Context, cache: KvCache, table, lens, cu=None, total: int | Non
 
 
 def _attend(ctx: Context, cache: KvCache, q, prefix_at, prefix_len: int, table, lens, cu, max_new, scale, out):
+    _of_device(ctx, cache)
     tag = _tag("q", q.dtype)
     heads, head_dim = q.shape[1] if q.dim() == 3 else 0, cache.head_dim
     if heads == 0 or heads % cache.kv_heads:
