@@ -338,11 +338,17 @@ int32_t tgaf_attention(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_
                        void *out, uint64_t out_token_stride, uint64_t out_head_stride);
 /* The same where every sequence continues one shared prefix of prefix_len tokens, in the pages d_prefix_table
  * i32 [ceil(prefix_len / page_tokens)]: every row sees the whole prefix, then its own sequence's tokens as above (d_lens and
- * d_table do not count the prefix).  The prefix is read once for all rows of the batch instead of once per sequence. */
+ * d_table do not count the prefix).  The prefix is read once for all rows of the batch instead of once per sequence.
+ * The rows' results against the prefix, total * q_heads * (head_dim + 1) f32, lie in a workspace of the context: 8 MB from its
+ * first cache on, and at least doubled by the first call that needs more, which waits for the context's stream and allocates
+ * (refused in a capture).  Blocks that captured calls have used are kept until the context ends. */
 int32_t tgaf_attention_shared_prefix(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const int32_t *d_prefix_table,
                                      uint32_t prefix_len, const tgaf_kv_seqs *seqs, uint32_t dtype, const void *q,
                                      uint64_t q_token_stride, uint64_t q_head_stride, uint32_t q_heads, uint32_t max_new,
                                      float scale, void *out, uint64_t out_token_stride, uint64_t out_head_stride);
+/* Makes that workspace large enough for shared-prefix calls of `rows` = total * q_heads rows over caches of this head size, so
+ * that neither they nor their capture have to wait for it. */
+int32_t tgaf_attention_reserve(tgaf_ctx *ctx, const tgaf_kv_cache *cache, uint64_t rows);
 
 /* ---- the SwiGLU FFN as one operator ---------------------------------------
  * y[m, d_model] = down( silu(gate(x)) * up(x) ), the body of SwiGLU.forward

@@ -33,10 +33,10 @@ from .gaf import (  # noqa: F401
     Batch,
     make_comm_id,
 )
-from .kv import KvCache, attention, attention_shared_prefix, kv_append, kv_read  # noqa: F401
+from .kv import KvCache, attention, attention_reserve, attention_shared_prefix, kv_append, kv_read  # noqa: F401
 
 __all__ = [
     "Context", "Weight", "GafError", "linear", "linear_fixed_scratch", "hint_next_weight", "linear_allreduce", "linear_bias", "ACT_SILU", "ACT_GELU", "ffn_swiglu", "linear_host", "HostBatch", "Batch", "make_comm_id", "dequant_f32", "dequant_f32_host", "embedding_lookup_f32",
-    "KvCache", "kv_append", "kv_read", "attention", "attention_shared_prefix",
+    "KvCache", "kv_append", "kv_read", "attention", "attention_shared_prefix", "attention_reserve",
     "gaffine_matvec_f32", "SCALES_F16", "SCALES_BF16", "SHARD_NONE", "SHARD_COL", "SHARD_ROW",
 ]

@@ -56,6 +56,7 @@ SIGNATURES = {
     "tgaf_kv_read": (_i32, [_vp, _vp, _sq, _u32, _vp, _u64, _u64, _vp, _u64, _u64]),
     "tgaf_attention": (_i32, [_vp, _vp, _sq, _u32, _vp, _u64, _u64, _u32, _u32, C.c_float, _vp, _u64, _u64]),
     "tgaf_attention_shared_prefix": (_i32, [_vp, _vp, _vp, _u32, _sq, _u32, _vp, _u64, _u64, _u32, _u32, C.c_float, _vp, _u64, _u64]),
+    "tgaf_attention_reserve": (_i32, [_vp, _vp, _u64]),
     "tgaf_comm_make_id": (_i32, [_vp]),
     "tgaf_comm_init": (_i32, [_vp, _vp, _u32, _u32]),
     "tgaf_comm_destroy": (_i32, [_vp]),

@@ -113,11 +113,16 @@ struct tgaf_ctx {
     unsigned int *gemm_flags = nullptr;
     size_t gemm_flag_count = 0;
     // attention over the quantised KV cache: partial results of sequences cut across CTAs, and the rows' results against a
-    // shared prefix.  The latter grows; what it has outgrown is kept until the context ends, since a captured graph may hold it
+    // shared prefix.  The latter at least doubles when it grows; a block that a captured call has used is kept until the context
+    // ends, since a graph may hold it (all of them together are smaller than the present one)
     float *attn_partials = nullptr;
     unsigned int *attn_tickets = nullptr;
-    std::vector<float *> attn_prefix;
+    float *attn_prefix = nullptr;
     size_t attn_prefix_bytes = 0;
+    bool attn_prefix_captured = false;
+    static constexpr int kPrefixKept = 32;   // doublings from kPrefixFirst on
+    float *attn_prefix_kept[kPrefixKept] = {};
+    int attn_prefix_kept_count = 0;
     std::vector<tgaf_batch *> batches;   // live launch lists (their counters are reset after an abandoned launch)
     NcclComm comm = nullptr;
     uint32_t comm_rank = 0, comm_size = 1;
@@ -403,24 +408,58 @@ int32_t kv_seqs(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *i
     return TGAF_OK;
 }
 
+bool is_capturing(tgaf_ctx *ctx, cudaError_t *e) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    *e = cudaStreamIsCapturing(ctx->stream, &cap);
+    return cap != cudaStreamCaptureStatusNone;
+}
 // Refuses (with `what` to do) to allocate while the context's stream is being captured.
 int32_t may_allocate(tgaf_ctx *ctx, const char *what) {
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    TGAF_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &cap));
-    return cap == cudaStreamCaptureStatusNone ? TGAF_OK : fail(ctx, TGAF_ERR_UNSUPPORTED, "the attention's workspace cannot be made in a capture: %s", what);
+    cudaError_t e;
+    const bool capturing = is_capturing(ctx, &e);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaStreamIsCapturing");
+    return capturing ? fail(ctx, TGAF_ERR_UNSUPPORTED, "the attention's workspace cannot be made in a capture: %s", what) : TGAF_OK;
 }
+
+// The rows' results against a shared prefix.  The first block is made with the rest of the workspace, so that calls of up to
+// kPrefixFirst bytes (16 k rows of 128 values) never allocate.
+constexpr size_t kPrefixFirst = size_t(8) << 20;
+int32_t ensure_prefix(tgaf_ctx *ctx, size_t need) {
+    if (need <= ctx->attn_prefix_bytes) return TGAF_OK;
+    const int32_t st = may_allocate(ctx, "reserve it (tgaf_attention_reserve) before");
+    if (st != TGAF_OK) return st;
+    if (ctx->attn_prefix && ctx->attn_prefix_captured && ctx->attn_prefix_kept_count == tgaf_ctx::kPrefixKept)
+        return fail(ctx, TGAF_ERR_OUT_OF_MEMORY, "too many workspaces of captured calls");
+    const size_t twice = 2 * ctx->attn_prefix_bytes, least = need < kPrefixFirst ? kPrefixFirst : need, want = least < twice ? twice : least;
+    float *old = ctx->attn_prefix;
+    const bool keep = old && ctx->attn_prefix_captured;
+    if (old && !keep) TGAF_CUDA(ctx, cudaStreamSynchronize(ctx->stream));   // calls in flight may still use it
+    ctx->attn_prefix = nullptr;
+    ctx->attn_prefix_bytes = 0;
+    ctx->attn_prefix_captured = false;
+    if (keep) ctx->attn_prefix_kept[ctx->attn_prefix_kept_count++] = old;
+    else if (old) cudaFree(old);
+    float *b = nullptr;
+    TGAF_CUDA(ctx, cudaMalloc(reinterpret_cast<void **>(&b), want));
+    ctx->attn_prefix = b;
+    ctx->attn_prefix_bytes = want;
+    return TGAF_OK;
+}
+size_t prefix_bytes(uint64_t rows, uint32_t head_dim) { return rows * (head_dim + 1u) * sizeof(float); }
 
 // The attention's workspace of a context: one size for all calls, so that captured calls may go on using it.  Made with the
 // context's first cache, or by its first attention call where the caches are another context's.
 int32_t ensure_attention(tgaf_ctx *ctx) {
-    if (ctx->attn_partials && ctx->attn_tickets) return TGAF_OK;
-    const int32_t st = may_allocate(ctx, "make a cache with this context, or an attention call, before it");
+    if (ctx->attn_partials && ctx->attn_tickets && ctx->attn_prefix) return TGAF_OK;
+    int32_t st = may_allocate(ctx, "make a cache with this context, or an attention call, before");
+    if (st == TGAF_OK) st = ensure_prefix(ctx, kPrefixFirst);
     if (st != TGAF_OK) return st;
     if (!ctx->attn_partials) {
         float *b = nullptr;
         TGAF_CUDA(ctx, cudaMalloc(reinterpret_cast<void **>(&b), attention_partial_bytes(ctx->sm_count)));
         ctx->attn_partials = b;
     }
+    if (ctx->attn_tickets) return TGAF_OK;
     unsigned int *t = nullptr;
     const size_t bytes = attention_ticket_count(ctx->sm_count) * sizeof(unsigned int);
     TGAF_CUDA(ctx, cudaMalloc(reinterpret_cast<void **>(&t), bytes));
@@ -464,20 +503,15 @@ int32_t attend(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const int32_t *prefix_
     if (cache->fast) {
         const int32_t made = ensure_attention(ctx);
         if (made != TGAF_OK) return made;
-        const uint64_t rows = static_cast<uint64_t>(a.seqs.total) * q_heads;
         if (prefix_table) {
-            const size_t need = rows * (a.kv.head_dim + 1u) * sizeof(float);
-            if (need > ctx->attn_prefix_bytes) {
-                const int32_t may = may_allocate(ctx, "make a call of this size before it");
-                if (may != TGAF_OK) return may;
-                float *b = nullptr;
-                const size_t want = need < (size_t(8) << 20) ? size_t(8) << 20 : need;
-                TGAF_CUDA(ctx, cudaMalloc(reinterpret_cast<void **>(&b), want));
-                ctx->attn_prefix.push_back(b);
-                ctx->attn_prefix_bytes = want;
+            const int32_t grown = ensure_prefix(ctx, prefix_bytes(static_cast<uint64_t>(a.seqs.total) * q_heads, a.kv.head_dim));
+            if (grown != TGAF_OK) return grown;
+            if (!ctx->attn_prefix_captured) {
+                ctx->attn_prefix_captured = is_capturing(ctx, &e);
+                if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaStreamIsCapturing");
             }
         }
-        const AttnWorkspace ws = {ctx->attn_partials, ctx->attn_tickets, prefix_table ? ctx->attn_prefix.back() : nullptr};
+        const AttnWorkspace ws = {ctx->attn_partials, ctx->attn_tickets, prefix_table ? ctx->attn_prefix : nullptr};
         e = attention(a, cache->tmap, ws, dtype == TGAF_DTYPE_F32, ctx->sm_count, ctx->stream);
     } else {
         e = attention_generic(a, dtype == TGAF_DTYPE_F32, ctx->stream);
@@ -685,7 +719,8 @@ int32_t tgaf_ctx_destroy(tgaf_ctx *ctx) {
     if (ctx->gemm_flags) cudaFree(ctx->gemm_flags);
     if (ctx->attn_partials) cudaFree(ctx->attn_partials);
     if (ctx->attn_tickets) cudaFree(ctx->attn_tickets);
-    for (float *b : ctx->attn_prefix) cudaFree(b);
+    if (ctx->attn_prefix) cudaFree(ctx->attn_prefix);
+    for (int i = 0; i < ctx->attn_prefix_kept_count; ++i) cudaFree(ctx->attn_prefix_kept[i]);
     if (ctx->owns_stream && ctx->stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
     return TGAF_OK;
@@ -1712,6 +1747,17 @@ int32_t tgaf_kv_cache_free(tgaf_ctx *ctx, tgaf_kv_cache *cache) {
     if (!ctx) return TGAF_ERR_INVALID_ARGUMENT;
     delete cache;   // nothing on the device belongs to it; launches in flight hold copies of what they need
     return TGAF_OK;
+}
+
+int32_t tgaf_attention_reserve(tgaf_ctx *ctx, const tgaf_kv_cache *cache, uint64_t rows) {
+    if (!ctx) return TGAF_ERR_INVALID_ARGUMENT;
+    if (!cache) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "null cache");
+    if (cache->device != ctx->device) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "the cache is on device %d, the context on %d", cache->device, ctx->device);
+    if (rows > 0x7FFFFFFFull) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "too many query rows");
+    if (!cache->fast) return TGAF_OK;
+    TGAF_CUDA(ctx, cudaSetDevice(ctx->device));
+    const int32_t st = ensure_attention(ctx);
+    return st == TGAF_OK ? ensure_prefix(ctx, prefix_bytes(rows, cache->v.head_dim)) : st;
 }
 
 int32_t tgaf_kv_append(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *seqs, uint32_t dtype, const void *k,

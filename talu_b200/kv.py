@@ -240,7 +240,7 @@ def attention_shared_prefix(ctx: Context, cache: KvCache, q, prefix_table, prefi
                             scale=None, out=None):
     """`attention` for sequences that all continue one shared prefix of `prefix_len` tokens in the pages `prefix_table`
     (int32 [pages], on the device); table and lens do not count the prefix.  Its pages are read once for the whole batch
-    (tgaf_attention_shared_prefix)."""
+    (tgaf_attention_shared_prefix).  Calls of more than some 16 k rows (tokens x heads of 128): see `attention_reserve`."""
     _tag("q", q.dtype)
     if prefix_table.dtype is not _I32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous():
         _refuse(f"prefix_table must be contiguous int32 [pages], got {prefix_table.dtype} {tuple(prefix_table.shape)}")
@@ -249,3 +249,12 @@ def attention_shared_prefix(ctx: Context, cache: KvCache, q, prefix_table, prefi
     if prefix_table.get_device() != ctx.device:
         _refuse(f"prefix_table must be on cuda:{ctx.device}, got {prefix_table.device}")
     return _attend(ctx, cache, q, prefix_table.data_ptr(), int(prefix_len), table, lens, cu, max_new, scale, out)
+
+
+def attention_reserve(ctx: Context, cache: KvCache, rows: int) -> None:
+    """Makes the context's workspace large enough for `attention_shared_prefix` calls of up to `rows` = tokens x heads rows
+    (tgaf_attention_reserve): in front of a capture of such calls, or so that the first of them need not wait for it."""
+    _of_device(ctx, cache)
+    if not 0 <= rows < 2 ** 31:
+        _refuse(f"rows must lie between 0 and 2^31 - 1, got {rows}")
+    ctx._check(ctx._lib.tgaf_attention_reserve(ctx._h, cache._h, rows))

@@ -67,3 +67,82 @@ def test_a_context_without_a_cache_of_its_own(new):
     cache.free()
     other.close()
     owner.close()
+
+
+def _prefix_calls(own, heads=64, most=600):
+    """A cache and a function that makes a shared-prefix call of n tokens, all tensors of the largest call in hand."""
+    import talu_b200 as gaf
+    cache = filled_cache(own, 6, 8, 128, 16, 8, 64)
+    prefix, table, lens = dev([1, 2, 3]), dev([[0]]), dev([16])
+    claim(cache, dev([[1, 2, 3], [0, 0, 0]]), [40, 16])
+    q = torch.randn(most, heads, 128, device="cuda").bfloat16()
+    out, cu = torch.zeros_like(q), [dev([0, n]) for n in range(most + 1)]
+    torch.cuda.synchronize()
+    return cache, lambda n: gaf.attention_shared_prefix(own, cache, q[:n], prefix, 40, table, lens, cu=cu[n], max_new=n, out=out[:n]), q, out
+
+
+@gpu
+def test_the_prefix_workspace_of_growing_calls():
+    """Calls that grow step by step hold twice what the largest of them needs at most, whatever was needed before."""
+    import talu_b200 as gaf
+    own = gaf.Context(0)
+    cache, call, q, out = _prefix_calls(own)
+    call(1)
+    own.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for n in range(20, 601, 20):
+        call(n)
+    own.synchronize()
+    assert free - torch.cuda.mem_get_info()[0] <= 2 * 600 * 64 * 129 * 4 + 2 ** 22
+    want, mass = ref.attention(cache, q, dev([[0]]), [16], [0, 600], dev([1, 2, 3]), 40)
+    assert ((out.double() - want).abs() <= 2.0 ** -8 * (mass + want.abs()) + 1e-7).all()
+    cache.free()
+    own.close()
+
+
+def test_bad_reservations_are_refused(fake):  # noqa: F811
+    from talu_b200 import GafError, attention_reserve
+    for rows in (-1, 2 ** 31, 2 ** 64 + 5):
+        with pytest.raises(GafError) as e:
+            attention_reserve(fake.ctx, fake, rows)
+        assert e.value.invalid_argument
+    from talu_b200 import _capi
+    assert _capi.load().tgaf_attention_reserve(None, None, 5) == 1
+
+
+@gpu
+def test_a_reserved_workspace_and_captured_calls():
+    """Reserved calls neither allocate nor are refused in a capture; a graph keeps its block when later calls outgrow it."""
+    import talu_b200 as gaf
+    own = gaf.Context(0, own_stream=True)
+    stream = torch.cuda.Stream()
+    own.set_stream(stream.cuda_stream)
+    cache, call, q, out = _prefix_calls(own)
+    gaf.attention_reserve(own, cache, 300 * 64)
+    want, mass = ref.attention(cache, q, dev([[0]]), [16], [0, 600], dev([1, 2, 3]), 40)
+    good = lambda n: bool(((out[:n].double() - w[:n]).abs() <= 2.0 ** -8 * (m[:n] + w[:n].abs()) + 1e-7).all())  # noqa: E731
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call(300)
+        w, m = ref.attention(cache, q, dev([[0]]), [16], [0, 300], dev([1, 2, 3]), 40)
+        free = torch.cuda.mem_get_info()[0]
+        call(600)
+        gaf.attention_reserve(own, cache, 600 * 64)
+        own.synchronize()
+        assert torch.cuda.mem_get_info()[0] < free                 # the graph's block is kept beside the new one
+        gaf.attention_reserve(own, cache, 2500 * 64)               # ... the one of the call in between is not
+        gaf.attention_reserve(own, cache, 5000 * 64)
+        own.synchronize()
+        assert free - torch.cuda.mem_get_info()[0] <= 2 * 2500 * 64 * 129 * 4 + 2 ** 22
+        out.zero_()
+        graph.replay()
+        own.synchronize()
+        assert good(300)
+        call(600)
+        own.synchronize()
+        w, m = want, mass
+        assert good(600)
+    del graph
+    cache.free()
+    own.close()
