@@ -7,12 +7,16 @@
 //   q_r . K_j  = sum_g s_jg (sum_{d in g} q_rd (c_jd - h)) + (b_jg + h s_jg) (sum_{d in g} q_rd),   h = 2^(bits - 1)
 //   out_rd     = sum_j (p_rj s_jg) (c_jd - h) + sum_j p_rj (b_jg + h s_jg)
 // q is scaled by a power of two per row (so that it fits f16, which holds bf16's 8 bits and the codes) and the products
-// p s are rounded to f16 once (2^-12 of each); everything else is f32.  The codes are centred because roundings
+// p s are rounded to f16 once (2^-11 of each); everything else is f32.  The codes are centred because roundings
 // are relative to s |c - h|: with plain codes they are relative to the distance from the group's minimum, some four times
 // the value itself.  f16 and not bf16 for the products, although s is the caller's and of any size: unpacking a
-// code to f16 takes two instructions a pair, to bf16 (8 bits of code in 8 bits of mantissa) four.  The range is kept
-// by the softmax's own freedom: weights are formed against a reference m that need not be the largest score, so m follows
-// the largest y_j + log2 s_j (y: scores in base 2), and p s stays within 2^-14 and 2^13 for every key that counts.
+// code to f16 takes two instructions a pair, to bf16 (8 bits of code in 8 bits of mantissa) four.  The range is kept by powers
+// of two: weights p are formed against a reference m, an integer within 2^8 of the row's largest score (base 2), and the products of
+// each group have a factor of their own per row, which keeps the largest of them between 2^4 and 2^15.  So a group whose
+// scales are far below its neighbours' has weights of as many bits, and a weight loses some only below 2^-18 of the group's
+// largest one, where its step is 2^-28 of that.  (With one factor for all groups, from the largest scale of each key, a group
+// 2^20 below it was 1.6e-3 off in f32.  A factor per group costs nothing per unit, but 0.3 to 1 us where a segment begins: 16
+// sequences of 2500 tokens, 32 heads on 8, 8 bits: 24.8 -> 26.2 us, f32 28.8 -> 30.4.)
 // LIMBS = 2 (f32 q): q and p s are split into two f16 terms each (22 bits).
 //
 // Both products are formed transposed (keys as the 16 rows of the MMA's A operand, query rows as its 8 columns): with one
@@ -43,7 +47,8 @@ constexpr int kKeys = 64;                      // keys of a unit
 constexpr int kConsumers = 4;                  // consumer warps
 constexpr int kThreads = (kConsumers + 1) * 32;
 constexpr float kLazy = 8.0f;                  // the reference follows only when it is exceeded by 2^8
-constexpr float kTarget = 4.0f;                // largest p s of a row when its reference is set: 2^4 to 2^5
+constexpr int kTarget = 4;                     // a group's factor brings the largest p s of a row to 2^4 to 2^5 when it is set
+constexpr int kMostExp = 15;                   // ... and keeps it below 2^15 (f16)
 constexpr float kNoMax = -3.0e38f;             // reference of a row that has seen no key: finite, so that -inf scores give 0
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -123,6 +128,8 @@ __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
+// 2^e; 0 below the normal numbers
+__device__ __forceinline__ float pow2_or_0(int e) { return e < -126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -131,6 +138,17 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y;\n\t"
+        "mov.b64 x, {%2, %3};\n\t"
+        "mov.b64 y, {%4, %5};\n\t"
+        "mul.rn.f32x2 x, x, y;\n\t"
+        "mov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -368,8 +386,9 @@ struct Shape {
     static constexpr int HALVES = NT >= 2 && NP >= 2 ? 2 : 1;   // the warps' sums are joined D / HALVES values at a time
     static constexpr int OW = D / HALVES + 4;              // pitch of a joined row (floats)
     static constexpr int JOIN = kConsumers * R * OW * 4;
+    static constexpr int FACTORS = kConsumers * R * (GS + 1) * 4;      // by warp: factors by group and row, limits by row
     static constexpr int CTAS = NT >= 2 ? 2 : 3;           // per SM
-    static constexpr int FIXED = QF + JOIN + 1024;
+    static constexpr int FIXED = QF + JOIN + FACTORS + 1024;
     static constexpr int FIT = (226 * 1024 / CTAS - 2048 - FIXED) / STAGE;
     static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static constexpr int SMEM = STAGES * STAGE + FIXED;
@@ -396,15 +415,6 @@ __device__ __forceinline__ void lds(uint32_t addr, uint32_t *w) {
     else if (BYTES == 8) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
     else if (BYTES == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
     else asm volatile("{\n\t.reg .u16 h;\n\tld.shared.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(w[0]) : "r"(addr));
-}
-// Floor of log2 of a key's largest scale, kept where 2^-it times the weights stays finite; a scale that is not finite lends nothing.
-template <int GS>
-__device__ __forceinline__ float key_exponent(const float (&v)[GS]) {
-    float top = fabsf(v[0]);
-#pragma unroll
-    for (int i = 1; i < GS; ++i) top = fmaxf(top, fabsf(v[i]));
-    const float e = static_cast<float>(static_cast<int>(__float_as_uint(top) >> 23) - 127);
-    return top <= 3.4e38f ? fmaxf(e, -40.0f) : -40.0f;
 }
 // The GS bf16 values of a row of scales or biases.
 template <int GS>
@@ -480,6 +490,7 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
     uint8_t *const qf_ptr = base_ptr + S::STAGES * S::STAGE;
     float *const join = reinterpret_cast<float *>(qf_ptr + S::QF);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float *const factor = join + S::JOIN / 4 + (warp < kConsumers ? warp : 0) * (R * (GS + 1)), *const limit = factor + R * GS;
     const KvView &kv = p.a.kv;
 
     if (threadIdx.x == 0) {
@@ -701,6 +712,11 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
 #pragma unroll
                 for (int j = 0; j < NP; ++j) qsum[nt][c][j] = s_qsum[nt * 8 + 2 * t + c][j];
             }
+        for (int x = lane; x < R * (GS + 1); x += 32) factor[x] = x < R * GS ? pow2_or_0(126) : 0.0f;     // of no weights yet
+        __syncwarp();
+        float most_scale[GS];    // a power of two above the warp's scales of the segment so far; 0: none
+#pragma unroll
+        for (int i = 0; i < GS; ++i) most_scale[i] = 0.0f;
         float m[NT][2], l[NT][2], bsum[NT][2][GS], o[S::KS][NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -718,6 +734,7 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[i][nt][c] = 0.0f;
 
+        bool fresh = true;       // this warp has summed no unit of the segment
         // One unit.  kBorder: some row of the tile does not see all its keys, or some of its keys are in no page.
         auto unit = [&](auto border_tag, uint32_t kc, int32_t key0, uint32_t bad) {
             constexpr bool kBorder = decltype(border_tag)::value;
@@ -787,12 +804,13 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                         }
                 }
             }
-            // ---- weights: against the row's reference; it follows lazily ----
-            float va[GS], vb[GS];     // scales of the values, and the exponents that they lend the weights
+            // ---- weights: against the row's reference and the groups' factors; both follow lazily ----
+            float va[GS], vb[GS];     // scales of the values
             row_f32<GS>(kc + s_off + 2 * S::SB, va);
             row_f32<GS>(kc + s_off + 2 * S::SB + 8 * GS * 2, vb);
-            const float ea = key_exponent<GS>(va), eb = key_exponent<GS>(vb);
             bool grow = false;
+#pragma unroll
+            for (int i = 0; i < GS; ++i) grow |= fmaxf(fabsf(va[i]), fabsf(vb[i])) >= most_scale[i];
             float z[NT][4];
             auto weigh = [&]() {
 #pragma unroll
@@ -803,31 +821,100 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
             };
             weigh();
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+                const float2 most = *reinterpret_cast<const float2 *>(limit + nt * 8 + 2 * t);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) grow |= z[nt][c] + (c < 2 ? ea : eb) > kTarget + kLazy;
+                for (int c = 0; c < 4; ++c) grow |= z[nt][c] > ((c & 1) ? most.y : most.x);
+            }
             if (__any_sync(0xFFFFFFFFu, grow)) {
+                // the largest finite scales of the warp's keys so far, rounded up to a power of two
+                float scale[GS];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int i = 0; i < GS; ++i) {
+                    const float x = fabsf(va[i]), y = fabsf(vb[i]);
+                    scale[i] = fmaxf(x <= 3.4e38f ? x : 0.0f, y <= 3.4e38f ? y : 0.0f);
+                }
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        // largest score and exponent of the row, not of its distance from the present reference, which may be none
-                        const float ya = kBorder && s[nt][c] == s_hidden ? -INFINITY : fmaf(s[nt][c], f[nt][c], ea);
-                        const float yb = kBorder && s[nt][2 + c] == s_hidden ? -INFINITY : fmaf(s[nt][2 + c], f[nt][c], eb);
-                        float top = fmaxf(ya, yb);
+                for (int x = 4; x <= 16; x <<= 1)
 #pragma unroll
-                        for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-                        const float next = fmaxf(m[nt][c], top - kTarget);
-                        const float keep = next == m[nt][c] ? 1.0f : exp2_approx(m[nt][c] - next);
-                        m[nt][c] = next;
-                        l[nt][c] *= keep;
+                    for (int i = 0; i < GS; ++i) scale[i] = fmaxf(scale[i], __shfl_xor_sync(0xFFFFFFFFu, scale[i], x));
 #pragma unroll
-                        for (int i = 0; i < GS; ++i) bsum[nt][c][i] *= keep;
+                for (int i = 0; i < GS; ++i)
+                    most_scale[i] = fmaxf(most_scale[i], __uint_as_float((__float_as_uint(scale[i]) & 0x7F800000u) + 0x00800000u));
+                // `kFirst`: nothing is summed yet (and code that runs once a segment comes from far: no more of it than needed)
+                auto settle = [&](auto first_tag) {
+                    constexpr bool kFirst = decltype(first_tag)::value;
 #pragma unroll
-                        for (int i = 0; i < S::KS; ++i) o[i][nt][c] *= keep, o[i][nt][2 + c] *= keep;
+                    for (int nt = 0; nt < NT; ++nt) {
+                        // the rows' largest scores, not their distance from the present reference, which may be none
+                        float y[4], top[2], most[2][GS], up[2];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) y[c] = kBorder && s[nt][c] == s_hidden ? -INFINITY : s[nt][c] * f[nt][c & 1];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) top[c] = fmaxf(y[c], y[2 + c]);
+#pragma unroll
+                        for (int x = 4; x <= 16; x <<= 1)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) top[c] = fmaxf(top[c], __shfl_xor_sync(0xFFFFFFFFu, top[c], x));
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const float next = fmaxf(m[nt][c], ceilf(top[c]));
+                            up[c] = fminf(next - m[nt][c], 1000.0f);
+                            m[nt][c] = next;
+                            // the groups' largest products; a scale that is not finite counts for nothing or for the most
+                            const float pa = exp2_approx(y[c] - next), pb = exp2_approx(y[2 + c] - next);
+#pragma unroll
+                            for (int i = 0; i < GS; ++i) most[c][i] = fmaxf(pa == 0.0f ? 0.0f : pa * fabsf(va[i]), pb == 0.0f ? 0.0f : pb * fabsf(vb[i]));
+                        }
+#pragma unroll
+                        for (int x = 4; x <= 16; x <<= 1)
+#pragma unroll
+                            for (int c = 0; c < 2 * GS; ++c) most[c / GS][c % GS] = fmaxf(most[c / GS][c % GS], __shfl_xor_sync(0xFFFFFFFFu, most[c / GS][c % GS], x));
+                        float reach[2] = {0.0f, 0.0f};       // product of a group's factor and largest scale
+#pragma unroll
+                        for (int i = 0; i < GS; ++i) {
+                            float *const at = factor + i * R + nt * 8 + 2 * t;
+                            float set[2];
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                // 2^(kTarget - floor(log2 most)), at most 2^126
+                                const uint32_t fit = min(((254u + kTarget) << 23) - (__float_as_uint(most[c][i]) & 0x7F800000u), 253u << 23);
+                                set[c] = __uint_as_float(fit);
+                                if (!kFirst) {
+                                    // the sums' present unit is 2^-have; it is kept while the products stay below 2^(kTarget + 8)
+                                    const int have = static_cast<int>(__float_as_uint(at[c]) >> 23) - 127 + static_cast<int>(up[c]), aim = static_cast<int>(fit >> 23) - 127;
+                                    const int want = have >= aim + 8 ? aim : min(have, 126);
+                                    const float ratio = pow2_or_0(want - have);
+                                    set[c] = pow2_or_0(want);
+#pragma unroll
+                                    for (int k = i * (GROUP / 16); k < (i + 1) * (GROUP / 16); ++k) o[k][nt][c] *= ratio, o[k][nt][2 + c] *= ratio;
+                                }
+                                reach[c] = fmaxf(reach[c], set[c] * most_scale[i]);
+                            }
+                            if (!kFirst) __syncwarp();       // the row's lanes have read it
+                            if (g == 0) *reinterpret_cast<float2 *>(at) = make_float2(set[0], set[1]);
+                        }
+                        float room[2];                       // scores above the reference by that, and no more, keep all products in range
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) room[c] = fminf(kLazy, static_cast<float>(kMostExp + 127 - static_cast<int>(__float_as_uint(reach[c]) >> 23)));
+                        if (g == 0) *reinterpret_cast<float2 *>(limit + nt * 8 + 2 * t) = make_float2(room[0], room[1]);
+                        if (!kFirst) {
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                const float keep = pow2_or_0(-static_cast<int>(up[c]));
+                                l[nt][c] *= keep;
+#pragma unroll
+                                for (int i = 0; i < GS; ++i) bsum[nt][c][i] *= keep;
+                            }
+                        }
                     }
+                };
+                if (fresh) settle(std::true_type());
+                else settle(std::false_type());
+                __syncwarp();
                 weigh();
             }
+            fresh = false;
             {
                 // ---- weights times scales as B fragments, weights times biases ----
                 uint32_t pf[LIMBS][GS][NT][2];
@@ -849,7 +936,10 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                     l[nt][1] += pr[1] + pr[3];
 #pragma unroll
                     for (int i = 0; i < GS; ++i) {
-                        float x[4] = {pr[0] * va[i], pr[1] * va[i], pr[2] * vb[i], pr[3] * vb[i]};
+                        const float2 gr = *reinterpret_cast<const float2 *>(factor + i * R + nt * 8 + 2 * t);
+                        const float2 xa = mul_pair(mul_pair(make_float2(pr[0], pr[1]), make_float2(va[i], va[i])), gr);
+                        const float2 xb = mul_pair(mul_pair(make_float2(pr[2], pr[3]), make_float2(vb[i], vb[i])), gr);
+                        float x[4] = {xa.x, xa.y, xb.x, xb.y};
                         if (kBorder) {   // rows behind the end may hold anything, NaN too
                             float y[4] = {pr[0] * ba[i], pr[1] * ba[i], pr[2] * bb[i], pr[3] * bb[i]};
 #pragma unroll
@@ -939,11 +1029,14 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
 #pragma unroll
                 for (int w = 1; w < kConsumers; ++w) top = fmaxf(top, s_ml[w][r][0]);
                 const float keep = m[nt][c] == top ? 1.0f : exp2_approx(m[nt][c] - top);
+                float unit_of[GS];       // 1 / factor
+#pragma unroll
+                for (int i = 0; i < GS; ++i) unit_of[i] = __uint_as_float((254u << 23) - __float_as_uint(factor[i * R + r]));
 #pragma unroll
                 for (int i = 0; i < S::KS; ++i) {
                     const int gi = i * 16 / GROUP;
-                    o[i][nt][c] = (o[i][nt][c] + bsum[nt][c][gi]) * keep;
-                    o[i][nt][2 + c] = (o[i][nt][2 + c] + bsum[nt][c][gi]) * keep;
+                    o[i][nt][c] = fmaf(o[i][nt][c], unit_of[gi], bsum[nt][c][gi]) * keep;
+                    o[i][nt][2 + c] = fmaf(o[i][nt][2 + c], unit_of[gi], bsum[nt][c][gi]) * keep;
                 }
             }
         const bool whole = tile0 == 0u && count == item.tiles;

@@ -1,18 +1,18 @@
 """What the roundings of the attention kernels may put their results off by, per row and value, in 64 bits.
 
 Notation: key j of a sequence, group g of value d, code c centred by h = 2^(bits - 1), scale s, z = b + h s the group's centre, so that a
-stored value is s (c - h) + z; y scores, w weights of the softmax, o results.  Types round by half a step: f32 2^-24, f16 2^-12
+stored value is s (c - h) + z; y scores, w weights of the softmax, o results.  Types round by half a step: f32 2^-24, f16 2^-11
 (subnormals: 2^-25 absolute), bf16 2^-8 of the value.  Accumulators of the tensor cores may cut instead of round: 2^-23.
 
 A score that is off by e_j multiplies its weight by exp(e_j), and o moves by at most sum_j w_j (exp(|e_j|) - 1) (|v_j| + |o|).
 
 f32 scores (all kernels): q, the codes and the products are exact or in two f16 terms (2^-22); what is left are the sums of D terms and
 the factor and the reference applied to them: (D + 16) 2^-24 of the absolute terms, and 2^-22 of 1 + |y| with exp2's own.
-tcgen05 kernel: key elements are f16 of fma(c - h, s, f16(z)).  The centres' roundings add up along a group, 2^-12 |z sum_g q|; those
-of the elements to 2^-12 sum |q k| at most: a key whose elements are of one size has one rounding error in all of them, so that
+tcgen05 kernel: key elements are f16 of fma(c - h, s, f16(z)).  The centres' roundings add up along a group, 2^-11 |z sum_g q|; those
+of the elements to 2^-11 sum |q k| at most: a key whose elements are of one size has one rounding error in all of them, so that
 they cannot be taken for independent.
-Its values are rounded alike, 2^-12 (|v| + |z|), its weights by 2^-12; elements below 2^-39 of the largest of 32 keys are lost.
-Register path: w s is one f16 (2^-12), or two (2^-22), times the exact centred code; w z is f32.
+Its values are rounded alike, 2^-11 (|v| + |z|), its weights by 2^-11; elements below 2^-39 of the largest of 32 keys are lost.
+Register path: w s is one f16 (2^-11), or two (2^-22), times the exact centred code; w z is f32.
 Weights below the normal f16 numbers are 2^-25 off, where the largest one of the row (w T, T: largest element of 32 keys), or of
 the row and group (w s), is 2^top at least.
 Sums of n keys: n / 16 accumulations by the tensor cores, 16 further ones.
@@ -52,13 +52,13 @@ def _sequence(cache, x, parts, seen, scale, f32, wide, top):
     if wide:
         sums = x.unflatten(-1, (-1, group)).sum(-1).abs()
         centres = kz.abs().unflatten(-1, (-1, group))[..., 0]
-        off = off + abs(scale) * 2.0 ** -12 * (torch.einsum("hgmd,hnd->hgmn", sums, centres) + torch.einsum("hgmd,hnd->hgmn", x.abs(), k.abs()))
+        off = off + abs(scale) * 2.0 ** -11 * (torch.einsum("hgmd,hnd->hgmn", sums, centres) + torch.einsum("hgmd,hnd->hgmn", x.abs(), k.abs()))
     off = w * torch.expm1(off.clamp(max=30.0))
     bound = torch.einsum("hgmn,hnd->hgmd", off, v.abs()) + off.sum(-1, keepdim=True) * o.abs()
 
     bound = bound + (n / 16 + 16) * 2.0 ** -23 * (mass(vc) + mass(vz) + o.abs())
     if wide:
-        bound = bound + 2.0 ** -12 * (2 * mass(v) + mass(vz))
+        bound = bound + 2.0 ** -11 * (2 * mass(v) + mass(vz))
         size, at = [], 0
         for _, m in parts:
             t = torch.nn.functional.pad((vc.abs() + vz.abs())[:, at:at + m], (0, 0, 0, -m % 32))
@@ -67,10 +67,17 @@ def _sequence(cache, x, parts, seen, scale, f32, wide, top):
         size = w * torch.cat(size, 1)[:, None, None]
         bound = bound + (2.0 ** -39 * size.sum(-1) + n * 2.0 ** (-25 - top) * size.amax(-1)).unsqueeze(-1)
     else:
-        bound = bound + (2.0 ** -22 if f32 else 2.0 ** -12) * mass(vc)
+        bound = bound + (2.0 ** -22 if f32 else 2.0 ** -11) * mass(vc)
         largest = torch.stack([(w * vs[:, None, None, :, i].abs()).amax(-1) for i in range(0, D, group)], -1)
         bound = bound + n * 2.0 ** (-25 - top) * 2.0 ** (cache.bits - 1) * largest.repeat_interleave(group, -1)
     return o, bound
+
+
+def takes_wide(q, cache, rows, sequences, prefix=False):
+    """Whether the tcgen05 kernel takes a call of that many rows per cached head and sequence (narrow_rows in gaf_kv.cu)."""
+    few = sequences * cache.kv_heads < torch.cuda.get_device_properties(0).multi_processor_count
+    most = (24 if not few else 16 if prefix else 8) if cache.head_dim == 128 else 16 if few else 32
+    return q.dtype == torch.bfloat16 and cache.head_dim in (64, 128) and rows > most
 
 
 def attention(cache, q, table, lens, cu, wide, prefix_table=None, prefix_len=0, scale=None, top=0):
