@@ -17,8 +17,10 @@
 //   warp 13          TMA of codes, bulk copies of scales and biases
 // K and V tiles share a ring of three 32 KB buffers, their codes one of three stages: K(i), V(i), K(i+1), ...
 //
-// The reference follows lazily, as in the narrow kernel: only when a row of the warp exceeds it by 2^8 are O (and the weights
-// of the unit that are formed already) rescaled in tensor memory.  A row's thread takes 32 scores at a time, the next 32 on
+// The reference is an integer and follows lazily: a row's largest weight is brought to 2^6 to 2^7 and rescaled (O, and the weights of
+// the unit that are formed already: exactly) when it exceeds 2^15, so that weights keep their 11 bits down to 2^-20 of the largest and
+// have a step of 2^-30 of it below.  (With 2^0 in place of 2^7, 40000 keys of 2^-22 each behind one key whose values are zero were
+// 15 % off; 2^10 costs 4 %, 2^12 11 % more time.)  A row's thread takes 32 scores at a time, the next 32 on
 // their way, and puts their weights into columns whose scores it has read.  Measured on a chunk of two prompts (768 and
 // 1024 new tokens over 3750 and 5000 cached ones, 32 heads on 8): 216 us; 262 with a pass of its own for the maximum,
 // 256 with that and two threads a row, 334 with two buffers of 64 keys for the scores (twice the MMAs, of half the
@@ -37,6 +39,8 @@ constexpr int kWideRows = 256;
 constexpr int kWideThreads = 14 * 32;    // 128 registers each
 constexpr int kDequantWarp0 = 8, kDequantWarps = 4, kMmaWarp = 12, kLoadWarp = 13;
 constexpr int kInfo = 4;             // units whose side information is kept
+constexpr float kWideTarget = 7.0f;  // a row's largest weight is brought to 2^6 to 2^7
+constexpr float kWideMost = 15.0f;   // ... when it exceeds 2^15 (f16)
 constexpr float kMinFactor = 1.0e-37f;   // of raw scores: not 0, since hidden ones are -inf
 constexpr int kMinExp = -50;         // values below 2^-36 lose bits instead of pushing the weights out of f32
 
@@ -527,9 +531,9 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
 #pragma unroll
                         for (int k = 4; k < 32; ++k) tops[k & 3] = fmaxf(tops[k & 3], __uint_as_float(x[k]));
                         const float top = fmaf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fk, ve);
-                        if (__any_sync(0xFFFFFFFFu, top > m + kLazy)) {
-                            const float m1 = fmaxf(m, top);
-                            const float keep = m1 == m ? 1.0f : exp2_approx(m - m1);
+                        if (__any_sync(0xFFFFFFFFu, top > m + kWideMost)) {
+                            const float m1 = fmaxf(m, ceilf(top) - kWideTarget);
+                            const float keep = pow2_or_0(-static_cast<int>(fminf(m1 - m, 1000.0f)));
                             m = m1;
                             l *= keep;
                             tmem_wait_st();      // the weights of the chunk before may still be on their way to the columns read here

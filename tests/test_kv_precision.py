@@ -88,3 +88,29 @@ def test_groups_of_different_size(ctx, dtype, new, dim, bits, group, by_key):  #
     # the whole of each group: roundings of single weights are independent
     err, size = ((x.unflatten(-1, (-1, group)) ** 2).sum((0, 1, 3)).sqrt() for x in (out.double() - want, want))
     assert bool((err <= (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -18) * size).all())
+
+
+@gpu
+@pytest.mark.parametrize("dim, bits, new, dtype", [(128, 8, 40, torch.bfloat16), (64, 4, 40, torch.bfloat16), (128, 8, 1, torch.bfloat16), (128, 4, 1, torch.float32)])
+@pytest.mark.parametrize("below", [18.4, 22.2, 25.3])
+def test_a_long_tail_behind_one_key(ctx, dtype, dim, bits, new, below):  # noqa: F811
+    """One key takes nearly all the weight and has values of zero; what counts are 40000 others, each 2^-18 to 2^-25 of it.  As many
+    sequences (of the same pages) as it takes to keep each in one piece: the parts of a cut one have references of their own."""
+    import talu_b200 as gaf
+    n, batch, kv_heads, per_kv, page = 40000, 40, 8, 2, 64
+    table, pages, _ = make_tables([n], page, 1)
+    cache = gaf.KvCache.allocate(ctx, pages, kv_heads, dim, page, bits, 64)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    unit = torch.where(torch.rand(dim, generator=gen, device="cuda") < 0.5, -1.0, 1.0)
+    k = torch.zeros(n, kv_heads, dim, device="cuda")
+    k[3] = unit * below * math.log(2.0) / math.sqrt(dim)
+    v = 1 + 0.1 * torch.randn(n, kv_heads, dim, generator=gen, device="cuda")
+    v[3] = 0
+    gaf.kv_append(ctx, cache, k.bfloat16(), v.bfloat16(), table, dev([n]))
+    flips = torch.rand(new, kv_heads * per_kv, dim, generator=gen, device="cuda") < 0.015
+    q = torch.where(flips, -unit, unit).to(dtype)
+    wide = kv_bounds.takes_wide(q, cache, new * per_kv, batch)
+    _, want, bound = check(ctx, cache, q, table, [n], [0, new], wide, top=6 if wide else 4)
+    out = gaf.attention(ctx, cache, q.repeat(batch, 1, 1), table.expand(batch, -1).contiguous(), dev([n] * batch))
+    ctx.synchronize()
+    assert max(worst(x, want, bound) for x in out.split(new)) <= 1.0
