@@ -650,12 +650,11 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
             for (int i = 0; i < PL; ++i)
                 x[i] = LIMBS == 2 ? __uint_as_float(raw[j][LIMBS == 2 ? i : 0])
                                   : (i & 1) ? __uint_as_float(raw[j][LIMBS == 2 ? 0 : i / 2] & 0xFFFF0000u) : bf16_f32(raw[j][LIMBS == 2 ? 0 : i / 2]);
-            float top = 0.0f;
+            uint32_t top = 0u;                                   // bits of the largest magnitude; NaN is above infinity
 #pragma unroll
-            for (int i = 0; i < PL; ++i) top = fmaxf(top, fabsf(x[i]));
-#pragma unroll
-            for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-            int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;      // 2^e <= top < 2^(e + 1)
+            for (int i = 0; i < PL; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+            top = __reduce_max_sync(0xFFFFFFFFu, top);
+            int e = static_cast<int>(top >> 23) - 127;           // 2^e <= top < 2^(e + 1)
             e = e < -100 ? -100 : e > 127 ? 127 : e;
             const float mul = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
             float sum = 0.0f;
@@ -679,7 +678,8 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
             for (int o = 1; o < 32 / NP; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
             if (lane % (32 / NP) == 0) s_qsum[r][lane / (32 / NP)] = sum;
             if (lane == 0) {
-                s_f[r] = __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23) * (p.a.scale * 1.4426950408889634f);
+                // a row that is not finite gives NaN wherever it sees a key (its scores may all be -inf)
+                s_f[r] = top < 0x7F800000u ? __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23) * (p.a.scale * 1.4426950408889634f) : __uint_as_float(0x7FC00000u);
                 const int32_t seen = p.prefix_pass ? item.seen0 : item.seen0 + static_cast<int32_t>(row / p.per_kv);
                 s_seen[r] = have ? (seen < item.keys ? seen : item.keys) : 0;
             }

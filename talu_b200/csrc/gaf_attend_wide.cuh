@@ -467,6 +467,7 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
             if (active) {
                 // ---- q: scaled by a power of two, f16 ----
                 float f;
+                bool finite;
                 {
                     uint32_t x[D / 2];      // bf16 pairs
 #pragma unroll
@@ -488,6 +489,7 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                     uint32_t top = 0u;
 #pragma unroll
                     for (int i = 0; i < D / 2; ++i) top = max(top, max((x[i] << 16) & 0x7FFFFFFFu, x[i] & 0x7FFF0000u));
+                    finite = top < 0x7F800000u;
                     int e = static_cast<int>(top >> 23) - 127;
                     e = e < -100 ? -100 : e > 127 ? 127 : e;
                     // the sign of the scale goes to q, so that the largest raw score is the largest score
@@ -611,6 +613,7 @@ gaf_attend_wide_kernel(const __grid_constant__ Params p, const __grid_constant__
                 wait(s_done[t], done_seen++ & 1u);
                 __syncwarp();
                 fence_after();
+                if (!finite && seen > 0) l = __uint_as_float(0x7FC00000u);    // a row that is not finite, whose scores may all be -inf
                 if (!whole && have) {
                     __stcg(part + kWideRows * D + t * 128u + r, m);
                     __stcg(part + kWideRows * (D + 1) + t * 128u + r, l);

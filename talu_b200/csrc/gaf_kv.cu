@@ -357,11 +357,14 @@ __global__ void __launch_bounds__(kWarpsGen * 32) gaf_attention_generic_kernel(c
         if (threadIdx.x == 0) atomicOr(a.error_word, kKvBadCount);
         return;
     }
+    bool bad = false;
     for (uint32_t d = threadIdx.x; d < D; d += kWarpsGen * 32) {
         const uint64_t at = t * a.qs.token + hq * a.qs.head + d;
         s_q[d] = F32 ? static_cast<const float *>(a.q)[at] : bf16_f32(static_cast<const uint16_t *>(a.q)[at]);
+        bad |= !(fabsf(s_q[d]) <= FLT_MAX);
     }
-    __syncthreads();
+    // a row that is not finite gives NaN wherever it sees a key (its scores may all be -inf)
+    const float scale = __syncthreads_or(bad) ? __uint_as_float(0x7FC00000u) : a.scale;
     const int64_t limit = static_cast<int64_t>(a.seqs.lens[b]) - (end - 1 - static_cast<int64_t>(t));   // keys seen
     float m = -INFINITY, l = 0.0f, o[kMaxDim / 32];
 #pragma unroll
@@ -386,7 +389,7 @@ __global__ void __launch_bounds__(kWarpsGen * 32) gaf_attention_generic_kernel(c
                     for (uint32_t d = g * kv.group; d < (g + 1u) * kv.group; ++d)
                         score = fmaf(s_q[d], fmaf(static_cast<float>(code_at(kv, row, d)), s, bias), score);
                 }
-                score *= a.scale;
+                score *= scale;
             }
             float top = score;
             for (int x = 16; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));

@@ -146,3 +146,37 @@ def test_a_reserved_workspace_and_captured_calls():
     del graph
     cache.free()
     own.close()
+
+
+@gpu
+@pytest.mark.parametrize("dtype, new, dim", [(torch.bfloat16, 1, 128), (torch.bfloat16, 40, 64), (torch.float32, 5, 128), (torch.bfloat16, 2, 96), (torch.bfloat16, 40, 128)])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_a_query_row_that_is_not_finite(ctx, dtype, new, dim, value, prefix):  # noqa: F811
+    """Keys whose values are all negative where the row has its infinity: every score is -inf (or inf), and the row is NaN as a
+    softmax of such scores is.  Rows that see no key stay zero, all others as they were."""
+    import talu_b200 as gaf
+    lens, page = [300, 0, 90], 32
+    table, pages, _ = make_tables(lens + [prefix], page, 1)
+    cache = gaf.KvCache.allocate(ctx, pages, 2, dim, page, 8, 32)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    for row, n in zip(table, lens + [prefix]):
+        if n:
+            kv = torch.randn(2, n, 2, dim, device="cuda", generator=gen)
+            kv[0] = -1 - kv[0].abs()
+            gaf.kv_append(ctx, cache, kv[0], kv[1], row[None].contiguous(), dev([n]))
+    cu = [0, new, 2 * new, 3 * new]
+    q = torch.randn(3 * new, 6, dim, device="cuda", generator=gen).to(dtype)
+    head = table[-1, :2].contiguous()
+
+    def run():
+        args = (ctx, cache, q) + ((head, prefix) if prefix else ()) + (table[:3], dev(lens))
+        return (gaf.attention_shared_prefix if prefix else gaf.attention)(*args, cu=dev(cu), max_new=new)
+    clean = run()
+    hit = torch.zeros(clean.shape, dtype=torch.bool, device="cuda")
+    for t, h in ((0, 1), (new, 4), (3 * new - 1, 0)):
+        q[t, h, 7] = value
+        hit[t, h] = prefix > 0 or t != new
+    out = run()
+    ctx.synchronize()
+    assert clean.isfinite().all() and torch.equal(out.isnan(), hit) and torch.equal(out[~hit], clean[~hit])
