@@ -42,7 +42,7 @@ extern "C" {
 #define TGAF_ERR_NCCL 4
 #define TGAF_ERR_UNSUPPORTED 5
 #define TGAF_ERR_TIMEOUT 6
-#define TGAF_ERR_DEVICE_FLAG 7 /* a kernel set its error word: a bounded wait ran out, or (tgaf_kv_*, tgaf_attention*) a bad block table */
+#define TGAF_ERR_DEVICE_FLAG 7 /* a kernel set its error word: a bounded wait ran out, or (tgaf_kv_*, tgaf_attention*) a bad block table or d_cu */
 
 /* scales dtype tags: core/src/compute/cuda/gaffine_u4_matvec.zig:13-14 */
 #define TGAF_SCALES_F16 0u
@@ -302,6 +302,8 @@ int32_t tgaf_kv_cache_free(tgaf_ctx *ctx, tgaf_kv_cache *cache);
  *            LAST ones of the sequence; non-decreasing, d_cu[0] = 0.  NULL: total / batch tokens of each sequence.
  *   total    rows of the packed tensors; rows from d_cu[batch] on are left as they were
  * A row whose position would be negative (more own tokens than d_lens has) is not stored, not read back and sees no key.
+ * Where d_cu reaches beyond total, the rows that there are are worked on and the next tgaf_synchronize returns
+ * TGAF_ERR_DEVICE_FLAG.
  * A table entry outside the cache, or a length beyond the table's width: the tokens in question are skipped (not stored, read
  * back or seen) and the next tgaf_synchronize returns TGAF_ERR_DEVICE_FLAG. */
 typedef struct tgaf_kv_seqs {

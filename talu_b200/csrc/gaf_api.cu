@@ -838,6 +838,7 @@ int32_t tgaf_synchronize(tgaf_ctx *ctx) {
             if (b->tagged) cudaMemset(b->tagged, 0, b->tagged_bytes);
         }
         if (flag & kKvBadTable) return fail(ctx, TGAF_ERR_DEVICE_FLAG, "a block table named a page outside the cache, or a length was beyond its table");
+        if (flag & kKvBadRows) return fail(ctx, TGAF_ERR_DEVICE_FLAG, "a sequence's own rows reached beyond the rows of the call");
         if (flag & kKvBadCount) return fail(ctx, TGAF_ERR_DEVICE_FLAG, "a sequence had more new tokens than max_new");
         return fail(ctx, TGAF_ERR_DEVICE_FLAG, "a kernel gave up a bounded wait (code 0x%x)", flag);
     }

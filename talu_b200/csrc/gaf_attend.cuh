@@ -240,8 +240,12 @@ __device__ __forceinline__ Item item_at(const Params &p, uint32_t n) {
     if (count > static_cast<int64_t>(p.a.max_new)) {
         atomicOr(p.a.error_word, kKvBadCount);
     }
-    const int64_t take = count > static_cast<int64_t>(p.a.max_new) ? static_cast<int64_t>(p.a.max_new) : count;
-    it.rows = take > 0 && begin >= 0 && begin + take <= static_cast<int64_t>(s.total) ? static_cast<uint32_t>(take) * p.per_kv : 0u;
+    int64_t take = count > static_cast<int64_t>(p.a.max_new) ? static_cast<int64_t>(p.a.max_new) : count;
+    if (count > 0 && begin + count > static_cast<int64_t>(s.total)) {
+        atomicOr(p.a.error_word, kKvBadRows);
+        take = begin + take > static_cast<int64_t>(s.total) ? static_cast<int64_t>(s.total) - begin : take;
+    }
+    it.rows = take > 0 && begin >= 0 ? static_cast<uint32_t>(take) * p.per_kv : 0u;
     it.token0 = begin;
     it.keys = it.first_seen = it.seen0 = 0;
     it.tiles = 0;

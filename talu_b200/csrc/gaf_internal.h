@@ -166,6 +166,7 @@ struct AttnArgs {
 // bits of the error word
 constexpr unsigned int kKvBadTable = 0x40000000u;   // a table entry outside the cache, or a length beyond the table
 constexpr unsigned int kKvBadCount = 0x20000000u;   // a sequence with more own tokens than max_new
+constexpr unsigned int kKvBadRows = 0x10000000u;    // a sequence whose own rows reach beyond the call's
 cudaError_t kv_append(const KvView &kv, const KvSeqs &seqs, bool f32, const void *k, KvStrides ks, const void *v, KvStrides vs,
                       unsigned int *error_word, cudaStream_t stream);
 cudaError_t kv_read(const KvView &kv, const KvSeqs &seqs, bool f32, void *k, KvStrides ks, void *v, KvStrides vs,

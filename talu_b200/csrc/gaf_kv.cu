@@ -162,7 +162,11 @@ struct Walk {
         split();
     }
 };
+__device__ __forceinline__ void check_rows(const KvSeqs &s, unsigned int *error_word) {
+    if (blockIdx.x == 0 && threadIdx.x == 0 && s.cu && s.cu[s.batch] > static_cast<int64_t>(s.total)) atomicOr(error_word, kKvBadRows);
+}
 __device__ __forceinline__ void find_rows(const KvView &kv, const KvSeqs &seqs, uint32_t tokens, int64_t *s_row, unsigned int *error_word) {
+    check_rows(seqs, error_word);
     for (uint32_t x = threadIdx.x; x < tokens; x += kThreadsKv) {
         const uint64_t t = static_cast<uint64_t>(blockIdx.x) * tokens + x;
         s_row[x] = t < seqs.total ? row_of(kv, seqs, static_cast<uint32_t>(t), error_word) : -1;
@@ -349,6 +353,7 @@ __global__ void __launch_bounds__(kWarpsGen * 32) gaf_attention_generic_kernel(c
     const uint32_t t = blockIdx.x / a.q_heads, hq = blockIdx.x % a.q_heads, head = hq / (a.q_heads / kv.kv_heads);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t D = kv.head_dim;
+    check_rows(a.seqs, a.error_word);
     const int b = seq_of(a.seqs, t);
     if (b < 0) return;
     const int64_t begin = a.seqs.cu ? static_cast<int64_t>(a.seqs.cu[b]) : static_cast<int64_t>(b) * a.seqs.per;

@@ -180,3 +180,41 @@ def test_a_query_row_that_is_not_finite(ctx, dtype, new, dim, value, prefix):  #
     out = run()
     ctx.synchronize()
     assert clean.isfinite().all() and torch.equal(out.isnan(), hit) and torch.equal(out[~hit], clean[~hit])
+
+
+@gpu
+@pytest.mark.parametrize("dtype, new, dim", [(torch.bfloat16, 3, 128), (torch.bfloat16, 40, 64), (torch.float32, 3, 64), (torch.bfloat16, 3, 96)])
+def test_own_rows_beyond_those_of_the_call(ctx, dtype, new, dim):  # noqa: F811
+    """cu ends two rows behind the tensors: every call works on the rows that there are, as if there were two more, and reports it."""
+    import talu_b200 as gaf
+    lens, page = [100, 80], 32
+    table, pages, _ = make_tables(lens, page, 1)
+    caches = [filled_cache(ctx, pages, 2, dim, page, 8, 32, garbage=False) for _ in range(2)]
+    for c in caches:
+        claim(c, table, lens)
+    x = torch.randn(2 * new, 8, dim, device="cuda").to(dtype)
+    cu, short, results = dev([0, new, 2 * new]), 2 * new - 2, []
+    for c, n in zip(caches, (2 * new, short)):
+        def call(f, c=c, n=n):
+            y = f(c, n)
+            if n == short:
+                with pytest.raises(gaf.GafError) as e:
+                    ctx.synchronize()
+                assert e.value.status == 7 and "rows" in e.value.message
+            ctx.synchronize()
+            return y
+        call(lambda c, n: gaf.kv_append(ctx, c, x[:n, :2], x[:n, 2:4], table, dev(lens), cu=cu))
+        k, v = call(lambda c, n: gaf.kv_read(ctx, c, table, dev(lens), cu=cu, total=n, dtype=dtype))
+        a = call(lambda c, n: gaf.attention(ctx, c, x[:n], table, dev(lens), cu=cu, max_new=new))
+        p = call(lambda c, n: gaf.attention_shared_prefix(ctx, c, x[:n], table[0, :2].contiguous(), 50, table, dev(lens), cu=cu, max_new=new))
+        results.append((k, v, a, p))
+        if n == 2 * new:                       # the two rows that the other cache does not get
+            for t, s in zip((caches[1].packed, caches[1].scales, caches[1].biases), (c.packed, c.scales, c.biases)):
+                last = table[1, 2].long()
+                t[last, :, :, 14:16] = s[last, :, :, 14:16]
+    whole, part = results
+    for w, y in zip(whole[:2], part[:2]):
+        assert torch.equal(w[:short], y)
+    bound = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -18
+    for w, y in zip(whole[2:], part[2:]):      # the row tiles differ, and with them the order of the sums
+        assert (w[:short].double() - y.double()).abs().max() <= bound * w.abs().max()
