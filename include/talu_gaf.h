@@ -296,7 +296,8 @@ int32_t tgaf_kv_cache_free(tgaf_ctx *ctx, tgaf_kv_cache *cache);
 
 /* The sequences of a call; all arrays on the device, so that a captured call follows them from replay to replay.
  *   d_table  i32 [batch][table_width], rows table_stride elements apart: page of the sequence's tokens
- *            [i*page_tokens, (i+1)*page_tokens); entries behind a sequence's last page are not read
+ *            [i*page_tokens, (i+1)*page_tokens); entries behind a sequence's last page are not read;
+ *            table_width * page_tokens < 2^31 - 256
  *   d_lens   i32 [batch]      cached tokens of each sequence, the call's own included
  *   d_cu     i32 [batch + 1]  the call's own tokens of sequence b are rows [d_cu[b], d_cu[b+1]) of its packed tensors and the
  *            LAST ones of the sequence; non-decreasing, d_cu[0] = 0.  NULL: total / batch tokens of each sequence.

@@ -387,6 +387,8 @@ int32_t raw_matvec(tgaf_ctx *ctx, uint32_t bits, const float *input, const uint3
     return linear_device(ctx, ctx->raw_cache[slot], input, batch_rows, out, true);
 }
 
+constexpr uint64_t kMostPositions = 0x7FFFFFFFull - 256u;
+
 // Checks shared by the cache's entry points, and the sequences as the kernels take them.
 int32_t kv_seqs(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *in, uint32_t dtype, const void *a, const void *b,
                 KvSeqs *out) {
@@ -399,6 +401,9 @@ int32_t kv_seqs(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_seqs *i
     if (in->batch == 0) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "rows without a sequence");
     if (!in->d_table || !in->d_lens || !a || !b) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "null device pointer");
     if (in->table_width == 0 || in->table_stride < in->table_width) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "bad table width %u", in->table_width);
+    // positions, and the end of the unit that holds one, are 32-bit numbers with a sign
+    if (static_cast<uint64_t>(in->table_width) * cache->v.page_tokens > kMostPositions)
+        return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "a table of %u pages of %u tokens is too wide", in->table_width, cache->v.page_tokens);
     if (in->batch > 0x7FFFFFFEu || static_cast<uint64_t>(in->total) * cache->v.kv_heads * cache->v.head_dim / 4 / 256 >= 0x7FFFFFFFull)
         return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "too many rows: %u", in->total);
     if (!in->d_cu) {
@@ -1798,7 +1803,7 @@ int32_t tgaf_attention_shared_prefix(tgaf_ctx *ctx, const tgaf_kv_cache *cache, 
                                      float scale, void *out, uint64_t out_token_stride, uint64_t out_head_stride) {
     if (!ctx) return TGAF_ERR_INVALID_ARGUMENT;
     if (prefix_len != 0 && !d_prefix_table) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "null prefix table");
-    if (prefix_len > 0x7FFFFFFFu) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "prefix_len %u too large", prefix_len);
+    if (prefix_len > kMostPositions) return fail(ctx, TGAF_ERR_INVALID_ARGUMENT, "prefix_len %u too large", prefix_len);
     return attend(ctx, cache, prefix_len ? d_prefix_table : nullptr, prefix_len, seqs, dtype, q, {q_token_stride, q_head_stride},
                   q_heads, max_new, scale, out, {out_token_stride, out_head_stride});
 }

@@ -43,6 +43,13 @@ def _tag(name: str, dtype) -> int:
     return DTYPE_F32
 
 
+def _count(name: str, value, least: int = 0, most: int = 2 ** 32 - 1) -> int:
+    """An integer that the C entry takes as it is: ctypes would drop the bits above 32, and a sign."""
+    if isinstance(value, bool) or not hasattr(value, "__index__") or not least <= value.__index__() <= most:
+        _refuse(f"{name} must be an integer from {least} to {most}, got {value!r}")
+    return value.__index__()
+
+
 def _of_device(ctx: Context, cache: KvCache):
     if cache.ctx.device != ctx.device:
         _refuse(f"the cache is on cuda:{cache.ctx.device}, the context on cuda:{ctx.device}")
@@ -64,6 +71,8 @@ def _rows(ctx: Context, name: str, t, heads: int, head_dim: int, written: bool =
                 if step < reach:
                     _refuse(f"{name} must not overlap itself")
                 reach = step * size
+    if shape[0] > 2 ** 32 - 1:
+        _refuse(f"{name} has too many rows: {shape[0]}")
     return shape[0], (t.data_ptr(), stride[0], stride[1])
 
 
@@ -177,9 +186,9 @@ def kv_read(ctx: Context, cache: KvCache, table, lens, cu=None, total: int | Non
     if out is None:
         if total is None:
             _refuse("total (or out) is needed")
-        tag, rows = DTYPE_BF16 if dtype is None else _tag("dtype", dtype), total
+        tag, rows = DTYPE_BF16 if dtype is None else _tag("dtype", dtype), _count("total", total)
         seqs = _seqs(ctx, table, lens, cu, rows)
-        k, v = cache.scales.new_empty((2, total, cache.kv_heads, cache.head_dim), dtype=dtype or _BF16).unbind(0)
+        k, v = cache.scales.new_empty((2, rows, cache.kv_heads, cache.head_dim), dtype=dtype or _BF16).unbind(0)
         at, step = k.data_ptr(), cache.kv_heads * cache.head_dim
         k_args, v_args = (at, step, cache.head_dim), (v.data_ptr(), step, cache.head_dim)
     else:
@@ -208,6 +217,8 @@ def _attend(ctx: Context, cache: KvCache, q, prefix_at, prefix_len: int, table, 
         if cu is not None:
             _refuse("max_new is needed with cu")
         max_new = total // max(1, seqs.batch)
+    else:
+        max_new = _count("max_new", max_new, 1 if total else 0)
     if out is None:
         out = q.new_empty((total, heads, head_dim))
         out_args = (out.data_ptr(), heads * head_dim, head_dim)
@@ -244,17 +255,17 @@ def attention_shared_prefix(ctx: Context, cache: KvCache, q, prefix_table, prefi
     _tag("q", q.dtype)
     if prefix_table.dtype is not _I32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous():
         _refuse(f"prefix_table must be contiguous int32 [pages], got {prefix_table.dtype} {tuple(prefix_table.shape)}")
-    if prefix_len < 0 or prefix_len > prefix_table.shape[0] * cache.page_tokens:
+    prefix_len = _count("prefix_len", prefix_len)
+    if prefix_len > prefix_table.shape[0] * cache.page_tokens:
         _refuse(f"prefix_len {prefix_len} does not fit {prefix_table.shape[0]} pages of {cache.page_tokens} tokens")
     if prefix_table.get_device() != ctx.device:
         _refuse(f"prefix_table must be on cuda:{ctx.device}, got {prefix_table.device}")
-    return _attend(ctx, cache, q, prefix_table.data_ptr(), int(prefix_len), table, lens, cu, max_new, scale, out)
+    return _attend(ctx, cache, q, prefix_table.data_ptr(), prefix_len, table, lens, cu, max_new, scale, out)
 
 
 def attention_reserve(ctx: Context, cache: KvCache, rows: int) -> None:
     """Makes the context's workspace large enough for `attention_shared_prefix` calls of up to `rows` = tokens x heads rows
     (tgaf_attention_reserve): in front of a capture of such calls, or so that the first of them need not wait for it."""
     _of_device(ctx, cache)
-    if not 0 <= rows < 2 ** 31:
-        _refuse(f"rows must lie between 0 and 2^31 - 1, got {rows}")
+    rows = _count("rows", rows, 0, 2 ** 31 - 1)
     ctx._check(ctx._lib.tgaf_attention_reserve(ctx._h, cache._h, rows))

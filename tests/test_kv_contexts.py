@@ -218,3 +218,42 @@ def test_own_rows_beyond_those_of_the_call(ctx, dtype, new, dim):  # noqa: F811
     bound = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -18
     for w, y in zip(whole[2:], part[2:]):      # the row tiles differ, and with them the order of the sums
         assert (w[:short].double() - y.double()).abs().max() <= bound * w.abs().max()
+
+
+def test_counts_that_do_not_fit_are_refused(fake):  # noqa: F811
+    """Negative numbers, numbers above 32 bits and numbers that are none: what C would read from them is something else."""
+    from talu_b200 import GafError, attention, attention_shared_prefix, kv_append, kv_read
+    x, table, lens = _args()
+    q, cu = torch.zeros(3, 4, 64, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int32)
+    head = torch.zeros(2, dtype=torch.int32)
+    many = torch.zeros(1, 2, 64, dtype=torch.bfloat16).expand(2 ** 32 + 3, 2, 64)
+    calls = [lambda: kv_append(fake.ctx, fake, many, many, table, lens, cu=cu),
+             lambda: attention(fake.ctx, fake, torch.zeros(1, 4, 64, dtype=torch.bfloat16).expand(2 ** 32 + 3, 4, 64), table, lens, cu=cu, max_new=3)]
+    for bad in (-1, 2 ** 32 + 1, 1.0, True, "3"):
+        calls += [lambda bad=bad: kv_read(fake.ctx, fake, table, lens, cu=cu, total=bad),
+                  lambda bad=bad: attention(fake.ctx, fake, q, table, lens, cu=cu, max_new=bad),
+                  lambda bad=bad: attention_shared_prefix(fake.ctx, fake, q, head, 8, table, lens, cu=cu, max_new=bad),
+                  lambda bad=bad: attention_shared_prefix(fake.ctx, fake, q, head, bad, table, lens)]
+    calls.append(lambda: attention(fake.ctx, fake, q, table, lens, cu=cu, max_new=0))
+    for call in calls:
+        with pytest.raises(GafError) as e:
+            call()
+        assert e.value.invalid_argument
+
+
+@gpu
+def test_tables_wider_than_positions_are_refused(ctx):  # noqa: F811
+    """Wider than what 32 bits with a sign count (rows of a table may overlap where their stride says so, so no memory is needed)."""
+    import ctypes as C
+    import talu_b200 as gaf
+    from talu_b200 import _capi
+    cache = gaf.KvCache.allocate(ctx, 1, 1, 64, 256, 8, 64)
+    t, n, q = dev([[0]]), dev([1]), torch.zeros(1, 1, 64, device="cuda", dtype=torch.bfloat16)
+    width = 2 ** 31 // 256
+    seqs = _capi.KvSeqs(t.data_ptr(), width, width, 1, n.data_ptr(), None, 1)
+    p = C.c_void_p(q.data_ptr())
+    assert ctx._lib.tgaf_kv_append(ctx._h, cache._h, seqs, gaf.gaf.DTYPE_BF16, p, 64, 64, p, 64, 64) == 1
+    assert ctx._lib.tgaf_attention(ctx._h, cache._h, seqs, gaf.gaf.DTYPE_BF16, p, 64, 64, 1, 1, C.c_float(1.0), p, 64, 64) == 1
+    assert ctx._lib.tgaf_attention_shared_prefix(ctx._h, cache._h, C.c_void_p(t.data_ptr()), 2 ** 31 - 100, _capi.KvSeqs(t.data_ptr(), 1, 1, 1, n.data_ptr(), None, 1),
+                                                 gaf.gaf.DTYPE_BF16, p, 64, 64, 1, 1, C.c_float(1.0), p, 64, 64) == 1
+    cache.free()
