@@ -4,7 +4,9 @@ Notation: key j of a sequence, group g of value d, code c centred by h = 2^(bits
 stored value is s (c - h) + z; y scores, w weights of the softmax, o results.  Types round by half a step: f32 2^-24, f16 2^-11
 (subnormals: 2^-25 absolute), bf16 2^-8 of the value.  Accumulators of the tensor cores may cut instead of round: 2^-23.
 
-A score that is off by e_j multiplies its weight by exp(e_j), and o moves by at most sum_j w_j (exp(|e_j|) - 1) (|v_j| + |o|).
+A score that is off by e_j multiplies its weight by exp(e_j).  Since sum_j w_j (v_j - o) = 0, o moves by
+sum_j w_j (exp(e_j) - 1) (v_j - o) / sum_j w_j exp(e_j), which is at most sum_j w_j (exp(|e_j|) - 1) |v_j - o| / sum_j w_j exp(-|e_j|).
+(|v_j - o| is taken for |v_j| + |o| where its table would be large.)
 
 f32 scores (all kernels): q, the codes and the products are exact or in two f16 terms (2^-22); what is left are the sums of D terms and
 the factor and the reference applied to them: (D + 16) 2^-24 of the absolute terms, and 2^-22 of 1 + |y| with exp2's own.
@@ -53,8 +55,14 @@ def _sequence(cache, x, parts, seen, scale, f32, wide, top):
         sums = x.unflatten(-1, (-1, group)).sum(-1).abs()
         centres = kz.abs().unflatten(-1, (-1, group))[..., 0]
         off = off + abs(scale) * 2.0 ** -11 * (torch.einsum("hgmd,hnd->hgmn", sums, centres) + torch.einsum("hgmd,hnd->hgmn", x.abs(), k.abs()))
+    least = (w * torch.exp(-off)).sum(-1, keepdim=True).clamp(min=1e-300)
     off = w * torch.expm1(off.clamp(max=30.0))
-    bound = torch.einsum("hgmn,hnd->hgmd", off, v.abs()) + off.sum(-1, keepdim=True) * o.abs()
+    if w.numel() * D <= 2 ** 27:
+        away = torch.stack([(v[:, None] - o[..., i, None, :]).abs() for i in range(x.shape[2])], 2)      # [h, g, m, n, d]
+        bound = torch.einsum("hgmn,hgmnd->hgmd", off, away)
+    else:
+        bound = torch.einsum("hgmn,hnd->hgmd", off, v.abs()) + off.sum(-1, keepdim=True) * o.abs()
+    bound = bound / least
 
     bound = bound + (n / 16 + 16) * 2.0 ** -23 * (mass(vc) + mass(vz) + o.abs())
     if wide:

@@ -84,7 +84,7 @@ def test_groups_of_different_size(ctx, dtype, new, dim, bits, group, by_key):  #
     cu = [0, new, 2 * new, 3 * new]
     q = torch.randn(cu[-1], kv_heads * per_kv, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(dtype)
     wide = kv_bounds.takes_wide(q, cache, new * per_kv, len(lens))
-    out, want, bound = check(ctx, cache, q, table, lens, cu, wide, top=0 if wide else 4)
+    out, want, bound = check(ctx, cache, q, table, lens, cu, wide, top=6 if wide else 4)
     # the whole of each group: roundings of single weights are independent
     err, size = ((x.unflatten(-1, (-1, group)) ** 2).sum((0, 1, 3)).sqrt() for x in (out.double() - want, want))
     assert bool((err <= (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -18) * size).all())
@@ -114,3 +114,25 @@ def test_a_long_tail_behind_one_key(ctx, dtype, dim, bits, new, below):  # noqa:
     out = gaf.attention(ctx, cache, q.repeat(batch, 1, 1), table.expand(batch, -1).contiguous(), dev([n] * batch))
     ctx.synchronize()
     assert max(worst(x, want, bound) for x in out.split(new)) <= 1.0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("dim, group", [(128, 64), (64, 32), (96, 32)])
+@pytest.mark.parametrize("k_size, v_size, q_size, scale", [(1e-12, 1e-9, 1.0, 1e11), (1e30, 1e30, 1e-30, 0.1), (1.0, 1e20, 0.0, 1.0), (1.0, 1.0, 30.0, 1.0),
+                                                         (1.0, 1.0, 1.0, -0.3), (1.0, 1.0, 1.0, 0.0), (30.0, 1e-6, 3e4, 1e-4)])
+def test_sizes_and_scales(ctx, dtype, new, dim, group, k_size, v_size, q_size, scale):  # noqa: F811
+    """Values of any size that f32 sums hold, scores in the hundreds, scale of either sign or zero, q of zeros: by rows, each to
+    the bound of its own scores, so that scores in the hundreds are checked as well as others."""
+    lens, kv_heads = [150, 700], 2
+    table, pages, _ = make_tables(lens, 32, 7)
+    cache = filled_cache(ctx, pages, kv_heads, dim, 32, 8, group)
+    claim(cache, table, lens)
+    for t in (cache.scales, cache.biases):
+        t[:, 0] *= k_size
+        t[:, 1] *= v_size
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q = (torch.randn(2 * new, 4 * kv_heads, dim, device="cuda", generator=gen) * q_size).to(dtype)
+    wide = kv_bounds.takes_wide(q, cache, 4 * new, 2)
+    check(ctx, cache, q, table, lens, cumulate([new, new]), wide, scale=scale, top=6 if wide else 4)
