@@ -842,6 +842,8 @@ int32_t tgaf_synchronize(tgaf_ctx *ctx) {
             if (b->list) gemv_list_reset(b->list);
             if (b->tagged) cudaMemset(b->tagged, 0, b->tagged_bytes);
         }
+        // a non-blocking stream does not wait for the resets: without this the next launch's counters could be among them
+        TGAF_CUDA(ctx, cudaStreamSynchronize(cudaStreamLegacy));
         if (flag & kKvBadTable) return fail(ctx, TGAF_ERR_DEVICE_FLAG, "a block table named a page outside the cache, or a length was beyond its table");
         if (flag & kKvBadRows) return fail(ctx, TGAF_ERR_DEVICE_FLAG, "a sequence's own rows reached beyond the rows of the call");
         if (flag & kKvBadCount) return fail(ctx, TGAF_ERR_DEVICE_FLAG, "a sequence had more new tokens than max_new");

@@ -257,3 +257,28 @@ def test_tables_wider_than_positions_are_refused(ctx):  # noqa: F811
     assert ctx._lib.tgaf_attention_shared_prefix(ctx._h, cache._h, C.c_void_p(t.data_ptr()), 2 ** 31 - 100, _capi.KvSeqs(t.data_ptr(), 1, 1, 1, n.data_ptr(), None, 1),
                                                  gaf.gaf.DTYPE_BF16, p, 64, 64, 1, 1, C.c_float(1.0), p, 64, 64) == 1
     cache.free()
+
+
+@gpu
+def test_calls_right_behind_a_reported_error():
+    """The reset of a context's counters after an error is over before the next launch, on a non-blocking stream too."""
+    import talu_b200 as gaf
+    own = gaf.Context(0, own_stream=True)
+    lens = [3000, 500]
+    table, pages, _ = make_tables(lens, 32, 1)
+    cache = filled_cache(own, pages, 2, 128, 32, 8, 64)
+    claim(cache, table, lens)
+    bad, n, q = table.clone(), dev(lens), torch.randn(2, 8, 128, device="cuda").bfloat16()
+    bad[0, 3] = pages
+    outs = [torch.zeros_like(q) for _ in range(50)]
+    torch.cuda.synchronize()
+    for out in outs:
+        gaf.attention(own, cache, q, bad, n, out=out)
+        with pytest.raises(gaf.GafError):
+            own.synchronize()
+        gaf.attention(own, cache, q, table, n, out=out)
+    own.synchronize()
+    assert close(outs[0], cache, q, table, lens, [0, 1, 2])
+    assert all(torch.equal(out, outs[0]) for out in outs)
+    cache.free()
+    own.close()
