@@ -42,7 +42,7 @@ constexpr int kInfo = 4;             // units whose side information is kept
 constexpr float kWideTarget = 7.0f;  // a row's largest weight is brought to 2^6 to 2^7
 constexpr float kWideMost = 15.0f;   // ... when it exceeds 2^15 (f16)
 constexpr float kMinFactor = 1.0e-37f;   // of raw scores: not 0, since hidden ones are -inf
-constexpr int kMinExp = -50;         // values below 2^-36 lose bits instead of pushing the weights out of f32
+constexpr int kMinExp = -90;         // values below 2^-76 lose bits instead of pushing the sums of weights, 2^(15 + 90) a key, out of f32
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
     uint64_t d = 0;

@@ -136,3 +136,23 @@ def test_sizes_and_scales(ctx, dtype, new, dim, group, k_size, v_size, q_size, s
     q = (torch.randn(2 * new, 4 * kv_heads, dim, device="cuda", generator=gen) * q_size).to(dtype)
     wide = kv_bounds.takes_wide(q, cache, 4 * new, 2)
     check(ctx, cache, q, table, lens, cumulate([new, new]), wide, scale=scale, top=6 if wide else 4)
+
+
+@gpu
+@pytest.mark.parametrize("dtype, new", [(torch.bfloat16, 1), (torch.bfloat16, 40), (torch.float32, 5)])
+@pytest.mark.parametrize("v_size", [2.0 ** -45, 2.0 ** -60, 2.0 ** -74])
+def test_small_values(ctx, dtype, new, v_size):  # noqa: F811
+    """Values far below one, in a whole cache and in every other page beside ordinary ones: sums of weights and weighted values
+    stay in range."""
+    lens, kv_heads, dim = [150, 700], 2, 128
+    table, pages, _ = make_tables(lens, 32, 7)
+    cache = filled_cache(ctx, pages, kv_heads, dim, 32, 8, 64)
+    claim(cache, table, lens)
+    for t in (cache.scales, cache.biases):
+        t[:, 1] *= v_size
+    q = torch.randn(2 * new, 4 * kv_heads, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(dtype)
+    wide = kv_bounds.takes_wide(q, cache, 4 * new, 2)
+    check(ctx, cache, q, table, lens, cumulate([new, new]), wide, top=6 if wide else 4)
+    for t in (cache.scales, cache.biases):
+        t[table[1, ::2].long(), 1] *= 1 / v_size
+    check(ctx, cache, q, table, lens, cumulate([new, new]), wide, top=6 if wide else 4)
