@@ -1776,7 +1776,7 @@ int32_t tgaf_kv_append(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_
     if (st != TGAF_OK || s.total == 0) return st;
     TGAF_CUDA(ctx, cudaSetDevice(ctx->device));
     const cudaError_t e = kv_append(cache->v, s, dtype == TGAF_DTYPE_F32, k, {k_token_stride, k_head_stride}, v,
-                                    {v_token_stride, v_head_stride}, ctx->d_error_word, ctx->stream);
+                                    {v_token_stride, v_head_stride}, ctx->d_error_word, ctx->sm_count, ctx->stream);
     return e == cudaSuccess ? TGAF_OK : cuda_fail(ctx, e, "kv_append launch");
 }
 
@@ -1788,7 +1788,7 @@ int32_t tgaf_kv_read(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_se
     if (st != TGAF_OK || s.total == 0) return st;
     TGAF_CUDA(ctx, cudaSetDevice(ctx->device));
     const cudaError_t e = kv_read(cache->v, s, dtype == TGAF_DTYPE_F32, k, {k_token_stride, k_head_stride}, v,
-                                  {v_token_stride, v_head_stride}, ctx->d_error_word, ctx->stream);
+                                  {v_token_stride, v_head_stride}, ctx->d_error_word, ctx->sm_count, ctx->stream);
     return e == cudaSuccess ? TGAF_OK : cuda_fail(ctx, e, "kv_read launch");
 }
 

@@ -168,9 +168,9 @@ constexpr unsigned int kKvBadTable = 0x40000000u;   // a table entry outside the
 constexpr unsigned int kKvBadCount = 0x20000000u;   // a sequence with more own tokens than max_new
 constexpr unsigned int kKvBadRows = 0x10000000u;    // a sequence whose own rows reach beyond the call's
 cudaError_t kv_append(const KvView &kv, const KvSeqs &seqs, bool f32, const void *k, KvStrides ks, const void *v, KvStrides vs,
-                      unsigned int *error_word, cudaStream_t stream);
+                      unsigned int *error_word, int sm_count, cudaStream_t stream);
 cudaError_t kv_read(const KvView &kv, const KvSeqs &seqs, bool f32, void *k, KvStrides ks, void *v, KvStrides vs,
-                    unsigned int *error_word, cudaStream_t stream);
+                    unsigned int *error_word, int sm_count, cudaStream_t stream);
 // Any head size the cache takes.
 cudaError_t attention_generic(const AttnArgs &a, bool f32, cudaStream_t stream);
 // Heads of 64 or 128 values.  The map covers all rows of the codes: a box of min(64, page_tokens) rows.

@@ -3,6 +3,8 @@
 //
 // A group of G values x along head_dim is stored as codes q, a bf16 scale s and a bf16 bias b:
 //   b = bf16(min x),  s = bf16((max x - min x) f32(1 / maxq)),  q = clamp(rint((x - b) / s), 0, maxq),  value = q s + b
+// (a product with the rounded reciprocal, since that is what dividing a tensor by a number comes to in torch on the GPU, so that a
+// cache filled there has the same scales; a true quotient gives a scale one bf16 step apart in some 1 in 10^5 groups of f32 rows)
 // b is exact for bf16 inputs (the minimum is one of them).  s and b are rounded to nearest once, because 16 bits each is
 // what the format stores; the codes are taken against the rounded pair, which makes the rounding of s part of the grid and
 // not an error of every value: only the top value can be off by more than half a step, (max x - min x) 2^-9 + s / 2.
@@ -115,7 +117,8 @@ struct KvRows {
 
 // Both kernels: a CTA takes `tokens` packed rows; it looks up where they lie once, and its threads then walk the rows'
 // vectors of 8 values (K heads, then V heads).  What bounds them: HBM, with enough rows; the index arithmetic has to stay
-// small beside 8 values' work, so it is carried from step to step and each thread has kUnroll loads in flight.
+// small beside 8 values' work, so it is carried from step to step and each thread has up to kUnroll loads in flight (fewer in calls
+// whose CTAs have few rows of few heads).
 constexpr int kMaxTokens = 32;    // of a CTA
 constexpr int kUnroll = 4;
 
@@ -324,8 +327,8 @@ __global__ void __launch_bounds__(kThreadsKv) gaf_kv_read_kernel(const KvView kv
 }
 
 // Rows of a CTA: as many as leave eight CTAs for each SM, so that the look-up in front of them is paid seldom and hidden
-uint32_t rows_of_cta(const KvSeqs &seqs) {
-    const uint32_t n = seqs.total / (148u * 8u);
+uint32_t rows_of_cta(const KvSeqs &seqs, int sm_count) {
+    const uint32_t n = seqs.total / (static_cast<uint32_t>(sm_count) * 8u);
     return n < 1u ? 1u : n < static_cast<uint32_t>(kMaxTokens) ? n : kMaxTokens;
 }
 
@@ -446,11 +449,11 @@ __global__ void __launch_bounds__(kWarpsGen * 32) gaf_attention_generic_kernel(c
 }  // namespace
 
 cudaError_t kv_append(const KvView &kv, const KvSeqs &seqs, bool f32, const void *k, KvStrides ks, const void *v, KvStrides vs,
-                      unsigned int *error_word, cudaStream_t stream) {
+                      unsigned int *error_word, int sm_count, cudaStream_t stream) {
     if (seqs.total == 0) return cudaSuccess;
     const KvRows in = {k, v, ks, vs};
     const bool vec = vec_ok(k, ks, f32) && vec_ok(v, vs, f32);
-    const uint32_t n = rows_of_cta(seqs), grid = (seqs.total - 1u) / n + 1u;
+    const uint32_t n = rows_of_cta(seqs, sm_count), grid = (seqs.total - 1u) / n + 1u;
     const bool fixed = kThreadsKv % (2u * kv.kv_heads * (kv.head_dim / 8u)) == 0u;
     auto go = [&](auto kernel) { kernel<<<grid, kThreadsKv, 0, stream>>>(kv, seqs, in, n, error_word); };
     if (f32 && vec && fixed) go(gaf_kv_append_kernel<true, true, true>);
@@ -463,11 +466,11 @@ cudaError_t kv_append(const KvView &kv, const KvSeqs &seqs, bool f32, const void
 }
 
 cudaError_t kv_read(const KvView &kv, const KvSeqs &seqs, bool f32, void *k, KvStrides ks, void *v, KvStrides vs,
-                    unsigned int *error_word, cudaStream_t stream) {
+                    unsigned int *error_word, int sm_count, cudaStream_t stream) {
     if (seqs.total == 0) return cudaSuccess;
     const KvRows out = {k, v, ks, vs};
     const bool vec = vec_ok(k, ks, f32) && vec_ok(v, vs, f32);
-    const uint32_t n = rows_of_cta(seqs), grid = (seqs.total - 1u) / n + 1u;
+    const uint32_t n = rows_of_cta(seqs, sm_count), grid = (seqs.total - 1u) / n + 1u;
     const bool fixed = kThreadsKv % (2u * kv.kv_heads * (kv.head_dim / 8u)) == 0u;
     auto go = [&](auto kernel) { kernel<<<grid, kThreadsKv, 0, stream>>>(kv, seqs, out, n, error_word); };
     if (f32 && vec && fixed) go(gaf_kv_read_kernel<true, true, true>);
