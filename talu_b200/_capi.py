@@ -75,8 +75,6 @@ SIGNATURES = {
     "tgaf_batch_destroy": (_i32, [_vp, _vp]),
 }
 
-
-
 # tgaf_watch_fns: the three hooks of tgaf_watchdog_wait
 WORK_DONE_FN = C.CFUNCTYPE(C.c_int32, C.c_void_p)
 ASYNC_ERROR_FN = C.CFUNCTYPE(C.c_int32, C.c_void_p)

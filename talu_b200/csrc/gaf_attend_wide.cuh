@@ -1,10 +1,12 @@
 // Attention over the quantised KV cache on tcgen05, for many query rows per cached head (prompts, shared prefixes).
 //
 // Mathematics.  Keys and values are dequantised to f16, 32 keys at a time with one power of two that brings their largest
-// magnitude to 2^14..2^15: 11 bits of every element that is within 2^-29 of that.  bf16 would hold any range as it is, but its
-// 8 bits on keys and values alone put the result 3e-3 off; f16 leaves them at 2^-12.
+// magnitude to 2^14..2^15.  bf16 would hold any range as it is, but its 8 bits on keys and values alone put the result 3e-3
+// off; f16 rounds the centre of a group and the element itself, 2^-11 of each (an element that is small beside its group's centre is
+// off by 2^-11 of the centre), and loses what is below 2^-39 of the largest magnitude.
 //   w 2^-e = (c - h) (s 2^-e) + (b + h s) 2^-e,   h = 2^(bits - 1): the centred code and s 2^-e are exact in f16
-// q is f16 with a power of two per row (exact), the weights are f16 (2^-12 of each), all statistics and sums f32.  The keys'
+// q is f16 with a power of two per row (exact), the weights are f16 (2^-11 of each), all statistics and sums f32.  Scores thus carry
+// 2^-11 of each key element, which those of the register path do not.  The keys'
 // power goes into the scores' factor, the values' into the weights: they are formed as 2^(y + e - m) (y: scores in base
 // 2), where m follows the largest y + e instead of the largest y, and leave it again in the row's sum.
 //
@@ -20,8 +22,8 @@
 // The reference is an integer and follows lazily: a row's largest weight is brought to 2^6 to 2^7 and rescaled (O, and the weights of
 // the unit that are formed already: exactly) when it exceeds 2^15, so that weights keep their 11 bits down to 2^-20 of the largest and
 // have a step of 2^-30 of it below.  (With 2^0 in place of 2^7, 40000 keys of 2^-22 each behind one key whose values are zero were
-// 15 % off; 2^10 costs 4 %, 2^12 11 % more time.)  A row's thread takes 32 scores at a time, the next 32 on
-// their way, and puts their weights into columns whose scores it has read.  Measured on a chunk of two prompts (768 and
+// 15 % off; 2^10 costs 4 %, 2^12 11 % more time.)  A row's thread takes 32 scores at a time
+// and puts their weights into columns whose scores it has read.  Measured on a chunk of two prompts (768 and
 // 1024 new tokens over 3750 and 5000 cached ones, 32 heads on 8): 216 us; 262 with a pass of its own for the maximum,
 // 256 with that and two threads a row, 334 with two buffers of 64 keys for the scores (twice the MMAs, of half the
 // width: the issuing warp does not keep up), 387 with everything unrolled (instruction cache).
@@ -102,16 +104,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
                  : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
-        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-          "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-          "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
-        : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
