@@ -331,8 +331,12 @@ int32_t tgaf_kv_read(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_se
 /* out[t, h] = sum_j softmax_j(scale * q[t, h] . K[j, h / (q_heads / kv_heads)]) V[j, ...] over the cached tokens j of t's
  * sequence up to t itself (causal; the sequence's tokens are appended first).  q, out: f32 or bf16
  * [total, q_heads, head_dim], strides in elements, head_dim contiguous; out must not overlap q.  f32 statistics and sums.
- * max_new: an upper bound of the own tokens of any sequence (the launch is sized by it; a sequence with more sets the
- * error word and its rows from max_new on are left as they were).  A row that sees no key gives 0.
+ * max_new: an upper bound of the own tokens of any sequence (the launch is sized by it, and it decides which kernel takes the
+ * call, so a close one is best; a sequence with more sets the error word and its rows from max_new on are left as they were).
+ * A row that sees no key gives 0; a row of q that is not finite gives NaN where it sees one.
+ * Roundings beside f32: bf16 calls round weights to f16 (2^-11 of each); those that go to the tcgen05 kernel (more than 8 to 32
+ * rows of a cached head and sequence) round keys and values to f16 as well, so that their scores are off by up to
+ * 2^-11 sum |q k|.  f32 calls hold q and weights in two f16 terms (22 bits).  Heads of other sizes than 64 and 128: f32 throughout.
  * The partial results of long sequences lie in a workspace of the context, made with its first cache (or by its first call,
  * where the cache is another context's; such a call cannot be captured): calls captured into
  * graphs must not be replayed at the same time as other attention calls of the same context (one context per stream). */
@@ -341,7 +345,8 @@ int32_t tgaf_attention(tgaf_ctx *ctx, const tgaf_kv_cache *cache, const tgaf_kv_
                        void *out, uint64_t out_token_stride, uint64_t out_head_stride);
 /* The same where every sequence continues one shared prefix of prefix_len tokens, in the pages d_prefix_table
  * i32 [ceil(prefix_len / page_tokens)]: every row sees the whole prefix, then its own sequence's tokens as above (d_lens and
- * d_table do not count the prefix).  The prefix is read once for all rows of the batch instead of once per sequence.
+ * d_table do not count the prefix).  With heads of 64 or 128 the prefix is read once for 256 rows of a cached head (at most 32 in
+ * small calls, 16 in f32) instead of once per sequence; other head sizes read it for every row.
  * The rows' results against the prefix, total * q_heads * (head_dim + 1) f32, lie in a workspace of the context: 8 MB from its
  * first cache on, and at least doubled by the first call that needs more, which waits for the context's stream and allocates
  * (refused in a capture).  Blocks that captured calls have used are kept until the context ends. */

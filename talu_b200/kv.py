@@ -45,14 +45,15 @@ def _tag(name: str, dtype) -> int:
 
 def _count(name: str, value, least: int = 0, most: int = 2 ** 32 - 1) -> int:
     """An integer that the C entry takes as it is: ctypes would drop the bits above 32, and a sign."""
+    if type(value) is int and least <= value <= most:
+        return value
     if isinstance(value, bool) or not hasattr(value, "__index__") or not least <= value.__index__() <= most:
         _refuse(f"{name} must be an integer from {least} to {most}, got {value!r}")
     return value.__index__()
 
 
-def _of_device(ctx: Context, cache: KvCache):
-    if cache.ctx.device != ctx.device:
-        _refuse(f"the cache is on cuda:{cache.ctx.device}, the context on cuda:{ctx.device}")
+def _other_device(ctx: Context, cache: KvCache):
+    _refuse(f"the cache is on cuda:{cache.ctx.device}, the context on cuda:{ctx.device}")
 
 
 def _rows(ctx: Context, name: str, t, heads: int, head_dim: int, written: bool = False):
@@ -164,7 +165,8 @@ def _seqs(ctx: Context, table, lens, cu, total: int) -> _capi.KvSeqs:
 def kv_append(ctx: Context, cache: KvCache, k, v, table, lens, cu=None) -> None:
     """Quantises the call's own rows k, v [tokens, kv_heads, head_dim] (bf16 or f32, any token and head strides) into the
     sequences' pages (tgaf_kv_append).  lens counts them already; without cu every sequence has tokens / batch of them."""
-    _of_device(ctx, cache)
+    if cache.ctx.device != ctx.device:
+        _other_device(ctx, cache)
     tag = _tag("k", k.dtype)
     total, k_args = _rows(ctx, "k", k, cache.kv_heads, cache.head_dim)
     v_rows, v_args = _rows(ctx, "v", v, cache.kv_heads, cache.head_dim)
@@ -182,7 +184,8 @@ def kv_read(ctx: Context, cache: KvCache, table, lens, cu=None, total: int | Non
     are cu = cumulated lens.  Rows that lie in no sequence are left as they were (undefined in new tensors)."""
     if _BF16 is None:
         _torch()
-    _of_device(ctx, cache)
+    if cache.ctx.device != ctx.device:
+        _other_device(ctx, cache)
     if out is None:
         if total is None:
             _refuse("total (or out) is needed")
@@ -206,7 +209,8 @@ def kv_read(ctx: Context, cache: KvCache, table, lens, cu=None, total: int | Non
 
 
 def _attend(ctx: Context, cache: KvCache, q, prefix_at, prefix_len: int, table, lens, cu, max_new, scale, out):
-    _of_device(ctx, cache)
+    if cache.ctx.device != ctx.device:
+        _other_device(ctx, cache)
     tag = _tag("q", q.dtype)
     heads, head_dim = q.shape[1] if q.dim() == 3 else 0, cache.head_dim
     if heads == 0 or heads % cache.kv_heads:
@@ -243,15 +247,17 @@ def attention(ctx: Context, cache: KvCache, q, table, lens, cu=None, max_new=Non
 
     q: [tokens, heads, head_dim], bf16 or f32, any token and head strides; heads / kv_heads query heads share a cached head.
     The tokens' own K / V rows are appended first (`lens` counts them).  max_new: an upper bound of the own tokens of any
-    sequence (the launch is sized by it), needed with cu.  scale: default 1 / sqrt(head_dim).  Rows that see no key are 0."""
+    sequence, needed with cu: the launch is sized by it, and it decides which kernel takes the call, so a close one is best.
+    scale: default 1 / sqrt(head_dim).  Rows that see no key are 0.  `out` must not overlap q."""
     return _attend(ctx, cache, q, None, 0, table, lens, cu, max_new, scale, out)
 
 
 def attention_shared_prefix(ctx: Context, cache: KvCache, q, prefix_table, prefix_len: int, table, lens, cu=None, max_new=None,
                             scale=None, out=None):
     """`attention` for sequences that all continue one shared prefix of `prefix_len` tokens in the pages `prefix_table`
-    (int32 [pages], on the device); table and lens do not count the prefix.  Its pages are read once for the whole batch
-    (tgaf_attention_shared_prefix).  Calls of more than some 16 k rows (tokens x heads of 128): see `attention_reserve`."""
+    (int32 [pages], on the device); table and lens do not count the prefix (tgaf_attention_shared_prefix).  Its pages are read
+    once for 256 rows of a cached head (at most 32 in small calls, 16 in f32) instead of once per sequence; head sizes other
+    than 64 and 128 read them for every row.  Calls of more than some 16 k rows (tokens x heads of 128): see `attention_reserve`."""
     _tag("q", q.dtype)
     if prefix_table.dtype is not _I32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous():
         _refuse(f"prefix_table must be contiguous int32 [pages], got {prefix_table.dtype} {tuple(prefix_table.shape)}")
@@ -266,6 +272,7 @@ def attention_shared_prefix(ctx: Context, cache: KvCache, q, prefix_table, prefi
 def attention_reserve(ctx: Context, cache: KvCache, rows: int) -> None:
     """Makes the context's workspace large enough for `attention_shared_prefix` calls of up to `rows` = tokens x heads rows
     (tgaf_attention_reserve): in front of a capture of such calls, or so that the first of them need not wait for it."""
-    _of_device(ctx, cache)
+    if cache.ctx.device != ctx.device:
+        _other_device(ctx, cache)
     rows = _count("rows", rows, 0, 2 ** 31 - 1)
     ctx._check(ctx._lib.tgaf_attention_reserve(ctx._h, cache._h, rows))
