@@ -15,8 +15,8 @@
 // each group have a factor of their own per row, which keeps the largest of them between 2^4 and 2^15.  So a group whose
 // scales are far below its neighbours' has weights of as many bits, and a weight loses some only below 2^-18 of the group's
 // largest one, where its step is 2^-28 of that.  (With one factor for all groups, from the largest scale of each key, a group
-// 2^20 below it was 1.6e-3 off in f32.  A factor per group costs nothing per unit, but 0.3 to 1 us where a segment begins: 16
-// sequences of 2500 tokens, 32 heads on 8, 8 bits: 24.8 -> 26.2 us, f32 28.8 -> 30.4.)
+// 2^20 below it was 1.6e-3 off in f32.  A factor per group costs some 1 % per unit, 0.3 to 1 us where a segment begins: 16
+// sequences of 2560 tokens, 32 heads on 8, 8 bits: 24.8 -> 25.4 us, f32 28.5 -> 29.5.)
 // LIMBS = 2 (f32 q): q and p s are split into two f16 terms each (22 bits).
 //
 // Both products are formed transposed (keys as the 16 rows of the MMA's A operand, query rows as its 8 columns): with one
@@ -723,7 +723,7 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
 #pragma unroll
                 for (int j = 0; j < NP; ++j) qsum[nt][c][j] = s_qsum[nt * 8 + 2 * t + c][j];
             }
-        for (int x = lane; x < R * (GS + 1); x += 32) factor[x] = x < R * GS ? pow2_or_0(126) : 0.0f;     // of no weights yet
+        for (int x = lane; x < R * GS; x += 32) factor[x] = 0.0f;     // until the first unit: the largest products
         __syncwarp();
         float most_scale[GS];    // a power of two above the warp's scales of the segment so far; 0: none
 #pragma unroll
@@ -837,22 +837,21 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
 #pragma unroll
                 for (int c = 0; c < 4; ++c) grow |= z[nt][c] > ((c & 1) ? most.y : most.x);
             }
-            if (__any_sync(0xFFFFFFFFu, grow)) {
+            if (fresh || __any_sync(0xFFFFFFFFu, grow)) {
                 // the largest finite scales of the warp's keys so far, rounded up to a power of two
-                float scale[GS];
 #pragma unroll
                 for (int i = 0; i < GS; ++i) {
-                    const float x = fabsf(va[i]), y = fabsf(vb[i]);
-                    scale[i] = fmaxf(x <= 3.4e38f ? x : 0.0f, y <= 3.4e38f ? y : 0.0f);
+                    const uint32_t x = __float_as_uint(va[i]) & 0x7FFFFFFFu, y = __float_as_uint(vb[i]) & 0x7FFFFFFFu;
+                    const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(x < 0x7F800000u ? x : 0u, y < 0x7F800000u ? y : 0u));
+                    most_scale[i] = fmaxf(most_scale[i], __uint_as_float((top & 0x7F800000u) + 0x00800000u));
                 }
-#pragma unroll
-                for (int x = 4; x <= 16; x <<= 1)
-#pragma unroll
-                    for (int i = 0; i < GS; ++i) scale[i] = fmaxf(scale[i], __shfl_xor_sync(0xFFFFFFFFu, scale[i], x));
-#pragma unroll
-                for (int i = 0; i < GS; ++i)
-                    most_scale[i] = fmaxf(most_scale[i], __uint_as_float((__float_as_uint(scale[i]) & 0x7F800000u) + 0x00800000u));
-                // `kFirst`: nothing is summed yet (and code that runs once a segment comes from far: no more of it than needed)
+                // 2^(kTarget - floor(log2 most)), at most 2^126
+                auto fitting = [](float most) { return min(((254u + kTarget) << 23) - (__float_as_uint(most) & 0x7F800000u), 253u << 23); };
+                // scores above the reference by that, and no more, keep all products in range; reach: a group's factor times its largest scale
+                auto room = [](float reach) { return fminf(kLazy, static_cast<float>(kMostExp + 127 - static_cast<int>(__float_as_uint(reach) >> 23))); };
+                // kFirst: nothing is summed yet.  Code that runs once a segment comes from far, so there is no more of it than needed: the
+                // groups' largest products by atomics in the array of the factors, instead of 6 instructions for each in every lane (a
+                // shared prefix of 1111 tokens for five sequences: 37.5 us, 38.9 with those)
                 auto settle = [&](auto first_tag) {
                     constexpr bool kFirst = decltype(first_tag)::value;
 #pragma unroll
@@ -875,8 +874,12 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                             // the groups' largest products; a scale that is not finite counts for nothing or for the most
                             const float pa = exp2_approx(y[c] - next), pb = exp2_approx(y[2 + c] - next);
 #pragma unroll
-                            for (int i = 0; i < GS; ++i) most[c][i] = fmaxf(pa == 0.0f ? 0.0f : pa * fabsf(va[i]), pb == 0.0f ? 0.0f : pb * fabsf(vb[i]));
+                            for (int i = 0; i < GS; ++i) {
+                                most[c][i] = fmaxf(fmaxf(pa * fabsf(va[i]), pb * fabsf(vb[i])), 0.0f);
+                                if (kFirst) atomicMax(reinterpret_cast<unsigned int *>(factor + i * R + nt * 8 + 2 * t + c), __float_as_uint(most[c][i]));
+                            }
                         }
+                        if (kFirst) continue;
 #pragma unroll
                         for (int x = 4; x <= 16; x <<= 1)
 #pragma unroll
@@ -888,35 +891,38 @@ gaf_attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUte
                             float set[2];
 #pragma unroll
                             for (int c = 0; c < 2; ++c) {
-                                // 2^(kTarget - floor(log2 most)), at most 2^126
-                                const uint32_t fit = min(((254u + kTarget) << 23) - (__float_as_uint(most[c][i]) & 0x7F800000u), 253u << 23);
-                                set[c] = __uint_as_float(fit);
-                                if (!kFirst) {
-                                    // the sums' present unit is 2^-have; it is kept while the products stay below 2^(kTarget + 8)
-                                    const int have = static_cast<int>(__float_as_uint(at[c]) >> 23) - 127 + static_cast<int>(up[c]), aim = static_cast<int>(fit >> 23) - 127;
-                                    const int want = have >= aim + 8 ? aim : min(have, 126);
-                                    const float ratio = pow2_or_0(want - have);
-                                    set[c] = pow2_or_0(want);
+                                const uint32_t fit = fitting(most[c][i]);
+                                // the sums' present unit is 2^-have; it is kept while the products stay below 2^(kTarget + 8)
+                                const int have = static_cast<int>(__float_as_uint(at[c]) >> 23) - 127 + static_cast<int>(up[c]), aim = static_cast<int>(fit >> 23) - 127;
+                                const int want = have >= aim + 8 ? aim : min(have, 126);
+                                const float ratio = pow2_or_0(want - have);
+                                set[c] = pow2_or_0(want);
 #pragma unroll
-                                    for (int k = i * (GROUP / 16); k < (i + 1) * (GROUP / 16); ++k) o[k][nt][c] *= ratio, o[k][nt][2 + c] *= ratio;
-                                }
+                                for (int k = i * (GROUP / 16); k < (i + 1) * (GROUP / 16); ++k) o[k][nt][c] *= ratio, o[k][nt][2 + c] *= ratio;
                                 reach[c] = fmaxf(reach[c], set[c] * most_scale[i]);
                             }
-                            if (!kFirst) __syncwarp();       // the row's lanes have read it
+                            __syncwarp();       // the row's lanes have read it
                             if (g == 0) *reinterpret_cast<float2 *>(at) = make_float2(set[0], set[1]);
                         }
-                        float room[2];                       // scores above the reference by that, and no more, keep all products in range
+                        if (g == 0) *reinterpret_cast<float2 *>(limit + nt * 8 + 2 * t) = make_float2(room(reach[0]), room(reach[1]));
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) room[c] = fminf(kLazy, static_cast<float>(kMostExp + 127 - static_cast<int>(__float_as_uint(reach[c]) >> 23)));
-                        if (g == 0) *reinterpret_cast<float2 *>(limit + nt * 8 + 2 * t) = make_float2(room[0], room[1]);
-                        if (!kFirst) {
+                        for (int c = 0; c < 2; ++c) {
+                            const float keep = pow2_or_0(-static_cast<int>(up[c]));
+                            l[nt][c] *= keep;
 #pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                const float keep = pow2_or_0(-static_cast<int>(up[c]));
-                                l[nt][c] *= keep;
+                            for (int i = 0; i < GS; ++i) bsum[nt][c][i] *= keep;
+                        }
+                    }
+                    if (kFirst) {
+                        // the array held the largest products: a lane for each
+                        __syncwarp();
+                        for (int x = lane; x < R * GS; x += 32) factor[x] = __uint_as_float(fitting(factor[x]));
+                        __syncwarp();
+                        if (lane < R) {
+                            float reach = 0.0f;
 #pragma unroll
-                                for (int i = 0; i < GS; ++i) bsum[nt][c][i] *= keep;
-                            }
+                            for (int i = 0; i < GS; ++i) reach = fmaxf(reach, factor[i * R + lane] * most_scale[i]);
+                            limit[lane] = room(reach);
                         }
                     }
                 };
