@@ -494,10 +494,11 @@ cudaError_t attention_generic(const AttnArgs &a, bool f32, cudaStream_t stream) 
 // Its time grows with the rows, the tcgen05 kernel's hardly does; with fewer items than SMs every item is cut across many CTAs,
 // and the larger units of the tcgen05 kernel leave fewer parts to join.  Measured (8 cached heads, 8 bits; register path
 // against tcgen05, us), 24 sequences of 3000 tokens, then 4 of 800:
-//   heads of 128   16 rows 61 / 111, 33 / 27    24 rows 106 / 112, 47 / 27    32 rows 168 / 112, 65 / 27
-//   heads of 64    16 rows 36 / 90, 21 / 22     24 rows 43 / 90, 28 / 22      32 rows 54 / 91, 36 / 22
+//   heads of 128   12 rows 61 / 113, 30 / 27    16 rows 63 / 114, 33 / 27    24 rows 110 / 114, 47 / 28    (32 rows: 168 / 112, 65 / 27)
+//   heads of 64    12 rows 37 / 90, 21 / 22     16 rows 37 / 90, 21 / 22     24 rows 44 / 90, 28 / 22      32 rows 55 / 91, 37 / 22
 // (times of captured calls; the tcgen05 kernel's joining pass is a launch of its own, some 4 us more where launches follow one
-// another from the host, which decides for 16 rows against a shared prefix: 35 against 39 us for one of 1111 tokens.)
+// another from the host, which decides for 16 rows against a shared prefix: 38 against 40 us for one of 1111 tokens.  With 4 bits:
+// heads of 128 16 rows 62 / 112, 24 rows 87 / 114; otherwise the same.)
 uint64_t narrow_rows(uint32_t head_dim, uint64_t items, bool prefix, int sm_count) {
     const bool few = items < static_cast<uint64_t>(sm_count);
     return head_dim == 128u ? (!few ? 24u : prefix ? 16u : 8u) : (few ? 16u : 32u);
