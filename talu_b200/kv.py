@@ -201,6 +201,8 @@ def kv_read(ctx: Context, cache: KvCache, table, lens, cu=None, total: int | Non
         v_rows, v_args = _rows(ctx, "out v", v, cache.kv_heads, cache.head_dim, True)
         if v.dtype is not k.dtype or v_rows != rows or (total is not None and total != rows):
             _refuse("out k and v must have one dtype and `total` rows")
+        if k_args[0] == v_args[0] and rows:
+            _refuse("out k and v must not be one tensor")
         seqs = _seqs(ctx, table, lens, cu, rows)
     st = ctx._lib.tgaf_kv_read(ctx._h, cache._h, seqs, tag, *k_args, *v_args)
     if st:

@@ -282,3 +282,12 @@ def test_calls_right_behind_a_reported_error():
     assert all(torch.equal(out, outs[0]) for out in outs)
     cache.free()
     own.close()
+
+
+def test_one_tensor_for_keys_and_values_is_refused(fake):  # noqa: F811
+    """Read back into one place, keys and values would overwrite each other in no order."""
+    from talu_b200 import GafError, kv_read
+    x, table, lens = _args()
+    with pytest.raises(GafError) as e:
+        kv_read(fake.ctx, fake, table, lens, out=(x, x))
+    assert e.value.invalid_argument and "one tensor" in e.value.message
