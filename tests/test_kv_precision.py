@@ -156,3 +156,29 @@ def test_small_values(ctx, dtype, new, v_size):  # noqa: F811
     for t in (cache.scales, cache.biases):
         t[table[1, ::2].long(), 1] *= 1 / v_size
     check(ctx, cache, q, table, lens, cumulate([new, new]), wide, top=6 if wide else 4)
+
+
+@gpu
+@pytest.mark.parametrize("dtype, new", [(torch.bfloat16, 1), (torch.bfloat16, 30), (torch.float32, 2)])
+@pytest.mark.parametrize("dim, bits, group", [(64, 8, 32), (128, 4, 64), (128, 8, 128), (96, 8, 32)])
+@pytest.mark.parametrize("prefix", [1, 333])
+def test_shared_prefix_to_the_bound(ctx, dtype, new, dim, bits, group, prefix):  # noqa: F811
+    """Prefix and own pass together, groups of different size in both, rows that see the prefix alone."""
+    lens, news, kv_heads, per_kv = [300, 0, 31, 64], [new, 2, min(31, new), new], 2, 3
+    table, pages, _ = make_tables(lens + [prefix], 32, 1)
+    cache = filled_cache(ctx, pages, kv_heads, dim, 32, bits, group)
+    scaled_groups(cache, table, lens + [prefix], 3, True)
+    cu = cumulate(news)
+    q = torch.randn(cu[-1], kv_heads * per_kv, dim, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(dtype)
+    most = max(news) * per_kv
+    wide = [kv_bounds.takes_wide(q, cache, most, len(lens)), kv_bounds.takes_wide(q, cache, cu[-1] * per_kv, 1, True)]
+    head = table[-1, :-(-prefix // 32)].contiguous()
+    kw = dict(prefix_table=head, prefix_len=prefix)
+    if all(wide) or not any(wide):
+        check(ctx, cache, q, table[:-1], lens, cu, wide[0], top=6 if wide[0] else 4, **kw)
+    else:                                   # one pass on either kernel: off by the sum of both bounds at most
+        import talu_b200 as gaf
+        out = gaf.attention_shared_prefix(ctx, cache, q, head, prefix, table[:-1], dev(lens), cu=dev(cu), max_new=max(news))
+        ctx.synchronize()
+        (want, a), (_, b) = (kv_bounds.attention(cache, q, table[:-1], lens, cu, w, top=4, **kw) for w in (True, False))
+        assert worst(out, want, a + b) <= 1.0
